@@ -25,6 +25,7 @@ MG_ETIMEOUT = 6
 
 MG_DTYPE_F32 = 0
 MG_DTYPE_BF16 = 1
+MG_DTYPE_E4M3 = 2
 
 MG_OUT_HIDDEN = 0
 MG_OUT_LOGITS_ALL = 1
@@ -113,6 +114,41 @@ class Profile(ctypes.Structure):
                    "launches": int(self.launches[i])}
             for i, name in enumerate(PROF_NAMES)
         }
+
+
+class PagedPool(ctypes.Structure):
+    _fields_ = [
+        ("k", _vp),
+        ("v", _vp),
+        ("k_scale", _vp),
+        ("v_scale", _vp),
+        ("k_page_stride", _i64),
+        ("k_head_stride", _i64),
+        ("k_token_stride", _i64),
+        ("v_page_stride", _i64),
+        ("v_head_stride", _i64),
+        ("v_token_stride", _i64),
+        ("k_scale_stride", _i64),
+        ("v_scale_stride", _i64),
+        ("num_pages", _i32),
+        ("page_size", _i32),
+        ("num_kv_heads", _i32),
+        ("head_dim", _i32),
+        ("cache_dtype", _i32),
+    ]
+
+
+class PagedBatch(ctypes.Structure):
+    _fields_ = [
+        ("page_table", _vp),
+        ("q_start", _vp),
+        ("kv_len", _vp),
+        ("table_stride", _i64),
+        ("batch", _i32),
+        ("tokens", _i32),
+        ("max_pages", _i32),
+        ("max_new", _i32),
+    ]
 
 
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
@@ -215,3 +251,14 @@ SIGNATURES["mg_linear_noalloc"] = (
     ctypes.c_int,
     [_i32, _vp, _i64, _vp, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _i64, _vp],
 )
+_pool, _batch = ctypes.POINTER(PagedPool), ctypes.POINTER(PagedBatch)
+SIGNATURES["mg_paged_append"] = (
+    ctypes.c_int,
+    [_pool, _batch, _i32, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _f32, _vp, _i64, _vp],
+)
+SIGNATURES["mg_paged_attention"] = (
+    ctypes.c_int,
+    [_pool, _batch, _i32, _vp, _i64, _i64, _i32, _f32, _vp, _i64, _i64, _vp, ctypes.c_uint64, _vp],
+)
+SIGNATURES["mg_paged_attention_workspace"] = (ctypes.c_uint64, [_pool, _batch, _i32, _i32])
+SIGNATURES["mg_paged_check_device"] = (ctypes.c_int, [_vp])

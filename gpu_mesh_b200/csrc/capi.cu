@@ -25,6 +25,7 @@
 #include "common.cuh"
 #include "kernels.h"
 #include "linear_tc.h"
+#include "paged.h"
 #include "tc_common.cuh"
 #include "meshgpu_b200.h"
 
@@ -1327,3 +1328,169 @@ extern "C" int mg_linear_noalloc(int32_t dtype, const void* X, int64_t ldx, cons
   return mg_linear(dtype, X, ldx, W, M, N, K, epilogue, R, ldr, Y, ldy, (float*)scratch,
                    kNoAllocScratch, stream);
 }
+
+// ---------------------------------------------------------------------------
+// Paged KV cache.
+// ---------------------------------------------------------------------------
+namespace {
+
+static __device__ int g_paged_err;
+SymbolCache g_paged_err_addr;
+
+int paged_err_word(void* stream, int** err) {
+  void* p = nullptr;
+  const int rc = symbol_address(g_paged_err_addr, (const void*)&g_paged_err, (cudaStream_t)stream, &p,
+                                "cudaGetSymbolAddress(paged error word)");
+  *err = (int*)p;
+  return rc;
+}
+
+bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
+
+// The checks that both operators share; fills the kernels' own forms.
+int paged_args(const mg_paged_pool* p, const mg_paged_batch* b, int32_t dtype, int32_t nq, PagedPool* pool,
+               PagedBatch* batch) {
+  if (!p || !b) return fail(MG_EINVAL, "null pool or batch");
+  if (dtype != MG_DTYPE_F32 && dtype != MG_DTYPE_BF16) return fail(MG_EINVAL, "dtype must be fp32 or bf16");
+  if (p->cache_dtype != dtype && p->cache_dtype != MG_DTYPE_E4M3)
+    return fail(MG_EINVAL, "the pages must hold the activation dtype or e4m3");
+  if (!p->k || !p->v) return fail(MG_EINVAL, "null pages");
+  const int ps = p->page_size, D = p->head_dim;
+  if (ps != 16 && ps != 32 && ps != 64 && ps != 128)
+    return fail(MG_EINVAL, "page_size must be 16, 32, 64 or 128 (got %d)", ps);
+  if (D != 8 && D != 16 && D != 32 && D != 64 && D != 128)
+    return fail(MG_EINVAL, "head_dim must be one of 8, 16, 32, 64, 128 (got %d)", D);
+  if (p->num_pages < 1 || p->num_kv_heads < 1) return fail(MG_EINVAL, "num_pages and num_kv_heads must be positive");
+  if (nq < 1 || nq % p->num_kv_heads != 0 || nq / p->num_kv_heads > 16)
+    return fail(MG_EINVAL, "num_q_heads must be 1 to 16 times num_kv_heads (%d and %d)", nq, p->num_kv_heads);
+  const bool e4m3 = p->cache_dtype == MG_DTYPE_E4M3;
+  if (e4m3 && (!p->k_scale || !p->v_scale)) return fail(MG_EINVAL, "e4m3 pages need k_scale and v_scale");
+  if (e4m3 && (p->k_scale_stride < p->num_kv_heads || p->v_scale_stride < p->num_kv_heads))
+    return fail(MG_EINVAL, "scale rows must hold num_kv_heads entries");
+  const int esz = e4m3 ? 1 : dtype == MG_DTYPE_BF16 ? 2 : 4;
+  const int64_t unit = std::min(16, D * esz) / esz;  // elements that a row starts on a multiple of
+  const int64_t st[] = {p->k_page_stride, p->k_head_stride, p->k_token_stride,
+                        p->v_page_stride, p->v_head_stride, p->v_token_stride};
+  for (int64_t x : st)
+    if (x < D || x % unit) return fail(MG_EINVAL, "page, head and token strides must be at least head_dim and multiples of 16 bytes");
+  if ((uintptr_t)p->k % (unit * esz) || (uintptr_t)p->v % (unit * esz))
+    return fail(MG_EINVAL, "pages must start on 16-byte boundaries");
+  if (b->batch < 0 || b->tokens < 0 || b->max_new < 0) return fail(MG_EINVAL, "negative batch, tokens or max_new");
+  if (b->batch > kPagedMaxBatch) return fail(MG_EINVAL, "at most %d sequences per call (got %d)", kPagedMaxBatch, b->batch);
+  if (b->batch > 0 && b->tokens > 0) {
+    if (!b->page_table || !b->q_start || !b->kv_len) return fail(MG_EINVAL, "null page_table, q_start or kv_len");
+    if (b->max_pages < 1 || (int64_t)b->max_pages * ps > INT32_MAX)
+      return fail(MG_EINVAL, "the table's columns must hold 1 to 2^31 - 1 tokens");
+    if (b->batch > 1 && b->table_stride < b->max_pages) return fail(MG_EINVAL, "table_stride is below max_pages");
+  }
+  *pool = PagedPool{p->k, p->v, p->k_scale, p->v_scale,
+                    p->k_page_stride, p->k_head_stride, p->k_token_stride,
+                    p->v_page_stride, p->v_head_stride, p->v_token_stride,
+                    p->k_scale_stride, p->v_scale_stride,
+                    p->num_pages, ps, p->num_kv_heads, D, p->cache_dtype};
+  *batch = PagedBatch{b->page_table, b->table_stride, b->max_pages, b->q_start, b->kv_len, b->batch, b->tokens,
+                      std::min(b->max_new, b->tokens)};
+  return MG_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int mg_paged_append(const mg_paged_pool* pool, const mg_paged_batch* batch, int32_t dtype, const void* qkv,
+                    int64_t ld_qkv, int32_t num_q_heads, const int64_t* positions, const float* cos,
+                    const float* sin, int32_t max_pos, const void* q_norm, const void* k_norm, float eps,
+                    void* q_out, int64_t ld_q, void* stream) {
+  PagedAppendArgs a{};
+  int rc = paged_args(pool, batch, dtype, num_q_heads, &a.pool, &a.batch);
+  if (rc) return rc;
+  if (a.batch.B == 0 || a.batch.T == 0) return MG_OK;
+  if (!qkv || !q_out) return fail(MG_EINVAL, "null qkv or q_out");
+  const int64_t vec = dtype == MG_DTYPE_BF16 ? 8 : 4, D = a.pool.D;
+  if (ld_qkv < (num_q_heads + 2LL * a.pool.nkv) * D || ld_qkv % vec || ld_q < num_q_heads * D || ld_q % vec)
+    return fail(MG_EINVAL, "qkv and q_out rows must hold every head and be multiples of 16 bytes apart");
+  if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(q_norm) || !aligned16(k_norm) || !aligned16(cos) || !aligned16(sin))
+    return fail(MG_EINVAL, "qkv, q_out, the norm weights and the tables must start on 16-byte boundaries");
+  if (!cos != !sin) return fail(MG_EINVAL, "cos and sin come together");
+  if (cos && max_pos < 1) return fail(MG_EINVAL, "the rotary tables are empty");
+  if ((q_norm || k_norm) && !(eps > 0.f)) return fail(MG_EINVAL, "eps must be positive");
+  rc = paged_err_word(stream, &a.err);
+  if (rc) return rc;
+  a.dtype = dtype;
+  a.qkv = qkv;
+  a.ldqkv = ld_qkv;
+  a.nq = num_q_heads;
+  a.positions = positions;
+  a.cos = cos;
+  a.sin = sin;
+  a.max_pos = max_pos;
+  a.q_norm = q_norm;
+  a.k_norm = k_norm;
+  a.eps = eps;
+  a.q_out = q_out;
+  a.ldq = ld_q;
+  MG_LAUNCH(launch_paged_append(a, (cudaStream_t)stream), "paged append");
+  return MG_OK;
+}
+
+uint64_t mg_paged_attention_workspace(const mg_paged_pool* pool, const mg_paged_batch* batch, int32_t dtype,
+                                      int32_t num_q_heads) {
+  PagedAttnArgs a{};
+  if (paged_args(pool, batch, dtype, num_q_heads, &a.pool, &a.batch) || a.batch.B == 0 || a.batch.T == 0) return 0;
+  a.dtype = dtype;
+  a.nq = num_q_heads;
+  return paged_attention_workspace(a);
+}
+
+int mg_paged_attention(const mg_paged_pool* pool, const mg_paged_batch* batch, int32_t dtype, const void* q,
+                       int64_t q_token_stride, int64_t q_head_stride, int32_t num_q_heads, float scale, void* out,
+                       int64_t out_token_stride, int64_t out_head_stride, void* workspace, uint64_t workspace_bytes,
+                       void* stream) {
+  PagedAttnArgs a{};
+  int rc = paged_args(pool, batch, dtype, num_q_heads, &a.pool, &a.batch);
+  if (rc) return rc;
+  if (!(scale > 0.f) || scale > 3.402823466e38f) return fail(MG_EINVAL, "scale must be positive and finite");
+  if (a.batch.B == 0 || a.batch.T == 0) return MG_OK;
+  if (!q || !out) return fail(MG_EINVAL, "null q or out");
+  const int64_t vec = dtype == MG_DTYPE_BF16 ? 8 : 4, D = a.pool.D;
+  for (int64_t x : {q_token_stride, q_head_stride, out_token_stride, out_head_stride})
+    if (x < D || x % vec)
+      return fail(MG_EINVAL, "token and head strides of q and out must be at least head_dim and multiples of 16 bytes");
+  if (!aligned16(q) || !aligned16(out)) return fail(MG_EINVAL, "q and out must start on 16-byte boundaries");
+  a.dtype = dtype;
+  a.nq = num_q_heads;
+  const uint64_t need = paged_attention_workspace(a);
+  if (workspace_bytes < need || (need && (!workspace || (uintptr_t)workspace % 256)))
+    return fail(MG_EINVAL, "the workspace must be 256-byte aligned and hold %llu bytes", (unsigned long long)need);
+  rc = paged_err_word(stream, &a.err);
+  if (rc) return rc;
+  a.q = q;
+  a.ldq = q_token_stride;
+  a.hdq = q_head_stride;
+  a.scale = scale;
+  a.out = out;
+  a.ldo = out_token_stride;
+  a.hdo = out_head_stride;
+  a.ws = workspace;
+  a.ws_bytes = workspace_bytes;
+  MG_LAUNCH(launch_paged_attention(a, (cudaStream_t)stream), "paged attention");
+  return MG_OK;
+}
+
+int mg_paged_check_device(void* stream) {
+  int* err = nullptr;
+  int rc = paged_err_word(stream, &err);
+  if (rc) return rc;
+  int h = 0;
+  MG_CUDA(cudaMemcpyAsync(&h, err, sizeof(int), cudaMemcpyDeviceToHost, (cudaStream_t)stream),
+          "paged error word read");
+  MG_CUDA(cudaStreamSynchronize((cudaStream_t)stream), "paged error word sync");
+  if (h == kErrNone) return MG_OK;
+  MG_CUDA(cudaMemsetAsync(err, 0, sizeof(int), (cudaStream_t)stream), "paged error word reset");
+  if (h == kErrPaged)
+    return fail(MG_EDEVICE, "a paged call met a page id, length or token range outside its pool, table or batch");
+  if (h == kErrPositionRange) return fail(MG_EDEVICE, "a paged append met a position outside its rotary tables");
+  return fail(MG_ETIMEOUT, "a paged launch gave up waiting for its data (code %d); its output is invalid", h);
+}
+
+}  // extern "C"

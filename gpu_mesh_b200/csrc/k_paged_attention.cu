@@ -1,0 +1,279 @@
+// Attention over a paged KV cache on the CUDA cores: every type, head size
+// and group that the pool can hold, and the launch rule between this kernel
+// and the tensor-core ones.
+//
+//   out[t, h] = Σ_j softmax_j(scale · q[t, h]·K[j]) V[j],   j <= past + s
+// for the s-th new token t of a sequence with `past` tokens before; a row
+// that sees no key gives 0.
+//
+// A CTA takes 16 query rows ((token, head) pairs that share a KV head) and a
+// range of keys, 32 keys at a time through shared memory in fp32, with the
+// running maximum and sum of the softmax in base 2.  Where the rows alone do
+// not fill the GPU the keys are cut into ranges, whose (max, sum, O) go to
+// the workspace and are joined in order by a second kernel.
+//
+// Bound: the fp32 FMA rate next to the shared-memory reads (each K and V
+// element read from memory once per 16 rows).
+#include <math.h>
+
+#include <algorithm>
+
+#include "kernels.h"
+#include "paged.h"
+
+namespace mg {
+namespace {
+
+constexpr int kRows = 16;     // query rows of a CTA
+constexpr int kKeys = 32;     // keys of a round
+constexpr int kSimt = 128;    // threads
+constexpr int kMaxSplits = 32;
+
+// One 16-byte (e4m3: 8-code) piece of a cached row, widened.
+template <typename C>
+struct Cached;
+template <>
+struct Cached<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void load(const float* p, float* v) { load16_f<float>(p, v); }
+};
+template <>
+struct Cached<__nv_bfloat16> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void load(const __nv_bfloat16* p, float* v) { load16_f<__nv_bfloat16>(p, v); }
+};
+template <>
+struct Cached<uint8_t> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void load(const uint8_t* p, float* v) {
+    const uint2 w = *reinterpret_cast<const uint2*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = from_e4m3x2((i < 2 ? w.x : w.y) >> (16 * (i & 1)));
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
+};
+
+template <typename T, typename C, int D>
+__global__ void __launch_bounds__(kSimt) paged_attn_simt_kernel(PagedAttnArgs a, int tiles, int splits) {
+  constexpr int RPT = kRows * D / kSimt;          // output rows of a thread
+  constexpr int P4 = Cached<C>::N;
+  __shared__ float sq[kRows][D + 1];
+  __shared__ float sk[kKeys][D + 1];
+  __shared__ float sv[kKeys][D];
+  __shared__ float sp[kRows][kKeys];
+  __shared__ float keep[kRows], sum[kRows], top[kRows];
+  pdl_trigger();
+  pdl_wait();
+  const PagedPool& pool = a.pool;
+  const PagedBatch& bt = a.batch;
+  const int tid = threadIdx.x, h = blockIdx.y, z = blockIdx.z;
+  const int b = blockIdx.x / tiles, tile = blockIdx.x % tiles;
+  const int G = a.nq / pool.nkv;
+  const SeqSpan span = seq_span(bt, b, pool.ps);
+  if (!span.ok) {
+    if (tid == 0) flag_error(a.err, kErrPaged);
+    return;
+  }
+  const int rows = span.n * G, r0 = tile * kRows;
+  if (r0 >= rows) return;
+  const int nr = min(kRows, rows - r0);
+  const int most = min(span.past + (r0 + nr - 1) / G + 1, span.past + span.n);  // keys the last row sees
+  const int step = most > 0 ? (int)(((long long)(most + kKeys - 1) / kKeys + splits - 1) / splits) * kKeys : 0;
+  const long long first = (long long)z * step;
+  const int k_lo = (int)min(first, (long long)max(most, 0)), k_hi = (int)min(first + step, (long long)max(most, 0));
+
+  for (int i = tid; i < kRows * D; i += kSimt) {
+    const int r = i / D, d = i % D;
+    float x = 0.f;
+    if (r < nr)
+      x = ldf<T>((const T*)a.q + (int64_t)(span.q0 + (r0 + r) / G) * a.ldq + (int64_t)(h * G + (r0 + r) % G) * a.hdq + d);
+    sq[r][d] = x;
+  }
+  const float scale2 = a.scale * 1.4426950408889634f;
+  const int qr = tid / 8, kq = tid % 8;                   // score row, first key
+  const int vis = qr < nr ? span.past + (r0 + qr) / G + 1 : 0;
+  float m = -INFINITY, l = 0.f;                           // of row qr (the same in its 8 threads)
+  const int od = tid % D, og = tid / D;                   // output dim, first output row / RPT
+  float acc[RPT];
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) acc[i] = 0.f;
+
+  for (int k0 = k_lo; k0 < k_hi; k0 += kKeys) {
+    __syncthreads();
+    for (int i = tid; i < kKeys * D / P4; i += kSimt) {
+      const int r = i / (D / P4), d = i % (D / P4) * P4, j = k0 + r;
+      float kx[P4], vx[P4];
+#pragma unroll
+      for (int e = 0; e < P4; ++e) kx[e] = vx[e] = 0.f;
+      if (j < k_hi) {
+        const int page = bt.table[(int64_t)b * bt.ld + j / pool.ps];
+        if (page >= 0 && page < pool.pages) {
+          const int o = j % pool.ps;
+          Cached<C>::load((const C*)pool.k + page * pool.kp + h * pool.kh + o * pool.kt + d, kx);
+          Cached<C>::load((const C*)pool.v + page * pool.vp + h * pool.vh + o * pool.vt + d, vx);
+          if constexpr (sizeof(C) == 1) {
+            const float fk = pool.ks[page * pool.kse + h], fv = pool.vs[page * pool.vse + h];
+#pragma unroll
+            for (int e = 0; e < P4; ++e) kx[e] *= fk, vx[e] *= fv;
+          }
+        } else {
+          flag_error(a.err, kErrPaged);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < P4; ++e) sk[r][d + e] = kx[e], sv[r][d + e] = vx[e];
+    }
+    __syncthreads();
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int d = 0; d < D; ++d) {
+      const float x = sq[qr][d];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[i] = fmaf(x, sk[kq + 8 * i][d], s[i]);
+    }
+    float mx = m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[i] = k0 + kq + 8 * i < vis ? s[i] * scale2 : -INFINITY;
+      mx = fmaxf(mx, s[i]);
+    }
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const float alpha = m == -INFINITY ? 0.f : exp2f(m - mx);
+    float part = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float p = s[i] == -INFINITY ? 0.f : exp2f(s[i] - mx);
+      sp[qr][kq + 8 * i] = p;
+      part += p;
+    }
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+    m = mx;
+    l = l * alpha + part;
+    if (kq == 0) keep[qr] = alpha;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) acc[i] *= keep[og * RPT + i];
+    // Keys that no row of the tile sees were loaded as zeros; a row's own
+    // invisible keys weigh 0, but 0 · NaN is not 0, so they are left out.
+    for (int k = 0; k < kKeys; ++k) {
+      const float v = sv[k][od];
+#pragma unroll
+      for (int i = 0; i < RPT; ++i) {
+        const float p = sp[og * RPT + i][k];
+        acc[i] = p != 0.f ? fmaf(p, v, acc[i]) : acc[i];
+      }
+    }
+  }
+  if (kq == 0) {
+    sum[qr] = l;
+    top[qr] = m;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    const int r = og * RPT + i;
+    if (r >= nr) continue;
+    const int64_t t = span.q0 + (r0 + r) / G;
+    const int head = h * G + (r0 + r) % G;
+    if (splits == 1) {
+      stf<T>((T*)a.out + t * a.ldo + (int64_t)head * a.hdo + od, sum[r] == 0.f ? 0.f : acc[i] / sum[r]);
+    } else {
+      float* w = (float*)a.ws + ((t * a.nq + head) * splits + z) * (D + 2);
+      w[2 + od] = acc[i];
+      if (od == 0) {
+        w[0] = top[r];
+        w[1] = sum[r];
+      }
+    }
+  }
+}
+
+// Join of the key ranges of one (token, head), in their order.
+template <typename T, int D>
+__global__ void __launch_bounds__(kSimt) paged_attn_join_kernel(PagedAttnArgs a, int splits) {
+  pdl_trigger();
+  pdl_wait();
+  __shared__ int found;
+  const int64_t t = blockIdx.x;
+  if (threadIdx.x == 0) found = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.batch.B; i += kSimt) {  // rows of no (valid) sequence stay as they are
+    const SeqSpan sp = seq_span(a.batch, i, a.pool.ps);
+    if (sp.ok && sp.q0 <= t && t < sp.q0 + sp.n) found = 1;
+  }
+  __syncthreads();
+  if (!found) return;
+  for (int i = threadIdx.x; i < a.nq * D; i += kSimt) {
+    const int head = i / D, d = i % D;
+    const float* w = (const float*)a.ws + (t * a.nq + head) * splits * (D + 2);
+    float mx = -INFINITY;
+    for (int z = 0; z < splits; ++z) mx = fmaxf(mx, w[z * (D + 2)]);
+    float l = 0.f, o = 0.f;
+    for (int z = 0; z < splits; ++z) {
+      const float mz = w[z * (D + 2)];
+      const float f = mz == -INFINITY ? 0.f : exp2f(mz - mx);
+      l += f * w[z * (D + 2) + 1];
+      o += f * w[z * (D + 2) + 2 + d];
+    }
+    stf<T>((T*)a.out + t * a.ldo + (int64_t)head * a.hdo + d, l == 0.f ? 0.f : o / l);
+  }
+}
+
+int simt_tiles(const PagedAttnArgs& a) {
+  return (int)(((int64_t)std::max(a.batch.max_new, 1) * (a.nq / a.pool.nkv) + kRows - 1) / kRows);
+}
+
+// Key ranges per row: enough CTAs for four per SM, at least 64 keys each.
+int simt_splits(const PagedAttnArgs& a) {
+  const int64_t ctas = (int64_t)a.batch.B * simt_tiles(a) * a.pool.nkv;
+  const int64_t keys = (int64_t)a.batch.max_pages * a.pool.ps;
+  int64_t n = ctas > 0 ? (4LL * usable_sms() + ctas - 1) / ctas : 1;
+  n = std::min<int64_t>(n, (keys + 63) / 64);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(n, kMaxSplits));
+}
+
+template <typename T, typename C, int D>
+cudaError_t launch_simt_d(const PagedAttnArgs& a, cudaStream_t s) {
+  const int tiles = simt_tiles(a), splits = simt_splits(a);
+  const dim3 grid((unsigned)(a.batch.B * tiles), (unsigned)a.pool.nkv, (unsigned)splits);
+  cudaError_t e = launch_pdl(paged_attn_simt_kernel<T, C, D>, grid, dim3(kSimt), 0, s, a, tiles, splits);
+  if (e == cudaSuccess && splits > 1)
+    e = launch_pdl(paged_attn_join_kernel<T, D>, dim3((unsigned)a.batch.T), dim3(kSimt), 0, s, a, splits);
+  return e;
+}
+
+template <typename T, typename C>
+cudaError_t launch_simt(const PagedAttnArgs& a, cudaStream_t s) {
+  switch (a.pool.D) {
+    case 8: return launch_simt_d<T, C, 8>(a, s);
+    case 16: return launch_simt_d<T, C, 16>(a, s);
+    case 32: return launch_simt_d<T, C, 32>(a, s);
+    case 64: return launch_simt_d<T, C, 64>(a, s);
+    case 128: return launch_simt_d<T, C, 128>(a, s);
+  }
+  return cudaErrorInvalidValue;
+}
+
+}  // namespace
+
+size_t paged_attention_workspace(const PagedAttnArgs& a) {
+  const int splits = simt_splits(a);
+  return splits > 1 ? (size_t)a.batch.T * a.nq * splits * (a.pool.D + 2) * sizeof(float) : 0;
+}
+
+cudaError_t launch_paged_attention(const PagedAttnArgs& a, cudaStream_t s) {
+  if (a.batch.T == 0 || a.batch.B == 0) return cudaSuccess;
+  if (a.ws_bytes < paged_attention_workspace(a)) return cudaErrorInvalidValue;
+  cudaError_t e;
+  if (a.dtype == kBF16)
+    e = a.pool.cdtype == kE4M3 ? launch_simt<__nv_bfloat16, uint8_t>(a, s) : launch_simt<__nv_bfloat16, __nv_bfloat16>(a, s);
+  else
+    e = a.pool.cdtype == kE4M3 ? launch_simt<float, uint8_t>(a, s) : launch_simt<float, float>(a, s);
+  return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+}  // namespace mg

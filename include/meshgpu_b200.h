@@ -310,6 +310,99 @@ int mg_linear_noalloc(int32_t dtype, const void* X, int64_t ldx, const void* W, 
                       int32_t N, int32_t K, int32_t epilogue, const void* R, int64_t ldr, void* Y,
                       int64_t ldy, void* stream);
 
+/* ---- Paged KV cache: one pool of pages that many requests share ----
+ * No counterpart in the reference, which keeps one contiguous cache per
+ * request and layer (llama_dense.py:166-170).  A page holds `page_size`
+ * consecutive tokens of one sequence for every KV head of one layer; a page
+ * table names each sequence's pages.  The pages hold the activation type or
+ * 8-bit e4m3 codes with one scale for each page and head. */
+
+#define MG_DTYPE_E4M3 2 /* cache type only */
+
+/* Device pointers of one layer's pool.  Element (page, head, token, dim) of
+ * k is at k[page k_page_stride + head k_head_stride + token k_token_stride +
+ * dim] (strides in elements, v likewise), so the pages can be slices of a
+ * larger pool and heads may lie before or after tokens.  Rows and strides are
+ * multiples of 16 bytes (of the row where it is shorter).  In an e4m3 pool
+ * the value of an element is its code times k_scale[page scale stride +
+ * head], a power of two that mg_paged_append keeps. */
+typedef struct mg_paged_pool {
+  void* k;
+  void* v;
+  float* k_scale; /* [num_pages, num_kv_heads], e4m3 pools only */
+  float* v_scale;
+  int64_t k_page_stride, k_head_stride, k_token_stride;
+  int64_t v_page_stride, v_head_stride, v_token_stride;
+  int64_t k_scale_stride, v_scale_stride; /* elements between the rows of two pages */
+  int32_t num_pages;
+  int32_t page_size; /* 16, 32, 64 or 128 tokens */
+  int32_t num_kv_heads;
+  int32_t head_dim;    /* 8, 16, 32, 64 or 128 */
+  int32_t cache_dtype; /* the activations' dtype, or MG_DTYPE_E4M3 */
+} mg_paged_pool;
+
+/* A ragged batch of at most 4096 sequences.  Sequence b brings the token rows
+ * q_start[b] .. q_start[b + 1] - 1 (possibly none) and holds kv_len[b] cached
+ * tokens with them; its token j lies in page page_table[b table_stride +
+ * j / page_size].  All three arrays are on the device and are read by the
+ * kernels only, so a captured call follows their contents; entries of the
+ * table past a sequence's last page are not read.  Rows of the token tensors
+ * behind q_start[batch] are left as they are.  A sequence whose ranges do not
+ * fit (a length above max_pages page_size, more than max_new new tokens, rows
+ * outside [0, tokens)) is left out, and, like a page id outside the pool,
+ * reported by mg_paged_check_device. */
+typedef struct mg_paged_batch {
+  const int32_t* page_table; /* [batch, max_pages] */
+  const int32_t* q_start;    /* [batch + 1] */
+  const int32_t* kv_len;     /* [batch] */
+  int64_t table_stride;
+  int32_t batch;
+  int32_t tokens;    /* rows of the token tensors */
+  int32_t max_pages; /* columns of the table */
+  int32_t max_new;   /* host bound: no sequence brings more new tokens */
+} mg_paged_batch;
+
+/* Append the batch's new tokens and rotate their queries: from the fused rows
+ * qkv [tokens, (num_q_heads + 2 num_kv_heads) head_dim] (row stride ld_qkv),
+ * q and k pass the optional per-head RMSNorm (q_norm / k_norm [head_dim],
+ * eps) and the rotary embedding of _apply_rope (llama_dense.py:112-125) with
+ * fp32 tables cos / sin [max_pos, head_dim / 2] (both NULL: no rotation) at
+ * positions[t], or at the token's place in its sequence where positions is
+ * NULL; q goes to q_out [tokens, num_q_heads, head_dim] (token stride ld_q),
+ * k and v to the token's place in its page.  Computed in fp32 and rounded
+ * once.  In an e4m3 pool a page's scale is the least power of two 2^e, e >=
+ * -100, with which its largest finite magnitude fits; a page that already
+ * holds tokens keeps a larger scale, and its codes are moved to a grown one.
+ * Infinities are stored as the largest magnitude, NaN as NaN.  A position
+ * outside the tables is clamped and reported.  Two sequences of a call must
+ * not append to the same page. */
+int mg_paged_append(const mg_paged_pool* pool, const mg_paged_batch* batch, int32_t dtype, const void* qkv,
+                    int64_t ld_qkv, int32_t num_q_heads, const int64_t* positions, const float* cos,
+                    const float* sin, int32_t max_pos, const void* q_norm, const void* k_norm, float eps,
+                    void* q_out, int64_t ld_q, void* stream);
+
+/* out[t, h] = softmax over the visible keys of scale q[t, h]·K, times V, with
+ * num_q_heads / num_kv_heads (at most 16) query heads per KV head.  The s-th
+ * of n new tokens sees the keys j <= kv_len - n + s; a row without any gives
+ * 0.  q and out: strides of tokens and heads in elements.  `workspace` (device
+ * memory, 256-byte aligned, mg_paged_attention_workspace bytes) belongs to
+ * the call until it has run on `stream`; it needs no initialisation. */
+int mg_paged_attention(const mg_paged_pool* pool, const mg_paged_batch* batch, int32_t dtype, const void* q,
+                       int64_t q_token_stride, int64_t q_head_stride, int32_t num_q_heads, float scale, void* out,
+                       int64_t out_token_stride, int64_t out_head_stride, void* workspace, uint64_t workspace_bytes,
+                       void* stream);
+
+/* Workspace of mg_paged_attention for this pool and batch (0 where the
+ * arguments are invalid; the call itself says why).  It depends on the sizes
+ * and on mg_reserve_sms alone, not on the lengths on the device. */
+uint64_t mg_paged_attention_workspace(const mg_paged_pool* pool, const mg_paged_batch* batch, int32_t dtype,
+                                      int32_t num_q_heads);
+
+/* Status of the mg_paged_* launches on the current device since the last
+ * check: waits for `stream`, then returns MG_EDEVICE (a page id, length, token
+ * range or position did not fit) or MG_ETIMEOUT, and clears it. */
+int mg_paged_check_device(void* stream);
+
 /* ---- Instrumentation (no counterpart in the reference, which has no
  * kernels of its own; used by the benchmark to report roofline fractions) ---- */
 
