@@ -1376,6 +1376,7 @@ int paged_args(const mg_paged_pool* p, const mg_paged_batch* b, int32_t dtype, i
   if ((uintptr_t)p->k % (unit * esz) || (uintptr_t)p->v % (unit * esz))
     return fail(MG_EINVAL, "pages must start on 16-byte boundaries");
   if (b->batch < 0 || b->tokens < 0 || b->max_new < 0) return fail(MG_EINVAL, "negative batch, tokens or max_new");
+  if (b->tokens >= kPagedMaxTokens) return fail(MG_EINVAL, "fewer than 2^26 token rows per call (got %d)", b->tokens);
   if (b->batch > kPagedMaxBatch) return fail(MG_EINVAL, "at most %d sequences per call (got %d)", kPagedMaxBatch, b->batch);
   if (b->batch > 0 && b->tokens > 0) {
     if (!b->page_table || !b->q_start || !b->kv_len) return fail(MG_EINVAL, "null page_table, q_start or kv_len");

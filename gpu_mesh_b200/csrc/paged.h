@@ -14,6 +14,8 @@ constexpr int kE4M3 = 2;             // cache type, next to kF32 / kBF16
 constexpr int kErrPaged = 4;         // a page id, length or token range outside the pool or the batch
 constexpr int kPagedMaxBatch = 4096; // sequences of one call (the kernels keep a prefix over them in shared memory)
 constexpr int kPagedMinExp = -100;   // least exponent of a page's scale
+constexpr int kPagedMaxExp = 100;    // largest: sums weighed by 2^-e stay in fp32's range
+constexpr int kPagedMaxTokens = 1 << 26;  // token rows of one call
 
 // Page p, KV head h, token o (of page_size) is the D contiguous elements at
 // k + p·kp + h·kh + o·kt (strides in elements, v likewise).  In an e4m3 pool
@@ -73,6 +75,13 @@ struct PagedAttnArgs {
   int* err;
 };
 size_t paged_attention_workspace(const PagedAttnArgs& a);
+
+// Tensor-core kernel for the sequences with at most kPagedFewRows query rows
+// ((token, head) pairs) per KV head (k_paged_decode.cu).
+constexpr int kPagedFewRows = 16;
+bool paged_decode_applicable(const PagedAttnArgs& a);
+size_t paged_decode_workspace(const PagedAttnArgs& a);
+cudaError_t launch_paged_decode(const PagedAttnArgs& a, cudaStream_t s);
 cudaError_t launch_paged_attention(const PagedAttnArgs& a, cudaStream_t s);
 
 #ifdef __CUDACC__
@@ -104,11 +113,11 @@ __device__ __forceinline__ float pow2i(int e) {
 __device__ __forceinline__ int scale_exp(float s) { return (int)((__float_as_uint(s) >> 23) & 0xffu) - 127; }
 
 // The least e >= kPagedMinExp with amax <= 448·2^e (448 = 1.75·2^8 is the
-// largest e4m3 value); amax >= 0 and finite.
+// largest e4m3 value), at most kPagedMaxExp; amax >= 0 and finite.
 __device__ __forceinline__ int e4m3_exp(float amax) {
   const uint32_t u = __float_as_uint(amax);
   const int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
-  return max(e, kPagedMinExp);
+  return min(max(e, kPagedMinExp), kPagedMaxExp);
 }
 
 // Two floats to two e4m3 codes, to nearest even; beyond ±448 (infinities

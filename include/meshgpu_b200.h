@@ -341,7 +341,7 @@ typedef struct mg_paged_pool {
   int32_t cache_dtype; /* the activations' dtype, or MG_DTYPE_E4M3 */
 } mg_paged_pool;
 
-/* A ragged batch of at most 4096 sequences.  Sequence b brings the token rows
+/* A ragged batch of at most 4096 sequences and fewer than 2^26 token rows.  Sequence b brings the token rows
  * q_start[b] .. q_start[b + 1] - 1 (possibly none) and holds kv_len[b] cached
  * tokens with them; its token j lies in page page_table[b table_stride +
  * j / page_size].  All three arrays are on the device and are read by the
@@ -370,10 +370,11 @@ typedef struct mg_paged_batch {
  * positions[t], or at the token's place in its sequence where positions is
  * NULL; q goes to q_out [tokens, num_q_heads, head_dim] (token stride ld_q),
  * k and v to the token's place in its page.  Computed in fp32 and rounded
- * once.  In an e4m3 pool a page's scale is the least power of two 2^e, e >=
- * -100, with which its largest finite magnitude fits; a page that already
+ * once.  In an e4m3 pool a page's scale is the least power of two 2^e, -100 <=
+ * e <= 100, with which its largest finite magnitude fits; a page that already
  * holds tokens keeps a larger scale, and its codes are moved to a grown one.
- * Infinities are stored as the largest magnitude, NaN as NaN.  A position
+ * What lies beyond (infinities, magnitudes above 448 2^100) is stored as the
+ * largest magnitude of its sign, NaN as NaN.  A position
  * outside the tables is clamped and reported.  Two sequences of a call must
  * not append to the same page. */
 int mg_paged_append(const mg_paged_pool* pool, const mg_paged_batch* batch, int32_t dtype, const void* qkv,

@@ -27,7 +27,7 @@ def least_exp(amax: float) -> int:
         e += 1
     while 448.0 * 2.0 ** (e - 1) >= amax:
         e -= 1
-    return max(e, -100)
+    return min(max(e, -100), 100)
 
 
 def rotate(x, w, cos, sin, eps):

@@ -58,6 +58,7 @@ SHARED = [
     (dict(), dict(batch=-1), dict(), "negative"),
     (dict(), dict(max_new=-1), dict(), "negative"),
     (dict(), dict(batch=4097), dict(), "4096"),
+    (dict(), dict(tokens=1 << 26), dict(), "2^26"),
     (dict(), dict(q_start=None), dict(), "null"),
     (dict(), dict(max_pages=0), dict(), "columns"),
     (dict(), dict(max_pages=1 << 28, table_stride=1 << 28), dict(), "columns"),
