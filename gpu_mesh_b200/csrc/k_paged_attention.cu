@@ -57,7 +57,7 @@ struct Cached<uint8_t> {
 };
 
 template <typename T, typename C, int D>
-__global__ void __launch_bounds__(kSimt) paged_attn_simt_kernel(PagedAttnArgs a, int tiles, int splits, int few) {
+__global__ void __launch_bounds__(kSimt) paged_attn_simt_kernel(PagedAttnArgs a, int tiles, int splits) {
   constexpr int RPT = kRows * D / kSimt;          // output rows of a thread
   constexpr int P4 = Cached<C>::N;
   __shared__ float sq[kRows][D + 1];
@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(kSimt) paged_attn_simt_kernel(PagedAttnArgs a,
     return;
   }
   const int rows = span.n * G, r0 = tile * kRows;
-  if (r0 >= rows || rows <= few) return;
+  if (r0 >= rows) return;
   const int nr = min(kRows, rows - r0);
   const int most = min(span.past + (r0 + nr - 1) / G + 1, span.past + span.n);  // keys the last row sees
   const int step = most > 0 ? (int)(((long long)(most + kKeys - 1) / kKeys + splits - 1) / splits) * kKeys : 0;
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(kSimt) paged_attn_simt_kernel(PagedAttnArgs a,
 
 // Join of the key ranges of one (token, head), in their order.
 template <typename T, int D>
-__global__ void __launch_bounds__(kSimt) paged_attn_join_kernel(PagedAttnArgs a, int splits, int few) {
+__global__ void __launch_bounds__(kSimt) paged_attn_join_kernel(PagedAttnArgs a, int splits) {
   pdl_trigger();
   pdl_wait();
   __shared__ int found;
@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(kSimt) paged_attn_join_kernel(PagedAttnArgs a,
   __syncthreads();
   for (int i = threadIdx.x; i < a.batch.B; i += kSimt) {  // rows of no (valid) sequence stay as they are
     const SeqSpan sp = seq_span(a.batch, i, a.pool.ps);
-    if (sp.ok && sp.q0 <= t && t < sp.q0 + sp.n && sp.n * (a.nq / a.pool.nkv) > few) found = 1;
+    if (sp.ok && sp.q0 <= t && t < sp.q0 + sp.n) found = 1;
   }
   __syncthreads();
   if (!found) return;
@@ -237,23 +237,23 @@ int simt_splits(const PagedAttnArgs& a) {
 }
 
 template <typename T, typename C, int D>
-cudaError_t launch_simt_d(const PagedAttnArgs& a, int few, cudaStream_t s) {
+cudaError_t launch_simt_d(const PagedAttnArgs& a, cudaStream_t s) {
   const int tiles = simt_tiles(a), splits = simt_splits(a);
   const dim3 grid((unsigned)(a.batch.B * tiles), (unsigned)a.pool.nkv, (unsigned)splits);
-  cudaError_t e = launch_pdl(paged_attn_simt_kernel<T, C, D>, grid, dim3(kSimt), 0, s, a, tiles, splits, few);
+  cudaError_t e = launch_pdl(paged_attn_simt_kernel<T, C, D>, grid, dim3(kSimt), 0, s, a, tiles, splits);
   if (e == cudaSuccess && splits > 1)
-    e = launch_pdl(paged_attn_join_kernel<T, D>, dim3((unsigned)a.batch.T), dim3(kSimt), 0, s, a, splits, few);
+    e = launch_pdl(paged_attn_join_kernel<T, D>, dim3((unsigned)a.batch.T), dim3(kSimt), 0, s, a, splits);
   return e;
 }
 
 template <typename T, typename C>
-cudaError_t launch_simt(const PagedAttnArgs& a, int few, cudaStream_t s) {
+cudaError_t launch_simt(const PagedAttnArgs& a, cudaStream_t s) {
   switch (a.pool.D) {
-    case 8: return launch_simt_d<T, C, 8>(a, few, s);
-    case 16: return launch_simt_d<T, C, 16>(a, few, s);
-    case 32: return launch_simt_d<T, C, 32>(a, few, s);
-    case 64: return launch_simt_d<T, C, 64>(a, few, s);
-    case 128: return launch_simt_d<T, C, 128>(a, few, s);
+    case 8: return launch_simt_d<T, C, 8>(a, s);
+    case 16: return launch_simt_d<T, C, 16>(a, s);
+    case 32: return launch_simt_d<T, C, 32>(a, s);
+    case 64: return launch_simt_d<T, C, 64>(a, s);
+    case 128: return launch_simt_d<T, C, 128>(a, s);
   }
   return cudaErrorInvalidValue;
 }
@@ -278,28 +278,29 @@ size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 size_t paged_attention_workspace(const PagedAttnArgs& a) {
   if (!paged_decode_applicable(a)) return simt_workspace(a);
   const size_t few = align256(paged_decode_workspace(a));
-  return only_few(a) ? few : few + simt_workspace(a);
+  return only_few(a) ? few : few + paged_extend_workspace(a);
 }
 
+// bf16 with head_dim 64 or 128 runs on the tensor cores: each sequence on the
+// kernel for few or for many query rows, by its new tokens as the device has
+// them (the host's bound says whether the second can be left out).  Other
+// types and sizes run on the CUDA cores.
 cudaError_t launch_paged_attention(const PagedAttnArgs& a, cudaStream_t s) {
   if (a.batch.T == 0 || a.batch.B == 0) return cudaSuccess;
   if (a.ws_bytes < paged_attention_workspace(a)) return cudaErrorInvalidValue;
-  cudaError_t e = cudaSuccess;
-  PagedAttnArgs rest = a;
-  int few = 0;
+  cudaError_t e;
   if (paged_decode_applicable(a)) {
     e = launch_paged_decode(a, s);
-    if (e != cudaSuccess || only_few(a)) return e != cudaSuccess ? e : cudaGetLastError();
-    few = kPagedFewRows;
-    const size_t used = align256(paged_decode_workspace(a));
-    rest.ws = (uint8_t*)a.ws + used;
-    rest.ws_bytes = a.ws_bytes - used;
+    if (e == cudaSuccess && !only_few(a)) {
+      PagedAttnArgs many = a;
+      many.ws = (uint8_t*)a.ws + align256(paged_decode_workspace(a));
+      e = launch_paged_extend(many, s);
+    }
+  } else if (a.dtype == kBF16) {
+    e = a.pool.cdtype == kE4M3 ? launch_simt<__nv_bfloat16, uint8_t>(a, s) : launch_simt<__nv_bfloat16, __nv_bfloat16>(a, s);
+  } else {
+    e = a.pool.cdtype == kE4M3 ? launch_simt<float, uint8_t>(a, s) : launch_simt<float, float>(a, s);
   }
-  if (a.dtype == kBF16)
-    e = a.pool.cdtype == kE4M3 ? launch_simt<__nv_bfloat16, uint8_t>(rest, few, s)
-                               : launch_simt<__nv_bfloat16, __nv_bfloat16>(rest, few, s);
-  else
-    e = a.pool.cdtype == kE4M3 ? launch_simt<float, uint8_t>(rest, few, s) : launch_simt<float, float>(rest, few, s);
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 

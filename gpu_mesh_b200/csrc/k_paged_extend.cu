@@ -1,0 +1,901 @@
+// Attention over a paged KV cache for sequences that bring many tokens
+// (prompts and prompt chunks; more than 16 query rows per KV head), on
+// tcgen05.  bf16 activations, head_dim 64 or 128, pages in bf16 or e4m3.
+//
+// A query tile is 128 / G tokens x the G query heads that share a KV head
+// (row r = token r / G, head r % G); an item is two adjacent tiles of one
+// (sequence, head), which share every key and value chunk they both see, and
+// a unit is an item's 128-key chunk.  Persistent CTAs (one per SM) count the
+// batch's units from the lengths on the device and take equal contiguous
+// runs, so chunks of long contexts fill the GPU however few items they make;
+// an item that a run's end cuts leaves (max, sum, O) of its rows in the
+// workspace, and a second kernel joins the pieces in order.
+//
+// Warp roles:
+//   * softmax (4 warps per tile): one thread per query row (its TMEM lane).
+//     Online softmax in base 2; the maximum moves only when a row's scores
+//     outgrow it by 2^8, and only then is the row of O in TMEM rescaled.  P
+//     goes back into TMEM over the scores.
+//   * MMA issuer: S_X = Q_X·Kᵀ and O_X += P_X·V per tile X, ping-ponging, P
+//     read from TMEM, V read MN-major.
+//   * producer: the tiles' query rows by 3-D TMA over {dim, head, token};
+//     bf16 pages by 4-D TMA, looked up four chunks at a time.
+//   * e4m3 pages, four converter warps: 16 codes per load, a chunk ahead in
+//     registers, to halves (exact) in the tiles' swizzled layout; rows behind
+//     the sequence become zeros.  Q becomes halves scaled by a power of two
+//     per row (exact), K's scale multiplies the fp32 scores, V's scale 2^e
+//     joins the exponent: P' = 2^(s + e - m + 7) in half (2^-11 relative, down
+//     to 2^-21 of the largest, and within 2^-31 of it below), while the sum
+//     adds 2^(s - m) in fp32.  fp8 MMAs would need P in e4m3: 2^-4.
+// P is bf16 over bf16 pages (2^-8 half step at most 2^-9 relative): the
+// precision in which the stage's own prefill multiplies the values.
+//
+// Bound: the MMA pipe and the exponentials, 4·D + 1 operations per score.
+// Every wait is bounded (code 3 in the error word on expiry); on expiry the
+// roles stop, issued loads and MMAs drain, and TMEM is freed.
+#include <math.h>
+
+#include <algorithm>
+
+#include "kernels.h"
+#include "paged_tc.cuh"
+
+namespace mg {
+namespace {
+
+using namespace tc;
+using namespace attn;
+using namespace paged;
+using bf16 = __nv_bfloat16;
+
+constexpr int kChunkE = 128;     // keys of a unit
+constexpr int kTile = 128;       // query rows of a tile = TMEM lanes
+constexpr int kBoxE = 128 * 128; // a 128-row x 128-byte swizzled block
+constexpr int kColSE = 0;        // TMEM: tile X's scores (then P) at 128·X, its output at 256 + D·X
+constexpr int kColOE = 256;
+constexpr int kSmemE = 227 * 1024;
+
+template <bool E4>
+struct Roles {
+  static constexpr int kSoft = 8;                   // warps 0-3 tile A, 4-7 tile B
+  static constexpr int kConv = E4 ? 4 : 0;          // warps 8-11
+  static constexpr int kProducer = kSoft + kConv;
+  static constexpr int kMma = kProducer + 1;
+  static constexpr int kThreads = 32 * (kMma + 1);
+};
+
+template <int D>
+struct ExtendLayout {
+  static constexpr int kDB = D / 64;
+  static constexpr int kQ = kDB * kBoxE;   // one tile's query rows
+  static constexpr int kKV = kDB * kBoxE;  // keys (or values) of a chunk, as 16-bit
+  static constexpr int kOffQ = 0;
+  static constexpr int kOffKV = 2 * kQ;
+  static constexpr int kOffBar = kOffKV + 2 * 2 * kKV;
+  static constexpr int kOffScale = kOffBar + 256;     // [stage][8] K scales, [stage][8] V exponents
+  static constexpr int kOffPre = kOffScale + 128;     // [B + 1] units before a sequence
+  static int bytes(int B) { return kOffPre + (B + 1 + 3) / 4 * 16 + 1024; }
+};
+
+// The tile pairs of one sequence.
+struct Pairs {
+  SeqSpan s;
+  int tq, n_pairs;  // tokens of a tile, tile pairs
+  __device__ Pairs(const SeqSpan& sp, int G) : s(sp) {
+    tq = kTile / G;
+    n_pairs = sp.n * G > kPagedFewRows ? (sp.n + 2 * tq - 1) / (2 * tq) : 0;
+  }
+  // Chunks that tile qt sees (0 for a tile past the sequence).
+  __device__ int tile_chunks(int qt) const {
+    if (qt * tq >= s.n) return 0;
+    return (max(0, s.past + min((qt + 1) * tq, s.n)) + kChunkE - 1) / kChunkE;
+  }
+  __device__ int units(int j) const { return max(1, max(tile_chunks(2 * j), tile_chunks(2 * j + 1))); }
+};
+
+// Units of a sequence and KV head, by a whole warp.
+__device__ __forceinline__ long long seq_units(const Pairs& p) {
+  long long n = 0;
+  for (int j = threadIdx.x & 31; j < p.n_pairs; j += 32) n += p.units(j);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  return n;
+}
+
+// Fills pre[0 .. B] (units before each sequence, saturated) with all warps of
+// the CTA; pre[B] is 0 where the batch is too large to count.
+__device__ __forceinline__ void count_units(const PagedAttnArgs& a, int* pre, bool report) {
+  const int G = a.nq / a.pool.nkv, warps = blockDim.x / 32, warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  for (int b = warp; b < a.batch.B; b += warps) {
+    const SeqSpan sp = seq_span(a.batch, b, a.pool.ps);
+    if (report && !sp.ok && lane == 0) flag_error(a.err, kErrPaged);
+    const long long n = seq_units(Pairs(sp, G)) * a.pool.nkv;
+    if (lane == 0) pre[b + 1] = (int)min(n, 0x7fffffffLL);
+  }
+  __syncthreads();
+  if (warp == 0) {
+    long long run = 0;
+    for (int b0 = 0; b0 < a.batch.B; b0 += 32) {
+      const int b = b0 + lane;
+      long long x = b < a.batch.B ? pre[b + 1] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      x += run;
+      if (b < a.batch.B) pre[b + 1] = (int)min(x, 0x7fffffffLL);
+      run = __shfl_sync(0xffffffffu, x, 31);
+    }
+    if (lane == 0) {
+      pre[0] = 0;
+      if (run >= 0x7fffffffLL) {
+        if (report) flag_error(a.err, kErrPaged);
+        pre[a.batch.B] = 0;
+      }
+    }
+  }
+  __syncthreads();
+}
+
+struct RunsE {
+  long long total;
+  int grid;
+  __device__ RunsE(long long n, int most) : total(n), grid((int)(n < most ? n : most)) {}
+  __device__ int begin(int c) const { return (int)((long long)c * total / grid); }
+};
+
+// Where a unit lies: sequence, KV head, tile pair, chunk inside the item.
+struct Place {
+  int b, h, j, chunk;
+};
+
+// By a whole warp (all lanes get the result).
+__device__ __forceinline__ Place place_of(const PagedAttnArgs& a, const int* pre, int u) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = a.batch.B;  // pre[lo] <= u < pre[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (pre[mid] <= u) lo = mid; else hi = mid;
+  }
+  const Pairs p(seq_span(a.batch, lo, a.pool.ps), a.nq / a.pool.nkv);
+  const int per = (pre[lo + 1] - pre[lo]) / a.pool.nkv;
+  Place r{lo, (u - pre[lo]) / per, 0, 0};
+  int rem = (u - pre[lo]) % per;
+  for (int j0 = 0;; j0 += 32) {
+    const int n = j0 + lane < p.n_pairs ? p.units(j0 + lane) : 0;
+    int x = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, x > rem);
+    if (past || j0 + 32 >= p.n_pairs) {
+      const int at = past ? __ffs(past) - 1 : 31;
+      r.j = j0 + at;
+      r.chunk = rem - __shfl_sync(0xffffffffu, x - n, at);
+      return r;
+    }
+    rem -= __shfl_sync(0xffffffffu, x, 31);
+  }
+}
+
+// The pieces of a CTA's run, one after another: item (b, h, j), its chunks
+// [lo, hi) that lie in the run, and the share of them that each tile sees.
+struct Walk {
+  const PagedAttnArgs& a;
+  const int* pre;
+  int u, u1, first;
+  Place at;
+  Pairs p;
+  int lo, hi, units, ca, cb, nch;  // ca, cb: chunks of each tile in this piece; nch: the larger
+  bool whole;
+  __device__ Walk(const PagedAttnArgs& args, const int* pre_, int u0, int u1_)
+      : a(args), pre(pre_), u(u0), u1(u1_), first(u0), at(place_of(args, pre_, u0)),
+        p(seq_span(args.batch, at.b, args.pool.ps), args.nq / args.pool.nkv) {
+    set();
+  }
+  __device__ void set() {
+    units = p.units(at.j);
+    lo = at.chunk;
+    hi = min(units, lo + (u1 - u));
+    whole = lo == 0 && hi == units;
+    ca = max(0, min(hi, p.tile_chunks(2 * at.j)) - lo);
+    cb = max(0, min(hi, p.tile_chunks(2 * at.j + 1)) - lo);
+    nch = max(ca, cb);
+  }
+  __device__ int c(int x) const { return x ? cb : ca; }
+  __device__ bool done() const { return u >= u1; }
+  __device__ void next() {
+    u += hi - lo;
+    if (u >= u1) return;
+    at.chunk = 0;
+    if (++at.j == p.n_pairs) {
+      at.j = 0;
+      if (++at.h == a.pool.nkv) {
+        at.h = 0;
+        do ++at.b; while (pre[at.b + 1] == pre[at.b]);
+        p = Pairs(seq_span(a.batch, at.b, a.pool.ps), a.nq / a.pool.nkv);
+      }
+    }
+    set();
+  }
+};
+
+// Rows of a partial: O [256][D], then the maxima and the sums.
+template <int D>
+__host__ __device__ constexpr size_t partial_floats() {
+  return (size_t)2 * kTile * (D + 2);
+}
+
+__device__ __forceinline__ uint64_t desc_mn(const void* p, uint32_t lbo) {
+  const uint64_t addr = smem_u32(p);
+  return ((addr & 0x3FFFFull) >> 4) | ((uint64_t)(lbo >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+
+__device__ __forceinline__ void mma_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(b), "r"(idesc), "r"(acc));
+}
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* tm, uint64_t* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          smem_u32(dst)),
+      "l"(tm), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+__device__ __forceinline__ bool warp_waits(uint64_t* bar, uint32_t parity, int* err) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err));
+}
+
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+template <int D, bool E4>
+__global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
+    paged_extend_kernel(const __grid_constant__ PoolMaps maps, const __grid_constant__ CUtensorMap tm_q,
+                        const __grid_constant__ PagedAttnArgs a) {
+  using L = ExtendLayout<D>;
+  using R = Roles<E4>;
+  const PagedPool& pool = a.pool;
+  const PagedBatch& bt = a.batch;
+  const int G = a.nq / pool.nkv;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* sq = smem + L::kOffQ;    // tile X's query rows at sq + X·kQ
+  uint8_t* skv = smem + L::kOffKV;  // stage s: keys at skv + 2·s·kKV, values kKV after them
+  uint64_t* bars = (uint64_t*)(smem + L::kOffBar);
+  uint64_t* kvfull = bars;        // [2] chunk in shared memory
+  uint64_t* kvempty = bars + 2;   // [2] chunk's products done
+  uint64_t* sfull = bars + 4;     // [tile] scores ready in TMEM
+  uint64_t* pready = bars + 6;    // [tile] P written, O rescaled
+  uint64_t* odone = bars + 8;     // [tile] value product done
+  uint64_t* qfull = bars + 10;    // [tile] query rows landed
+  uint64_t* qempty = bars + 12;   // [tile] the piece's score products read them
+  uint64_t* qconv = bars + 14;    // [tile] query rows are halves (e4m3)
+  uint64_t* drain = bars + 16;    // every MMA finished
+  uint32_t* tmem_holder = (uint32_t*)(bars + 17);
+  volatile int* abort_flag = (volatile int*)(tmem_holder + 1);
+  float* sks = (float*)(smem + L::kOffScale);  // [stage][8]
+  int* sve = (int*)(sks + 16);                 // [stage][8]
+  int* pre = (int*)(smem + L::kOffPre);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&kvfull[s], E4 ? 4 : 1);
+      mbar_init(&kvempty[s], 1);
+      mbar_init(&sfull[s], 1);
+      mbar_init(&pready[s], 4);
+      mbar_init(&odone[s], 1);
+      mbar_init(&qfull[s], 1);
+      mbar_init(&qempty[s], 1);
+      mbar_init(&qconv[s], 4);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  pdl_wait();
+  pdl_trigger();  // the join kernel reads, before its own wait, only what was written before this kernel
+  count_units(a, pre, blockIdx.x == 0);
+  const RunsE runs(pre[bt.B], (int)gridDim.x);
+  const int c = blockIdx.x;
+  if (c >= runs.grid) return;
+  if (warp == R::kProducer) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
+                 "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *tmem_holder;
+  const int u0 = runs.begin(c), u1 = runs.begin(c + 1);
+
+  int issued = 0;         // chunks requested by TMA (bf16 producer)
+  int qn[2] = {0, 0};     // query tiles requested (producer)
+  if (warp < R::kSoft) {
+    const int x = warp >> 2, q4 = warp & 3;
+    const int r = q4 * 32 + lane;
+    const uint32_t lanes = (uint32_t)(q4 * 32) << 16;
+    const float scale2 = a.scale * 1.4426950408889634f;
+    int n = 0;    // ring position of the piece's first chunk
+    int cnt = 0;  // this tile's chunks so far (its sfull / pready / odone phases)
+    int qm = 0;   // query tiles so far
+    bool ok = true;
+    for (Walk w(a, pre, u0, u1); !w.done() && ok; w.next()) {
+      const int qt = 2 * w.at.j + x;
+      const int s_tok = qt * w.p.tq + r / G;  // this row's token
+      const bool valid = r / G < w.p.tq && s_tok < w.p.s.n;
+      const int vis = valid ? w.p.s.past + s_tok + 1 : 0;
+      const int len = w.p.s.past + w.p.s.n;
+      const int nchx = w.c(x);
+      float rowf = scale2;
+      if (E4 && nchx > 0) {
+        // The tile's rows, one per thread: to halves, scaled to [128, 256).
+        ok = warp_waits(&qfull[x], qm & 1, a.err);
+        ++qm;
+        if (!ok) break;
+        uint8_t* row = sq + x * L::kQ + r * 128;
+        float amax = 0.f;
+#pragma unroll
+        for (int p = 0; p < D / 8; ++p) {
+          const uint4 v = *reinterpret_cast<const uint4*>(row + (p >> 3) * kBoxE + (((p & 7) ^ (r & 7)) << 4));
+          const uint32_t wv[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fmaxf(fabsf(lo_bf16(wv[i])), fabsf(hi_bf16(wv[i]))));
+        }
+        const int sh = row_shift(amax);
+        const float f = pow2i(sh);
+        rowf = scale2 * pow2i(-sh);
+#pragma unroll
+        for (int p = 0; p < D / 8; ++p) {
+          uint4* at = reinterpret_cast<uint4*>(row + (p >> 3) * kBoxE + (((p & 7) ^ (r & 7)) << 4));
+          const uint4 v = *at;
+          *at = make_uint4(pack_f16(lo_bf16(v.x) * f, hi_bf16(v.x) * f), pack_f16(lo_bf16(v.y) * f, hi_bf16(v.y) * f),
+                           pack_f16(lo_bf16(v.z) * f, hi_bf16(v.z) * f), pack_f16(lo_bf16(v.w) * f, hi_bf16(v.w) * f));
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&qconv[x]);
+      }
+
+      float m = -INFINITY, l = 0.f;  // base-2 maximum that P is taken against, sum
+      for (int ch = 0; ch < nchx; ++ch, ++cnt) {
+        const int pos = n + ch, k0 = (w.lo + ch) * kChunkE;
+        if (!warp_waits(&sfull[x], (int)(cnt & 1), a.err)) {
+          ok = false;
+          break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if constexpr (E4) {
+          if (!warp_waits(&kvfull[pos & 1], (int)(pos >> 1) & 1, a.err)) {
+            ok = false;
+            break;
+          }
+        }
+        const int nv = vis - k0;  // visible keys of this chunk for this row
+        const bool clear = __all_sync(0xffffffffu, nv >= kChunkE);
+        const uint32_t tS = tmem + lanes + kColSE + 128 * x;
+        // Half a chunk's scores, in base 2.  e4m3: with the page's K scale and
+        // V exponent, 16 keys at a time; bf16: the factor is left to the
+        // exponential (it is positive and commutes with the maximum).
+        auto scores = [&](int hf, float* sc) {
+          tmem_ld64(tS + 64 * hf, sc);
+          if constexpr (E4) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const float f = rowf * sks[(pos & 1) * 8 + 4 * hf + g], e = (float)sve[(pos & 1) * 8 + 4 * hf + g];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) sc[16 * g + i] = fmaf(sc[16 * g + i], f, e);
+            }
+          }
+          if (!clear) {
+#pragma unroll
+            for (int k = 0; k < 64; ++k) sc[k] = 64 * hf + k < nv ? sc[k] : -INFINITY;
+          }
+        };
+        // The maximum first, then the weights: the scores are read from TMEM
+        // twice, 64 at a time, which keeps the kernel's warps within their registers.
+        float t8[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t8[i] = -INFINITY;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          float sc[64];
+          scores(hf, sc);
+#pragma unroll
+          for (int k = 0; k < 64; ++k) t8[k & 7] = fmaxf(t8[k & 7], sc[k]);
+        }
+        float mt = fmaxf(fmaxf(fmaxf(t8[0], t8[1]), fmaxf(t8[2], t8[3])), fmaxf(fmaxf(t8[4], t8[5]), fmaxf(t8[6], t8[7])));
+        if constexpr (!E4) mt *= scale2;
+        float m_new = m;
+        bool moved = false;
+        if (m == -INFINITY) {
+          m_new = mt;
+        } else if (mt - m > 8.f) {
+          m_new = mt;
+          moved = true;
+        }
+        const float alpha = moved ? ex2(m - m_new) : 1.f;
+        const float mb = m_new == -INFINITY ? 0.f : m_new - (E4 ? 7.f : 0.f);
+        m = m_new;
+        float add = 0.f;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          float sc[64];
+          scores(hf, sc);
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+            for (int i = 16 * g; i < 16 * g + 16; i += 2) {
+              sc[i] = ex2(E4 ? sc[i] - mb : fmaf(sc[i], scale2, -mb));
+              sc[i + 1] = ex2(E4 ? sc[i + 1] - mb : fmaf(sc[i + 1], scale2, -mb));
+              s0 += sc[i];
+              s1 += sc[i + 1];
+              sc[i / 2] = __uint_as_float(E4 ? pack_f16(sc[i], sc[i + 1]) : bf16_pair(sc[i], sc[i + 1]));
+            }
+            add = E4 ? fmaf(s0 + s1, pow2i(-7 - sve[(pos & 1) * 8 + 4 * hf + g]), add) : add + (s0 + s1);
+          }
+          tmem_st32(tS + 32 * hf, sc);  // P over scores that have been read for good
+        }
+        l = l * alpha + add;
+        // The previous value product of this tile has finished (the score
+        // product just read was issued after it).
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll 1
+          for (int c4 = 0; c4 < D / 32; ++c4) {
+            float o[32];
+            tmem_ld32(tmem + lanes + kColOE + D * x + c4 * 32, o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] *= alpha;
+            tmem_st32(tmem + lanes + kColOE + D * x + c4 * 32, o);
+          }
+        }
+        // bf16: value rows behind the sequence were not loaded (P is 0 there,
+        // but 0 · NaN is not): cleared before the value products.
+        if constexpr (!E4) {
+          if (k0 + kChunkE > len && k0 + r >= len) {
+            if (!mbar_wait(&kvfull[pos & 1], (int)(pos >> 1) & 1, a.err)) ok = false;
+            uint8_t* v = skv + (pos & 1) * 2 * L::kKV + L::kKV;
+#pragma unroll
+            for (int p = 0; p < D / 8; ++p)
+              *reinterpret_cast<uint4*>(v + (p >> 3) * kBoxE + r * 128 + (p & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          if (!__all_sync(0xffffffffu, ok)) {
+            ok = false;
+            break;
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&pready[x]);
+      }
+      if (!ok) break;
+      if (nchx > 0) {
+        if (!warp_waits(&odone[x], (int)((cnt - 1) & 1), a.err)) {
+          ok = false;
+          break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      }
+      {
+        const float unit = E4 ? 1.f / 128.f : 1.f;
+        const float f = !w.whole ? unit : l == 0.f ? 0.f : unit / l;
+        bf16* out = (bf16*)a.out + (int64_t)(w.p.s.q0 + s_tok) * a.ldo + (int64_t)(w.at.h * G + r % G) * a.hdo;
+        float* part = (float*)a.ws + (size_t)(2 * c + (w.lo > 0 ? 0 : 1)) * partial_floats<D>();
+        const int row = x * kTile + r;
+#pragma unroll
+        for (int c4 = 0; c4 < D / 32; ++c4) {
+          float o[32];
+          if (nchx > 0) {
+            tmem_ld32(tmem + lanes + kColOE + D * x + c4 * 32, o);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = 0.f;
+          }
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] *= f;
+          if (!w.whole) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              *reinterpret_cast<float4*>(part + (size_t)row * D + 32 * c4 + 4 * e) =
+                  make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          } else if (valid) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              *reinterpret_cast<uint4*>(out + 32 * c4 + 8 * e) =
+                  make_uint4(bf16_pair(o[8 * e], o[8 * e + 1]), bf16_pair(o[8 * e + 2], o[8 * e + 3]),
+                             bf16_pair(o[8 * e + 4], o[8 * e + 5]), bf16_pair(o[8 * e + 6], o[8 * e + 7]));
+          }
+        }
+        if (!w.whole) {
+          part[2 * kTile * D + row] = m;
+          part[2 * kTile * D + 2 * kTile + row] = l;
+        }
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      n += w.nch;
+    }
+    if (!ok) *abort_flag = 1;
+  } else if (E4 && warp < R::kProducer) {
+    // Converters: thread dt takes 16 codes (piece pc) of rows rr + RPI·i.
+    constexpr int PPR = D / 16, RPI = 128 / PPR, NI = kChunkE / RPI;
+    const int dt = threadIdx.x - R::kSoft * 32;
+    const int rr = dt / PPR, pc = dt % PPR;
+    int n = 0;
+    bool ok = true;
+    uint4 kx[NI], vx[NI];
+    float ks = 0.f, vs = 1.f;
+    // Codes of chunk `chunk` of the walk's sequence and head (zeros behind its end).
+    auto load = [&](const Walk& w, int chunk) {
+      const int len = w.p.s.past + w.p.s.n;
+      const int32_t* tab = bt.table + (int64_t)w.at.b * bt.ld;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int j = chunk * kChunkE + rr + RPI * i;
+        kx[i] = vx[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (j < len) {
+          const int page = __ldg(tab + j / pool.ps);
+          if (page >= 0 && page < pool.pages) {
+            const int o = j % pool.ps;
+            kx[i] = *reinterpret_cast<const uint4*>((const uint8_t*)pool.k + page * pool.kp + w.at.h * pool.kh + o * pool.kt + pc * 16);
+            vx[i] = *reinterpret_cast<const uint4*>((const uint8_t*)pool.v + page * pool.vp + w.at.h * pool.vh + o * pool.vt + pc * 16);
+          } else {
+            flag_error(a.err, kErrPaged);
+          }
+        }
+      }
+      ks = 0.f;
+      vs = 1.f;
+      const int j = chunk * kChunkE + dt * 16;  // threads 0-7: the scales of 16 keys
+      if (dt < 8 && j < len) {
+        const int page = __ldg(tab + j / pool.ps);
+        if (page >= 0 && page < pool.pages) {
+          ks = pool.ks[(int64_t)page * pool.kse + w.at.h];
+          vs = pool.vs[(int64_t)page * pool.vse + w.at.h];
+        }
+      }
+    };
+    auto put = [&](uint8_t* tile, int row, const uint4& v) {
+      const uint32_t cw[4] = {v.x, v.y, v.z, v.w};
+      uint32_t f[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f[2 * i] = e4m3x2_to_f16x2(cw[i]);
+        f[2 * i + 1] = e4m3x2_hi_to_f16x2(cw[i]);
+      }
+      uint8_t* base = tile + (pc >> 2) * kBoxE + row * 128;
+      const int p0 = (pc & 3) * 2;
+      const uint4 lo = make_uint4(f[0], f[1], f[2], f[3]), hi = make_uint4(f[4], f[5], f[6], f[7]);
+      // The second block's lanes write their odd piece first: eight lanes then cover eight banks' groups.
+      const bool odd = (pc >> 2) & 1;
+      *reinterpret_cast<uint4*>(base + (((p0 + odd) ^ (row & 7)) << 4)) = odd ? hi : lo;
+      *reinterpret_cast<uint4*>(base + (((p0 + 1 - odd) ^ (row & 7)) << 4)) = odd ? lo : hi;
+    };
+    Walk w(a, pre, u0, u1);
+    while (!w.done() && w.nch == 0) w.next();
+    if (!w.done()) load(w, w.lo);
+    while (!w.done() && ok) {
+      for (int ch = 0; ch < w.nch; ++ch, ++n) {
+        const int s = n & 1;
+        if (n >= 2 && !warp_waits(&kvempty[s], (int)((n >> 1) - 1) & 1, a.err)) ok = false;
+        if (*abort_flag) ok = false;
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        uint8_t* st = skv + s * 2 * L::kKV;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          put(st, rr + RPI * i, kx[i]);
+          put(st + L::kKV, rr + RPI * i, vx[i]);
+        }
+        if (dt < 8) {
+          sks[s * 8 + dt] = ks;
+          sve[s * 8 + dt] = scale_exp(vs);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&kvfull[s]);
+        if (ch + 1 < w.nch) load(w, w.lo + ch + 1);
+      }
+      if (!ok) break;
+      do w.next(); while (!w.done() && w.nch == 0);
+      if (!w.done()) load(w, w.lo);
+    }
+    if (!ok) *abort_flag = 1;
+  } else if (warp == R::kProducer) {
+    int n = 0;
+    bool ok = true;
+    const int ppc = kChunkE / pool.ps;
+    for (Walk w(a, pre, u0, u1); !w.done() && ok; w.next()) {
+      // The tiles' query rows, once the previous piece's score products have read theirs.
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        if (w.c(x) == 0 || !ok) continue;
+        if (lane == 0) {
+          if (qn[x] > 0) ok = mbar_wait(&qempty[x], (qn[x] - 1) & 1, a.err);
+          if (ok) {
+            mbar_expect_tx(&qfull[x], L::kDB * 128 * G * w.p.tq);
+            for (int db = 0; db < L::kDB; ++db)
+              tma_load_3d(sq + x * L::kQ + db * kBoxE, &tm_q, &qfull[x], db * 64, w.at.h * G,
+                          w.p.s.q0 + (2 * w.at.j + x) * w.p.tq);
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+        if (ok) ++qn[x];
+      }
+      if constexpr (!E4) {
+        const int len = w.p.s.past + w.p.s.n;
+        for (int c0 = 0; c0 < w.nch && ok; c0 += 4) {
+          // Lane (j, i): page i of chunk c0 + j.
+          const int i = lane & 7, cj = c0 + (lane >> 3);
+          const int first = (w.lo + cj) * kChunkE + i * pool.ps;
+          int keys = 0, page = -1;
+          if (cj < w.nch && i < ppc && first < len) {
+            keys = min(pool.ps, len - first);
+            page = bt.table[(int64_t)w.at.b * bt.ld + first / pool.ps];
+            if (page < 0 || page >= pool.pages) {
+              flag_error(a.err, kErrPaged);
+              page = -1;  // outside the pool: the box is filled with zeros
+            }
+          }
+          const int nsl = (keys + kSlice - 1) / kSlice;
+          for (int j = 0; j < 4 && c0 + j < w.nch; ++j, ++n) {
+            const int s = n & 1;
+            if (n >= 2 && lane == 0) ok = mbar_wait(&kvempty[s], (int)((n >> 1) - 1) & 1, a.err);
+            ok = __shfl_sync(0xffffffffu, (int)(ok && !*abort_flag), 0);
+            if (!ok) break;
+            const bool mine = (lane >> 3) == j && keys > 0;
+            uint32_t bytes = mine ? 2u * nsl * kSlice * D * 2 : 0u;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) bytes += __shfl_xor_sync(0xffffffffu, bytes, o);
+            if (lane == 0) mbar_expect_tx(&kvfull[s], bytes);
+            __syncwarp();
+            if (mine) {
+              uint8_t* kd = skv + s * 2 * L::kKV + i * pool.ps * 128;
+              if (nsl * kSlice >= pool.ps) {
+                for (int db = 0; db < L::kDB; ++db) {
+                  tma_load_4d(kd + db * kBoxE, &maps.k, &kvfull[s], db * 64, 0, w.at.h, page);
+                  tma_load_4d(kd + L::kKV + db * kBoxE, &maps.v, &kvfull[s], db * 64, 0, w.at.h, page);
+                }
+              } else {
+                for (int q = 0; q < nsl; ++q)
+                  for (int db = 0; db < L::kDB; ++db) {
+                    tma_load_4d(kd + q * kSlice * 128 + db * kBoxE, &maps.k_tail, &kvfull[s], db * 64, q * kSlice,
+                                w.at.h, page);
+                    tma_load_4d(kd + q * kSlice * 128 + L::kKV + db * kBoxE, &maps.v_tail, &kvfull[s], db * 64,
+                                q * kSlice, w.at.h, page);
+                  }
+              }
+            }
+            issued = n + 1;
+          }
+        }
+      }
+      if (*abort_flag) ok = false;
+      ok = __all_sync(0xffffffffu, ok);
+    }
+    if (!ok) *abort_flag = 1;
+  } else if (warp == R::kMma) {
+    // bf16 x bf16, or half x half for e4m3 pages.
+    constexpr uint32_t kTypes = E4 ? 0u : (1u << 7) | (1u << 10);
+    constexpr uint32_t idS = (instr_desc(kChunkE) & ~((1u << 7) | (1u << 10))) | kTypes;
+    constexpr uint32_t idPV = ((instr_desc(D) & ~((1u << 7) | (1u << 10))) | kTypes) | (1u << 16);  // B MN-major
+    int n = 0, kv_seen = 0;
+    int cnt[2] = {0, 0}, qm[2] = {0, 0};
+    bool ok = true;
+    auto wait_kv = [&](int upto) -> bool {
+      for (; kv_seen < upto; ++kv_seen)
+        if (!mbar_wait(&kvfull[kv_seen & 1], (int)(kv_seen >> 1) & 1, a.err)) return false;
+      return true;
+    };
+    auto score = [&](int x, int pos) {
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint8_t* k = skv + (pos & 1) * 2 * L::kKV;
+      const uint8_t* q = sq + x * L::kQ;
+#pragma unroll
+      for (int kd = 0; kd < D / 16; ++kd)
+        mma_bf16(tmem + kColSE + 128 * x, smem_desc(q + (kd >> 2) * kBoxE) + (uint64_t)((kd & 3) * 2),
+                 smem_desc(k + (kd >> 2) * kBoxE) + (uint64_t)((kd & 3) * 2), idS, kd > 0 ? 1u : 0u);
+      mma_commit(&sfull[x]);
+    };
+    auto value = [&](int x, int pos, bool first) -> bool {
+      if (!mbar_wait(&pready[x], (int)(cnt[x] & 1), a.err)) return false;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint8_t* v = skv + (pos & 1) * 2 * L::kKV + L::kKV;
+#pragma unroll
+      for (int kk = 0; kk < kChunkE / 16; ++kk)
+        mma_ta(tmem + kColOE + D * x, tmem + kColSE + 128 * x + kk * 8, desc_mn(v + kk * 16 * 128, kBoxE), idPV,
+               (first && kk == 0) ? 0u : 1u);
+      mma_commit(&odone[x]);
+      // The next score product overwrites the columns that P is read from.
+      const bool done = mbar_wait(&odone[x], (int)(cnt[x] & 1), a.err);
+      ++cnt[x];
+      return done;
+    };
+    for (Walk w(a, pre, u0, u1); !w.done() && ok; w.next()) {
+      if (lane == 0) {
+        if (w.nch > 0) ok = wait_kv(n + 1);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (w.c(x) == 0 || !ok) continue;
+          if (!mbar_wait(E4 ? &qconv[x] : &qfull[x], qm[x] & 1, a.err)) {
+            ok = false;
+            continue;
+          }
+          score(x, n);
+          if (w.c(x) == 1) mma_commit(&qempty[x]);  // the tile's last score product
+          ++qm[x];
+        }
+        for (int ch = 0; ch < w.nch && ok; ++ch) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if (ch >= w.c(x) || !ok) continue;
+            if (!value(x, n + ch, ch == 0) || *abort_flag) {
+              ok = false;
+              continue;
+            }
+            if (ch + 1 < w.c(x)) {
+              if (!wait_kv(n + ch + 2)) {
+                ok = false;
+                continue;
+              }
+              score(x, n + ch + 1);
+              if (ch + 2 == w.c(x)) mma_commit(&qempty[x]);
+            }
+          }
+          mma_commit(&kvempty[(n + ch) & 1]);  // every product reading this chunk is issued
+        }
+        n += w.nch;
+        if (*abort_flag) ok = false;
+      }
+      ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+    }
+    if (lane == 0) {
+      if (!ok) *abort_flag = 1;
+      mma_commit(drain);  // arrives once every MMA issued above has finished
+    }
+  }
+
+  __syncthreads();
+  if (warp == R::kProducer && lane == 0 && *abort_flag) {
+    // Let the loads this CTA issued land before its shared memory goes away.
+    for (int i = issued > 2 ? issued - 2 : 0; i < issued; ++i) mbar_wait(&kvfull[i & 1], (int)(i >> 1) & 1, a.err);
+    for (int x = 0; x < 2; ++x)
+      if (qn[x] > 0) mbar_wait(&qfull[x], (qn[x] - 1) & 1, a.err);
+  }
+  if (warp == R::kMma && lane == 0) mbar_wait(drain, 0, a.err);
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == R::kProducer) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  }
+}
+
+// Joins the pieces of cut items: block (c, y) takes the item that CTA c's run
+// begins in the middle of, if no earlier run does, and 32 of its 256 rows.
+template <int D>
+__global__ void __launch_bounds__(256) paged_extend_join_kernel(const __grid_constant__ PagedAttnArgs a, int most) {
+  extern __shared__ int pre_s[];
+  __shared__ Place where;
+  pdl_trigger();
+  // Lengths were written before the attention kernel began, which allows this
+  // kernel to start only after its own wait.
+  count_units(a, pre_s, false);
+  const RunsE runs(pre_s[a.batch.B], most);
+  const int c = blockIdx.x + 1;  // a cut lies at the beginning of run 1 or a later one
+  if (c >= runs.grid) return;
+  const int u = runs.begin(c);
+  if (threadIdx.x < 32) {
+    const Place p = place_of(a, pre_s, u);
+    if (threadIdx.x == 0) where = p;
+  }
+  __syncthreads();
+  const Place pl = where;
+  if (pl.chunk == 0) return;               // the item begins here: nothing is cut
+  const int start = u - pl.chunk;          // the item's first unit
+  if (runs.begin(c - 1) > start) return;   // an earlier run begins inside the item too
+  const int G = a.nq / a.pool.nkv;
+  const Pairs p(seq_span(a.batch, pl.b, a.pool.ps), G);
+  const int end = start + p.units(pl.j);
+  int last = c;
+  while (last + 1 < runs.grid && runs.begin(last + 1) < end) ++last;
+  pdl_wait();
+  // Eight lanes per row, each D / 8 dims.
+  const int row = blockIdx.y * 32 + (threadIdx.x >> 3), d0 = (threadIdx.x & 7) * (D / 8);
+  const int r = row % kTile, s_tok = (2 * pl.j + row / kTile) * p.tq + r / G;
+  if (r / G >= p.tq || s_tok >= p.s.n) return;
+  auto piece = [&](int k) {  // run k's slot: 1 if the item begins in it, 0 if it began earlier
+    return (const float*)a.ws + (size_t)(2 * k + (runs.begin(k) > start ? 0 : 1)) * partial_floats<D>();
+  };
+  float M = -INFINITY;
+  for (int k = c - 1; k <= last; ++k) M = fmaxf(M, __ldcg(piece(k) + 2 * kTile * D + row));
+  float L = 0.f, o[D / 8];
+#pragma unroll
+  for (int e = 0; e < D / 8; ++e) o[e] = 0.f;
+  for (int k = c - 1; k <= last; ++k) {
+    const float* q = piece(k);
+    const float mk = __ldcg(q + 2 * kTile * D + row);
+    if (mk == -INFINITY) continue;
+    const float f = ex2(mk - M);
+    L += f * __ldcg(q + 2 * kTile * D + 2 * kTile + row);
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(q + (size_t)row * D + d0 + 4 * e));
+      o[4 * e] += f * v.x;
+      o[4 * e + 1] += f * v.y;
+      o[4 * e + 2] += f * v.z;
+      o[4 * e + 3] += f * v.w;
+    }
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  bf16* out = (bf16*)a.out + (int64_t)(p.s.q0 + s_tok) * a.ldo + (int64_t)(pl.h * G + r % G) * a.hdo + d0;
+#pragma unroll
+  for (int e = 0; e < D / 64; ++e)
+    *reinterpret_cast<uint4*>(out + 8 * e) =
+        make_uint4(bf16_pair(o[8 * e] * inv, o[8 * e + 1] * inv), bf16_pair(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
+                   bf16_pair(o[8 * e + 4] * inv, o[8 * e + 5] * inv), bf16_pair(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
+}
+
+int extend_grid() { return usable_sms(); }
+
+template <int D, bool E4>
+cudaError_t launch_extend(const PagedAttnArgs& a, cudaStream_t s) {
+  PoolMaps maps{};
+  if (!E4 && !pool_maps<D, false>(&maps, a.pool)) return cudaErrorInvalidValue;
+  const int G = a.nq / a.pool.nkv, tq = kTile / G;
+  CUtensorMap tq_map;
+  {
+    const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)a.nq, (cuuint64_t)a.batch.T};
+    const cuuint64_t strides[2] = {(cuuint64_t)a.hdq * 2, (cuuint64_t)a.ldq * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)tq};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    if (tc_host::encoder()(&tq_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(a.q), dims, strides, box,
+                           estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return cudaErrorInvalidValue;
+  }
+  auto kernel = paged_extend_kernel<D, E4>;
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!configured[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemE);
+    if (e != cudaSuccess) return e;
+    configured[dev] = true;
+  }
+  const int grid = extend_grid();
+  cudaError_t e = launch_pdl(kernel, dim3(grid), dim3(Roles<E4>::kThreads), ExtendLayout<D>::bytes(a.batch.B), s, maps,
+                             tq_map, a);
+  if (e != cudaSuccess || grid == 1) return e;
+  return launch_pdl(paged_extend_join_kernel<D>, dim3(grid - 1, 2 * kTile / 32), dim3(256),
+                    (a.batch.B + 1) * sizeof(int), s, a, grid);
+}
+
+}  // namespace
+
+size_t paged_extend_workspace(const PagedAttnArgs& a) {
+  return (size_t)2 * extend_grid() * (a.pool.D == 128 ? partial_floats<128>() : partial_floats<64>()) * sizeof(float);
+}
+
+cudaError_t launch_paged_extend(const PagedAttnArgs& a, cudaStream_t s) {
+  const bool e4 = a.pool.cdtype == kE4M3;
+  if (a.pool.D == 128) return e4 ? launch_extend<128, true>(a, s) : launch_extend<128, false>(a, s);
+  return e4 ? launch_extend<64, true>(a, s) : launch_extend<64, false>(a, s);
+}
+
+}  // namespace mg

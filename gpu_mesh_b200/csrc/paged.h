@@ -82,6 +82,10 @@ constexpr int kPagedFewRows = 16;
 bool paged_decode_applicable(const PagedAttnArgs& a);
 size_t paged_decode_workspace(const PagedAttnArgs& a);
 cudaError_t launch_paged_decode(const PagedAttnArgs& a, cudaStream_t s);
+// Tensor-core kernel for the sequences with more (k_paged_extend.cu), on the
+// same types and head sizes.
+size_t paged_extend_workspace(const PagedAttnArgs& a);
+cudaError_t launch_paged_extend(const PagedAttnArgs& a, cudaStream_t s);
 cudaError_t launch_paged_attention(const PagedAttnArgs& a, cudaStream_t s);
 
 #ifdef __CUDACC__
