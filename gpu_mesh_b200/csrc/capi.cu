@@ -1365,13 +1365,15 @@ int paged_args(const mg_paged_pool* p, const mg_paged_batch* b, int32_t dtype, i
     return fail(MG_EINVAL, "num_q_heads must be 1 to 16 times num_kv_heads (%d and %d)", nq, p->num_kv_heads);
   const bool e4m3 = p->cache_dtype == MG_DTYPE_E4M3;
   if (e4m3 && (!p->k_scale || !p->v_scale)) return fail(MG_EINVAL, "e4m3 pages need k_scale and v_scale");
-  if (e4m3 && (p->k_scale_stride < p->num_kv_heads || p->v_scale_stride < p->num_kv_heads))
+  if (e4m3 && p->num_pages > 1 && (p->k_scale_stride < p->num_kv_heads || p->v_scale_stride < p->num_kv_heads))
     return fail(MG_EINVAL, "scale rows must hold num_kv_heads entries");
   const int esz = e4m3 ? 1 : dtype == MG_DTYPE_BF16 ? 2 : 4;
   const int64_t unit = std::min(16, D * esz) / esz;  // elements that a row starts on a multiple of
-  const int64_t st[] = {p->k_page_stride, p->k_head_stride, p->k_token_stride,
-                        p->v_page_stride, p->v_head_stride, p->v_token_stride};
-  for (int64_t x : st)
+  // The stride between a single page, or a single head, means nothing.
+  const bool one_page = p->num_pages == 1, one_head = p->num_kv_heads == 1;
+  const int64_t kp = one_page ? D : p->k_page_stride, kh = one_head ? D : p->k_head_stride;
+  const int64_t vp = one_page ? D : p->v_page_stride, vh = one_head ? D : p->v_head_stride;
+  for (int64_t x : {kp, kh, p->k_token_stride, vp, vh, p->v_token_stride})
     if (x < D || x % unit) return fail(MG_EINVAL, "page, head and token strides must be at least head_dim and multiples of 16 bytes");
   if ((uintptr_t)p->k % (unit * esz) || (uintptr_t)p->v % (unit * esz))
     return fail(MG_EINVAL, "pages must start on 16-byte boundaries");
@@ -1385,8 +1387,7 @@ int paged_args(const mg_paged_pool* p, const mg_paged_batch* b, int32_t dtype, i
     if (b->batch > 1 && b->table_stride < b->max_pages) return fail(MG_EINVAL, "table_stride is below max_pages");
   }
   *pool = PagedPool{p->k, p->v, p->k_scale, p->v_scale,
-                    p->k_page_stride, p->k_head_stride, p->k_token_stride,
-                    p->v_page_stride, p->v_head_stride, p->v_token_stride,
+                    kp, kh, p->k_token_stride, vp, vh, p->v_token_stride,
                     p->k_scale_stride, p->v_scale_stride,
                     p->num_pages, ps, p->num_kv_heads, D, p->cache_dtype};
   *batch = PagedBatch{b->page_table, b->table_stride, b->max_pages, b->q_start, b->kv_len, b->batch, b->tokens,
@@ -1408,6 +1409,7 @@ int mg_paged_append(const mg_paged_pool* pool, const mg_paged_batch* batch, int3
   if (a.batch.B == 0 || a.batch.T == 0) return MG_OK;
   if (!qkv || !q_out) return fail(MG_EINVAL, "null qkv or q_out");
   const int64_t vec = dtype == MG_DTYPE_BF16 ? 8 : 4, D = a.pool.D;
+  if (a.batch.T == 1) ld_qkv = (num_q_heads + 2LL * a.pool.nkv) * D, ld_q = num_q_heads * D;
   if (ld_qkv < (num_q_heads + 2LL * a.pool.nkv) * D || ld_qkv % vec || ld_q < num_q_heads * D || ld_q % vec)
     return fail(MG_EINVAL, "qkv and q_out rows must hold every head and be multiples of 16 bytes apart");
   if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(q_norm) || !aligned16(k_norm) || !aligned16(cos) || !aligned16(sin))
@@ -1454,6 +1456,8 @@ int mg_paged_attention(const mg_paged_pool* pool, const mg_paged_batch* batch, i
   if (a.batch.B == 0 || a.batch.T == 0) return MG_OK;
   if (!q || !out) return fail(MG_EINVAL, "null q or out");
   const int64_t vec = dtype == MG_DTYPE_BF16 ? 8 : 4, D = a.pool.D;
+  if (a.batch.T == 1) q_token_stride = out_token_stride = D;
+  if (num_q_heads == 1) q_head_stride = out_head_stride = D;
   for (int64_t x : {q_token_stride, q_head_stride, out_token_stride, out_head_stride})
     if (x < D || x % vec)
       return fail(MG_EINVAL, "token and head strides of q and out must be at least head_dim and multiples of 16 bytes");

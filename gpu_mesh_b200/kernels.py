@@ -32,7 +32,7 @@ pool, a length outside the table) leaves that sequence out and is raised by ``pa
 """
 from __future__ import annotations
 
-import math
+import contextlib
 
 import torch
 
@@ -74,15 +74,8 @@ _PAGED_DT = {torch.float32: _lib.MG_DTYPE_F32, torch.bfloat16: _lib.MG_DTYPE_BF1
              torch.float8_e4m3fn: _lib.MG_DTYPE_E4M3}
 
 
-def _index(name: str, t: torch.Tensor, device: torch.device, ndim: int, dtype: torch.dtype = torch.int32) -> None:
-    if t.dtype != dtype or t.ndim != ndim or t.device != device:
-        raise ValueError(f"{name} must be a {ndim}-D {dtype} tensor on {device}")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{name} rows must be contiguous")
-
-
-def _paged(x, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale, max_new):
-    """The C structures of a pool and a batch, checked against the activations ``x``."""
+def _refuse(x, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale) -> None:
+    """Raise for what ``_paged`` found wrong; return where it was only the stride of a dimension of one element."""
     dev = x.device
     if x.dtype not in _DT or dev.type != "cuda":
         raise ValueError("the paged operators need CUDA fp32 or bf16 activations")
@@ -92,43 +85,76 @@ def _paged(x, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale, m
         raise ValueError("the pages must be on the activations' device")
     if k_pages.dtype != x.dtype and k_pages.dtype != torch.float8_e4m3fn:
         raise ValueError("the pages must hold the activation dtype or torch.float8_e4m3fn")
-    if k_pages.stride(3) != 1 or v_pages.stride(3) != 1:
+    if k_pages.shape[3] > 1 and (k_pages.stride(3) != 1 or v_pages.stride(3) != 1):
         raise ValueError("head_dim must be contiguous in the pages")
-    pages, nkv, ps, D = k_pages.shape
-    scales = (None, None, 0, 0)
     if k_pages.dtype == torch.float8_e4m3fn:
         for s in (k_scale, v_scale):
-            if s is None or s.dtype != torch.float32 or s.device != dev or s.shape != (pages, nkv) or \
-                    (nkv > 1 and s.stride(1) != 1):
+            if s is None or s.dtype != torch.float32 or s.device != dev or s.shape != k_pages.shape[:2] or \
+                    (s.shape[1] > 1 and s.stride(1) != 1):
                 raise ValueError("e4m3 pages need fp32 k_scale and v_scale [pages, kv heads] on their device")
-        scales = (k_scale.data_ptr(), v_scale.data_ptr(), max(k_scale.stride(0), nkv), max(v_scale.stride(0), nkv))
-        if pages > 1 and (k_scale.stride(0) < nkv or v_scale.stride(0) < nkv):
-            raise ValueError("scale rows of two pages must not overlap")
     elif k_scale is not None or v_scale is not None:
         raise ValueError("only e4m3 pages have scales")
-    _index("page_table", page_table, dev, 2)
-    _index("q_start", q_start, dev, 1)
-    _index("kv_len", kv_len, dev, 1)
-    B = kv_len.shape[0]
-    if page_table.shape[0] != B or q_start.shape[0] != B + 1:
+    for name, t, ndim in (("page_table", page_table, 2), ("q_start", q_start, 1), ("kv_len", kv_len, 1)):
+        if t.dtype != torch.int32 or t.ndim != ndim or t.device != dev:
+            raise ValueError(f"{name} must be a {ndim}-D torch.int32 tensor on {dev}")
+        if t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise ValueError(f"{name} rows must be contiguous")
+    if page_table.shape[0] != kv_len.shape[0] or q_start.shape[0] != kv_len.shape[0] + 1:
         raise ValueError("page_table, q_start and kv_len disagree on the number of sequences")
-    if max_new is None:
-        max_new = x.shape[0]
+
+
+def _paged(x, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale, max_new):
+    """The C structures of a pool and a batch, checked against the activations ``x``.
+
+    Decode steps call this twice per layer, so each tensor property is read once and the checks are one expression;
+    ``_refuse`` then names what it found."""
+    dev, kd, shape = x.device, k_pages.dtype, k_pages.shape
+    ks, vs = k_pages.stride(), v_pages.stride()
+    e4m3 = kd is torch.float8_e4m3fn
+    B = kv_len.shape[0] if kv_len.ndim == 1 else -1
+    if not (x.is_cuda and x.dtype in _DT and len(shape) == 4 and v_pages.shape == shape and v_pages.dtype is kd
+            and (e4m3 or kd is x.dtype) and k_pages.device == dev and v_pages.device == dev
+            and ks[3] == 1 and vs[3] == 1
+            and page_table.dtype is torch.int32 and q_start.dtype is torch.int32 and kv_len.dtype is torch.int32
+            and page_table.device == dev and q_start.device == dev and kv_len.device == dev
+            and page_table.ndim == 2 and page_table.shape[0] == B and page_table.stride(1) == 1
+            and q_start.shape == (B + 1,) and q_start.stride(0) == 1 and kv_len.stride(0) == 1):
+        _refuse(x, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale)
+    pages, nkv, ps, D = shape
+    if e4m3:
+        if not (k_scale is not None and v_scale is not None and k_scale.dtype is torch.float32
+                and v_scale.dtype is torch.float32 and k_scale.device == dev and v_scale.device == dev
+                and k_scale.shape == (pages, nkv) and v_scale.shape == (pages, nkv)
+                and k_scale.stride(1) == 1 and v_scale.stride(1) == 1):
+            _refuse(x, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale)
+        scales = (k_scale.data_ptr(), v_scale.data_ptr(), k_scale.stride(0), v_scale.stride(0))
+    else:
+        if k_scale is not None or v_scale is not None:
+            _refuse(x, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale)
+        scales = (None, None, 0, 0)
+    T = x.shape[0]
+    if max_new is None or max_new > T:
+        max_new = T
     elif max_new < 0:
         raise ValueError("max_new must not be negative")
-    pool = _lib.PagedPool(
-        k_pages.data_ptr(), v_pages.data_ptr(), scales[0], scales[1],
-        _stride(k_pages, 0), _stride(k_pages, 1), _stride(k_pages, 2),
-        _stride(v_pages, 0), _stride(v_pages, 1), _stride(v_pages, 2), scales[2], scales[3],
-        pages, ps, nkv, D, _PAGED_DT[k_pages.dtype])
+    pool = _lib.PagedPool(k_pages.data_ptr(), v_pages.data_ptr(), scales[0], scales[1], ks[0], ks[1], ks[2],
+                          vs[0], vs[1], vs[2], scales[2], scales[3], pages, ps, nkv, D, _PAGED_DT[kd])
     batch = _lib.PagedBatch(page_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), page_table.stride(0),
-                            B, x.shape[0], page_table.shape[1], min(max_new, x.shape[0]))
+                            B, T, page_table.shape[1], max_new)
     return pool, batch
 
 
-def _stride(t: torch.Tensor, dim: int) -> int:
-    """The stride of a dimension; of one element, whose stride means nothing, the one that a dense tensor has."""
-    return t.stride(dim) if t.shape[dim] > 1 else max(1, math.prod(t.shape[dim + 1:]))
+_HERE = contextlib.nullcontext()
+
+
+def _current(index: int):
+    """Makes device ``index`` current, at no cost where it is already."""
+    return _HERE if torch.cuda.current_device() == index else torch.cuda.device(index)
+
+
+# The current stream's handle, without the Stream object that torch.cuda.current_stream builds.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -150,34 +176,40 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     dev, nkv, D = qkv.device, pool.num_kv_heads, pool.head_dim
     if qkv.ndim != 2 or num_q_heads < 1 or qkv.shape[1] != (num_q_heads + 2 * nkv) * D:
         raise ValueError("qkv must be [T, (num_q_heads + 2 kv heads) * head_dim]")
-    if qkv.stride(1) != 1:
+    T, (ld, inner) = qkv.shape[0], qkv.stride()
+    if inner != 1 and qkv.shape[1] > 1:
         raise ValueError("qkv rows must be contiguous")
-    if (cos is None) != (sin is None):
-        raise ValueError("cos and sin come together")
-    for name, t in (("cos", cos), ("sin", sin)):
-        if t is not None and (t.dtype != torch.float32 or t.device != dev or t.ndim != 2 or t.shape[1] != D // 2
-                              or t.shape != cos.shape or not t.is_contiguous()):
-            raise ValueError(f"{name} must be a contiguous fp32 [positions, head_dim / 2] table on {dev}")
-    for name, t in (("q_norm", q_norm), ("k_norm", k_norm)):
-        if t is not None and (t.dtype != qkv.dtype or t.device != dev or t.shape != (D,) or not t.is_contiguous()):
-            raise ValueError(f"{name} must be a contiguous [head_dim] tensor in the activation dtype")
-    T = qkv.shape[0]
+    c = sn = qn = kn = pos = None
+    max_pos = 0
+    if cos is not None or sin is not None:
+        if cos is None or sin is None:
+            raise ValueError("cos and sin come together")
+        for name, t in (("cos", cos), ("sin", sin)):
+            if t.dtype is not torch.float32 or t.device != dev or t.ndim != 2 or t.shape[1] * 2 != D or \
+                    t.shape != cos.shape or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous fp32 [positions, head_dim / 2] table on {dev}")
+        c, sn, max_pos = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
+    if q_norm is not None or k_norm is not None:
+        for name, t in (("q_norm", q_norm), ("k_norm", k_norm)):
+            if t is not None and (t.dtype is not qkv.dtype or t.device != dev or t.shape != (D,) or t.stride(0) != 1):
+                raise ValueError(f"{name} must be a contiguous [head_dim] tensor in the activation dtype")
+        qn = None if q_norm is None else q_norm.data_ptr()
+        kn = None if k_norm is None else k_norm.data_ptr()
     if positions is not None:
-        _index("positions", positions, dev, 1, torch.int64)
-        if positions.shape[0] != T:
-            raise ValueError("positions must have one entry per token row")
+        if positions.dtype is not torch.int64 or positions.shape != (T,) or positions.device != dev or \
+                (T > 1 and positions.stride(0) != 1):
+            raise ValueError("positions must be contiguous int64 with one entry per token row")
+        pos = positions.data_ptr()
     if out is None:
-        out = torch.empty(T, num_q_heads, D, dtype=qkv.dtype, device=dev)
+        out = qkv.new_empty((T, num_q_heads, D))
     elif out.shape != (T, num_q_heads, D) or out.dtype != qkv.dtype or out.device != dev or \
             out.stride(2) != 1 or (num_q_heads > 1 and out.stride(1) != D):
         raise ValueError("out must be [T, num_q_heads, head_dim] with contiguous token rows")
-    with torch.cuda.device(dev):
+    index = dev.index
+    with _current(index):
         _lib.check(_lib.lib().mg_paged_append(
-            pool, batch, _DT[qkv.dtype], qkv.data_ptr(), _stride(qkv, 0), num_q_heads,
-            None if positions is None else positions.data_ptr(), None if cos is None else cos.data_ptr(),
-            None if sin is None else sin.data_ptr(), 0 if cos is None else cos.shape[0],
-            None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(),
-            eps, out.data_ptr(), _stride(out, 0), torch.cuda.current_stream(dev).cuda_stream))
+            pool, batch, _DT[qkv.dtype], qkv.data_ptr(), ld, num_q_heads, pos, c, sn, max_pos, qn, kn, eps,
+            out.data_ptr(), out.stride(0), _raw_stream(index)))
     return out
 
 
@@ -198,17 +230,19 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if q.shape[2] != pool.head_dim:
         raise ValueError("q and the pages disagree on head_dim")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out = q.new_empty(q.shape)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1:
         raise ValueError("out must have q's shape and dtype, with head_dim contiguous")
-    lib, dt = _lib.lib(), _DT[q.dtype]
-    with torch.cuda.device(dev):
-        need = lib.mg_paged_attention_workspace(pool, batch, dt, nq)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    lib, dt, index = _lib.lib(), _DT[q.dtype], dev.index
+    (ql, qh, _), (ol, oh, _) = q.stride(), out.stride()
+    with _current(index):
+        need, ws = lib.mg_paged_attention_workspace(pool, batch, dt, nq), None
+        if need:
+            scratch = q.new_empty(need, dtype=torch.uint8)
+            ws = scratch.data_ptr()
         _lib.check(lib.mg_paged_attention(
-            pool, batch, dt, q.data_ptr(), _stride(q, 0), _stride(q, 1), nq,
-            pool.head_dim ** -0.5 if scale is None else scale, out.data_ptr(), _stride(out, 0), _stride(out, 1),
-            None if ws is None else ws.data_ptr(), need, torch.cuda.current_stream(dev).cuda_stream))
+            pool, batch, dt, q.data_ptr(), ql, qh, nq, pool.head_dim ** -0.5 if scale is None else scale,
+            out.data_ptr(), ol, oh, ws, need, _raw_stream(index)))
     return out
 
 

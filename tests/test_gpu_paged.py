@@ -455,6 +455,25 @@ def test_python_refusals():
             app(**kw)
 
 
+def test_strides_of_single_elements_do_not_matter():
+    """One row, one head, one page: their strides may hold anything."""
+    for cache in (BF16, E4M3):
+        c = Cache([9], 1, 16, 64, BF16, cache, spare=0)
+        c.fill([8])
+        qkv = torch.randn(1, 3 * 64, device=DEV).to(BF16)
+        want = kernels.paged_append(qkv, c.k, c.v, c.table.to(DEV), dev32([0, 1]), dev32([9]), num_q_heads=1, **c.scales())
+        odd = lambda t, dims: t.as_strided(t.shape, [s if n > 1 else 3 for n, s in zip(t.shape, t.stride())][:dims])  # noqa: E731
+        k, v = odd(c.k, 4), odd(c.v, 4)
+        sc = {} if c.ks is None else {"k_scale": odd(c.ks, 2), "v_scale": odd(c.vs, 2)}
+        args = (odd(c.table[:, :1].contiguous().to(DEV), 2), dev32([0, 1]), dev32([9, 0])[::2])
+        got = kernels.paged_append(odd(qkv, 2), k, v, *args, num_q_heads=1, **sc)
+        assert torch.equal(got, want)
+        a = kernels.paged_attention(want, c.k, c.v, c.table.to(DEV), dev32([0, 1]), dev32([9]), **c.scales())
+        b = kernels.paged_attention(odd(want, 3), k, v, *args, **sc)
+        assert torch.equal(a, b)
+    kernels.paged_check_device()
+
+
 def test_empty_calls():
     c = Cache([20], 2, 16, 64, BF16, E4M3)
     t = c.table.to(DEV)
