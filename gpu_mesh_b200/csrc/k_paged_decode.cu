@@ -14,9 +14,10 @@
 //     time (lane = (chunk, page)), ahead of their use, and requests each page
 //     with 4-D TMA into a ring of stages; a sequence's last page comes in
 //     16-token slices, so at most 15 invisible tokens are read.
-//   * Compute.  Transposed products, so that the query rows sit on the MMA's
-//     N = 8 side: Sᵀ = K·Qᵀ (M = a warp's 16 keys), Oᵀ = Vᵀ·Pᵀ (M = 16 dims),
-//     fp32 accumulators, online softmax in base 2.
+//   * Compute.  Two groups of four warps take chunks in turn, 32 keys a warp.
+//     Transposed products, so that the query rows sit on the MMA's N = 8
+//     side: Sᵀ = K·Qᵀ (M = 16 keys), Oᵀ = Vᵀ·Pᵀ (M = 16 dims), fp32
+//     accumulators, online softmax in base 2.
 //       bf16 pages: bf16 MMAs, P split into bf16 high + low parts (2^-17).
 //       e4m3 pages: codes become halves in registers (exact), Q as halves
 //       scaled by a power of two per row (exact), K's scale multiplies the
@@ -43,10 +44,13 @@ using namespace tc;
 using namespace attn;
 using namespace paged;
 
-constexpr int kWarps = 8;                     // consumer warps
+constexpr int kWarps = 8;                     // consumer warps, in two groups that take chunks in turn
+constexpr int kGroup = kWarps / 2;            // warps of a group
 constexpr int kThreadsD = (kWarps + 1) * 32;  // + the producer warp
-constexpr int kKeysW = 16;                    // keys per consumer warp
-constexpr int kChunkD = kWarps * kKeysW;      // keys per unit (128)
+constexpr int kKeysW = 32;                    // keys per consumer warp
+constexpr int kSub = kKeysW / 16;             // its 16-key tiles
+constexpr int kChunkD = kGroup * kKeysW;      // keys per unit (128)
+constexpr int kSnap = 4;                      // units a run's end moves to end with a (sequence, head)
 constexpr int kMaxStagesD = 8;
 constexpr int kSmemD = 227 * 1024;
 constexpr int kRowsD = 16;                    // most query rows of a (sequence, head)
@@ -74,13 +78,14 @@ __device__ __forceinline__ int decode_chunks(const SeqSpan& s, int G) {
   return len > 0 ? (len + kChunkD - 1) / kChunkD : 1;  // no keys at all: one unit that writes zeros
 }
 
-// Equal runs of `total` units over `grid` CTAs, none of them empty.
+// Runs of the `total` units over `grid` CTAs: equal ones, but for ends that
+// lie within kSnap units of a (sequence, head)'s end and move there, which
+// saves a cut (an empty run is possible then).
 struct Runs {
   long long total;
   int grid;
   __device__ Runs(long long n, int most) : total(n), grid((int)(n < most ? n : most)) {}
-  __device__ long long begin(int c) const { return (long long)c * total / grid; }
-  __device__ int owner(long long u) const { return (int)(((u + 1) * grid - 1) / total); }
+  __device__ long long raw(int c) const { return (long long)c * total / grid; }
 };
 
 // Shared memory: `stages` ring stages (K, V, the piece's query rows, the
@@ -131,8 +136,8 @@ __global__ void __launch_bounds__(kThreadsD, 1)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) {
     for (int s = 0; s < stages; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], kWarps);
+      mbar_init(&full[s], E4 ? 2 : 1);  // the loads, and the scales
+      mbar_init(&empty[s], kGroup);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -175,7 +180,6 @@ __global__ void __launch_bounds__(kThreadsD, 1)
   const Runs runs(pre[bt.B], (int)gridDim.x);
   const int c = blockIdx.x;
   if (c >= runs.grid) return;
-  const int u0 = (int)runs.begin(c), u1 = (int)runs.begin(c + 1);
   // The sequence that unit u belongs to.
   auto seq_of = [&](int u) {
     int lo = 0, hi = bt.B;  // pre[lo] <= u < pre[hi]
@@ -185,6 +189,14 @@ __global__ void __launch_bounds__(kThreadsD, 1)
     }
     return lo;
   };
+  auto begin = [&](int k) {
+    const int u = (int)runs.raw(k);
+    if (u >= (int)runs.total) return u;
+    const int b = seq_of(u), C = max(1, (slen[b] + kChunkD - 1) / kChunkD), off = (u - pre[b]) % C;
+    return off <= kSnap ? u - off : C - off <= kSnap ? u + C - off : u;
+  };
+  const int u0 = begin(c), u1 = begin(c + 1);
+  if (u0 >= u1) return;
 
   if (warp == kWarps) {
     const int ppc = kChunkD / pool.ps;  // pages per chunk
@@ -238,20 +250,17 @@ __global__ void __launch_bounds__(kThreadsD, 1)
         uint8_t* st = smem + s * lay.stage;
         const bool mine = (lane >> 3) == j && f.keys > 0;
         const int nsl = (f.keys + kSlice - 1) / kSlice;  // 16-token slices that hold keys
-        uint32_t bytes = mine ? 2u * nsl * kSlice * Row::kRowBytes : 0u;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) bytes += __shfl_xor_sync(0xffffffffu, bytes, o);
         const int src = j * 8;
         const int b = __shfl_sync(0xffffffffu, f.b, src), h = __shfl_sync(0xffffffffu, f.h, src);
         const int chunk = __shfl_sync(0xffffffffu, f.chunk, src);
         const int qn = sqn[b], rows = (qn & 31) * G;
-        const bool with_q = chunk == 0 || n == 0;  // the piece's first chunk carries its query rows
-        if (E4 && (lane >> 3) == j) {
-          ((float*)(st + 2 * L::kKV))[lane & 7] = f.ks;
-          ((int*)(st + 2 * L::kKV))[8 + (lane & 7)] = scale_exp(f.vs);
+        // The query rows come with the first chunk that each warp group sees of a piece.
+        const bool with_q = chunk <= 1 || n <= 1;
+        if (lane == 0) {
+          const int keys = min(kChunkD, slen[b] - chunk * kChunkD);
+          mbar_expect_tx(&full[s], 2u * ((max(keys, 0) + kSlice - 1) / kSlice) * kSlice * Row::kRowBytes +
+                                       (with_q ? (uint32_t)rows * D * 2 : 0u));
         }
-        __syncwarp();
-        if (lane == 0) mbar_expect_tx(&full[s], bytes + (with_q ? (uint32_t)rows * D * 2 : 0u));
         __syncwarp();
         if (mine) {
           const int i = lane & 7;
@@ -277,6 +286,14 @@ __global__ void __launch_bounds__(kThreadsD, 1)
           bulk_load(st + 2 * L::kKV + L::kScales + lane * D * 2,
                     (const __nv_bfloat16*)a.q + (int64_t)((qn >> 5) + lane / G) * a.ldq + (int64_t)(h * G + lane % G) * a.hdq,
                     D * 2, &full[s]);
+        if constexpr (E4) {
+          if ((lane >> 3) == j) {
+            ((float*)(st + 2 * L::kKV))[lane & 7] = f.ks;
+            ((int*)(st + 2 * L::kKV))[8 + (lane & 7)] = scale_exp(f.vs);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full[s]);
+        }
       }
       fetch_scales(next);
     }
@@ -288,6 +305,8 @@ __global__ void __launch_bounds__(kThreadsD, 1)
     }
   } else {
     const int g = lane >> 2, t = lane & 3;
+    const int grp = warp / kGroup, wk = warp % kGroup;
+    const int page_shift = 31 - __clz(pool.ps);
     const float scale2 = a.scale * 1.4426950408889634f;
     int n = 0;
     bool stop = false;  // set by a vote only, so that all warps leave together
@@ -319,12 +338,15 @@ __global__ void __launch_bounds__(kThreadsD, 1)
       }
       const int least = past + 1;  // keys that every row sees
       uint32_t qb[NT][KS][2];
+      bool have_q = false;
       for (int uc = u; uc < ue; ++uc, ++n) {
+        if ((n & 1) != grp) continue;
         const int s = n % stages;
         if (!mbar_wait(&full[s], (n / stages) & 1, a.err)) *abort_flag = 1;
         if (*abort_flag) break;  // the vote at the end of the piece stops every warp
         uint8_t* st = smem + s * lay.stage;
-        if (uc == u) {
+        if (!have_q) {
+          have_q = true;
           const __nv_bfloat16* Qs = (const __nv_bfloat16*)(st + 2 * L::kKV + L::kScales);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
@@ -360,139 +382,176 @@ __global__ void __launch_bounds__(kThreadsD, 1)
             }
           }
         }
-        const int j0 = (uc - pu) * kChunkD + warp * kKeysW;  // the warp's first key
+        const int j0 = (uc - pu) * kChunkD + wk * kKeysW;  // the warp's first key
         const int nk = min(kKeysW, len - j0);
         if (nk > 0) {
-          float ksc = 1.f;
-          int ve = 0;
-          if constexpr (E4) {
-            const int pg = warp * kKeysW / pool.ps;
-            ksc = ((const float*)(st + 2 * L::kKV))[pg];
-            ve = ((const int*)(st + 2 * L::kKV))[8 + pg];
-          }
-          float sc[NT][4];
+          float ksc[kSub];
+          int ve[kSub];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+          for (int u2 = 0; u2 < kSub; ++u2) {
+            ksc[u2] = 1.f;
+            ve[u2] = 0;
+            if constexpr (E4) {
+              const int pg = (wk * kKeysW + 16 * u2) >> page_shift;
+              ksc[u2] = ((const float*)(st + 2 * L::kKV))[pg];
+              ve[u2] = ((const int*)(st + 2 * L::kKV))[8 + pg];
+            }
+          }
+          float sc[NT][kSub][4];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int u2 = 0; u2 < kSub; ++u2) sc[nt][u2][0] = sc[nt][u2][1] = sc[nt][u2][2] = sc[nt][u2][3] = 0.f;
           const uint32_t kbase = smem_u32(st);
-          const int kr = warp * kKeysW + (lane & 7) + 8 * ((lane >> 3) & 1);
+          const int kr = wk * kKeysW + (lane & 7) + 8 * ((lane >> 3) & 1);
           if constexpr (E4) {
 #pragma unroll
             for (int jj = 0; jj < KS / 2; ++jj) {
-              uint32_t x[4];
-              ldsm_x4(kbase + Row::at(kr, 2 * jj + (lane >> 4)), x);
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const uint32_t a0 = e4m3x2_to_f16x2(x[2 * e]), a1 = e4m3x2_to_f16x2(x[2 * e + 1]);
-                const uint32_t a2 = e4m3x2_hi_to_f16x2(x[2 * e]), a3 = e4m3x2_hi_to_f16x2(x[2 * e + 1]);
+              for (int u2 = 0; u2 < kSub; ++u2) {
+                uint32_t x[4];
+                ldsm_x4(kbase + Row::at(kr + 16 * u2, 2 * jj + (lane >> 4)), x);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-                  mma16816_f16(sc[nt], a0, a1, a2, a3, qb[nt][2 * jj + e][0], qb[nt][2 * jj + e][1]);
+                for (int e = 0; e < 2; ++e) {
+                  const uint32_t a0 = e4m3x2_to_f16x2(x[2 * e]), a1 = e4m3x2_to_f16x2(x[2 * e + 1]);
+                  const uint32_t a2 = e4m3x2_hi_to_f16x2(x[2 * e]), a3 = e4m3x2_hi_to_f16x2(x[2 * e + 1]);
+#pragma unroll
+                  for (int nt = 0; nt < NT; ++nt)
+                    mma16816_f16(sc[nt][u2], a0, a1, a2, a3, qb[nt][2 * jj + e][0], qb[nt][2 * jj + e][1]);
+                }
               }
             }
           } else {
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
               const int cc = 2 * ks + (lane >> 4);
-              uint32_t x[4];
-              ldsm_x4(kbase + (cc >> 3) * L::kBlock + Row::at(kr, cc & 7), x);
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-                mma16816_full(sc[nt], x[0], x[1], x[2], x[3], qb[nt][ks][0], qb[nt][ks][1]);
+              for (int u2 = 0; u2 < kSub; ++u2) {
+                uint32_t x[4];
+                ldsm_x4(kbase + (cc >> 3) * L::kBlock + Row::at(kr + 16 * u2, cc & 7), x);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                  mma16816_full(sc[nt][u2], x[0], x[1], x[2], x[3], qb[nt][ks][0], qb[nt][ks][1]);
+              }
             }
           }
-          // Online softmax per query row (column): keys g (c0, c1), g + 8 (c2, c3).
-          uint32_t ph[NT][2], plo[NT][2];
+          // Online softmax per query row (column): keys g (c0, c1), g + 8 (c2, c3) of each tile.
+          uint32_t ph[NT][kSub][2], plo[NT][kSub][2];
           const bool clear = j0 + kKeysW <= least;  // every key of the warp is visible to every row
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            float p[4], mx[2], keep[2];
+            float mx[2] = {mrow[nt][0], mrow[nt][1]};
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float f = rowf[nt][e] * ksc;
-              p[e] = sc[nt][e] * f;
-              p[2 + e] = sc[nt][2 + e] * f;
-              if constexpr (E4) {
-                p[e] += (float)ve;
-                p[2 + e] += (float)ve;
+            for (int u2 = 0; u2 < kSub; ++u2) {
+              float* p = sc[nt][u2];
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float f = rowf[nt][e] * ksc[u2];
+                p[e] = E4 ? fmaf(p[e], f, (float)ve[u2]) : p[e] * f;
+                p[2 + e] = E4 ? fmaf(p[2 + e], f, (float)ve[u2]) : p[2 + e] * f;
+                if (!clear) {
+                  p[e] = j0 + 16 * u2 + g < vis[nt][e] ? p[e] : -INFINITY;
+                  p[2 + e] = j0 + 16 * u2 + g + 8 < vis[nt][e] ? p[2 + e] : -INFINITY;
+                }
+                mx[e] = fmaxf(mx[e], fmaxf(p[e], p[2 + e]));
               }
-              if (!clear) {
-                p[e] = j0 + g < vis[nt][e] ? p[e] : -INFINITY;
-                p[2 + e] = j0 + g + 8 < vis[nt][e] ? p[2 + e] : -INFINITY;
-              }
-              mx[e] = fmaxf(mrow[nt][e], fmaxf(p[e], p[2 + e]));
             }
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) {
               mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], off));
               mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], off));
             }
+            if (__any_sync(0xffffffffu, mx[0] != mrow[nt][0] || mx[1] != mrow[nt][1])) {
+              float keep[2];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              // A row that has seen no key yet keeps m = -inf: every weight is 0.
-              const float base = mx[e] == -INFINITY ? 0.f : mx[e] - (E4 ? 14.f : 0.f);
-              keep[e] = mrow[nt][e] == -INFINITY ? 0.f : ex2(mrow[nt][e] - mx[e]);
-              mrow[nt][e] = mx[e];
-              p[e] = ex2(p[e] - base);
-              p[2 + e] = ex2(p[2 + e] - base);
-              const float add = p[e] + p[2 + e];
-              lrow[nt][e] = lrow[nt][e] * keep[e] + (E4 ? add * pow2i(-ve - 14) : add);
-            }
+              for (int e = 0; e < 2; ++e) {
+                keep[e] = mrow[nt][e] == -INFINITY ? 0.f : ex2(mrow[nt][e] - mx[e]);
+                mrow[nt][e] = mx[e];
+                lrow[nt][e] *= keep[e];
+              }
 #pragma unroll
-            for (int i = 0; i < DM; ++i) {
-              o[nt][i][0] *= keep[0];
-              o[nt][i][1] *= keep[1];
-              o[nt][i][2] *= keep[0];
-              o[nt][i][3] *= keep[1];
+              for (int i = 0; i < DM; ++i) {
+                o[nt][i][0] *= keep[0];
+                o[nt][i][1] *= keep[1];
+                o[nt][i][2] *= keep[0];
+                o[nt][i][3] *= keep[1];
+              }
             }
-            // Pᵀ as the B operand of Oᵀ += Vᵀ·Pᵀ: an 8x8 (keys x rows) matrix each, transposed in registers.
-            if constexpr (E4) {
-              ph[nt][0] = movm_trans(pack_f16(p[0], p[1]));
-              ph[nt][1] = movm_trans(pack_f16(p[2], p[3]));
-            } else {
-              const uint32_t h01 = pack2(p[0], p[1]), h23 = pack2(p[2], p[3]);
-              ph[nt][0] = movm_trans(h01);
-              ph[nt][1] = movm_trans(h23);
-              plo[nt][0] = movm_trans(pack2(p[0] - lo_bf16(h01), p[1] - hi_bf16(h01)));
-              plo[nt][1] = movm_trans(pack2(p[2] - lo_bf16(h23), p[3] - hi_bf16(h23)));
+            // A row that has seen no key yet keeps m = -inf: every weight is 0.
+            const float base0 = mx[0] == -INFINITY ? 0.f : mx[0] - (E4 ? 14.f : 0.f);
+            const float base1 = mx[1] == -INFINITY ? 0.f : mx[1] - (E4 ? 14.f : 0.f);
+#pragma unroll
+            for (int u2 = 0; u2 < kSub; ++u2) {
+              float* p = sc[nt][u2];
+              p[0] = ex2(p[0] - base0);
+              p[1] = ex2(p[1] - base1);
+              p[2] = ex2(p[2] - base0);
+              p[3] = ex2(p[3] - base1);
+              if constexpr (E4) {
+                const float w = pow2i(-ve[u2] - 14);
+                lrow[nt][0] = fmaf(p[0] + p[2], w, lrow[nt][0]);
+                lrow[nt][1] = fmaf(p[1] + p[3], w, lrow[nt][1]);
+                // Pᵀ as the B operand of Oᵀ += Vᵀ·Pᵀ: an 8x8 (keys x rows) matrix each, transposed in registers.
+                ph[nt][u2][0] = movm_trans(pack_f16(p[0], p[1]));
+                ph[nt][u2][1] = movm_trans(pack_f16(p[2], p[3]));
+              } else {
+                lrow[nt][0] += p[0] + p[2];
+                lrow[nt][1] += p[1] + p[3];
+                const uint32_t h01 = pack2(p[0], p[1]), h23 = pack2(p[2], p[3]);
+                ph[nt][u2][0] = movm_trans(h01);
+                ph[nt][u2][1] = movm_trans(h23);
+                plo[nt][u2][0] = movm_trans(pack2(p[0] - lo_bf16(h01), p[1] - hi_bf16(h01)));
+                plo[nt][u2][1] = movm_trans(pack2(p[2] - lo_bf16(h23), p[3] - hi_bf16(h23)));
+              }
             }
           }
           // Value rows behind the sequence can hold anything (P is 0 there,
           // but 0 · NaN is not): their halves of the fragments are cleared.
-          const int kk = 2 * t;
-          const uint32_t m01 = (kk < nk ? 0x0000ffffu : 0u) | (kk + 1 < nk ? 0xffff0000u : 0u);
-          const uint32_t m89 = (kk + 8 < nk ? 0x0000ffffu : 0u) | (kk + 9 < nk ? 0xffff0000u : 0u);
+          const bool full_keys = nk == kKeysW;
+          uint32_t m01[kSub], m89[kSub];
+#pragma unroll
+          for (int u2 = 0; u2 < kSub; ++u2) {
+            const int kk = 16 * u2 + 2 * t;
+            m01[u2] = (kk < nk ? 0x0000ffffu : 0u) | (kk + 1 < nk ? 0xffff0000u : 0u);
+            m89[u2] = (kk + 8 < nk ? 0x0000ffffu : 0u) | (kk + 9 < nk ? 0xffff0000u : 0u);
+          }
           const uint32_t vbase = smem_u32(st + L::kKV);
           if constexpr (E4) {
 #pragma unroll
             for (int jj = 0; jj < DM / 2; ++jj) {
-              uint32_t x[4];
-              ldsm_x4_t(vbase + Row::at(kr, 2 * jj + (lane >> 4)), x);
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                // bytes (key 2t: dims 2g, 2g + 1; key 2t + 1: the same) to one key pair per dim
-                const uint32_t y0 = __byte_perm(x[2 * e], 0u, 0x3120), y1 = __byte_perm(x[2 * e + 1], 0u, 0x3120);
-                const uint32_t a0 = e4m3x2_to_f16x2(y0) & m01, a1 = e4m3x2_hi_to_f16x2(y0) & m01;
-                const uint32_t a2 = e4m3x2_to_f16x2(y1) & m89, a3 = e4m3x2_hi_to_f16x2(y1) & m89;
+              for (int u2 = 0; u2 < kSub; ++u2) {
+                uint32_t x[4];
+                ldsm_x4_t(vbase + Row::at(kr + 16 * u2, 2 * jj + (lane >> 4)), x);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma16816_f16(o[nt][2 * jj + e], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
+                for (int e = 0; e < 2; ++e) {
+                  // bytes (key 2t: dims 2g, 2g + 1; key 2t + 1: the same) to one key pair per dim
+                  const uint32_t y0 = __byte_perm(x[2 * e], 0u, 0x3120), y1 = __byte_perm(x[2 * e + 1], 0u, 0x3120);
+                  uint32_t a0 = e4m3x2_to_f16x2(y0), a1 = e4m3x2_hi_to_f16x2(y0);
+                  uint32_t a2 = e4m3x2_to_f16x2(y1), a3 = e4m3x2_hi_to_f16x2(y1);
+                  if (!full_keys) a0 &= m01[u2], a1 &= m01[u2], a2 &= m89[u2], a3 &= m89[u2];
+#pragma unroll
+                  for (int nt = 0; nt < NT; ++nt)
+                    mma16816_f16(o[nt][2 * jj + e], a0, a1, a2, a3, ph[nt][u2][0], ph[nt][u2][1]);
+                }
               }
             }
           } else {
             const int mi = lane >> 3;
-            const int vr = warp * kKeysW + (lane & 7) + 8 * (mi >> 1);
+            const int vr = wk * kKeysW + (lane & 7) + 8 * (mi >> 1);
 #pragma unroll
             for (int dm = 0; dm < DM; ++dm) {
               const int cc = 2 * dm + (mi & 1);
-              uint32_t x[4];
-              ldsm_x4_t(vbase + (cc >> 3) * L::kBlock + Row::at(vr, cc & 7), x);
-              x[0] &= m01;
-              x[1] &= m01;
-              x[2] &= m89;
-              x[3] &= m89;
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                mma16816_full(o[nt][dm], x[0], x[1], x[2], x[3], ph[nt][0], ph[nt][1]);
-                mma16816_full(o[nt][dm], x[0], x[1], x[2], x[3], plo[nt][0], plo[nt][1]);
+              for (int u2 = 0; u2 < kSub; ++u2) {
+                uint32_t x[4];
+                ldsm_x4_t(vbase + (cc >> 3) * L::kBlock + Row::at(vr + 16 * u2, cc & 7), x);
+                if (!full_keys) x[0] &= m01[u2], x[1] &= m01[u2], x[2] &= m89[u2], x[3] &= m89[u2];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                  mma16816_full(o[nt][dm], x[0], x[1], x[2], x[3], ph[nt][u2][0], ph[nt][u2][1]);
+                  mma16816_full(o[nt][dm], x[0], x[1], x[2], x[3], plo[nt][u2][0], plo[nt][u2][1]);
+                }
               }
             }
           }
@@ -603,13 +662,18 @@ __global__ void __launch_bounds__(128) paged_decode_join_kernel(PagedAttnArgs a,
   pdl_wait();
   if (C == 0 || total_s >= 0x7fffffffLL) return;
   const Runs runs(total_s, grid);
+  // The ends of runs that cut this pair (none of them moved): c_lo + 1 .. c_hi.
   const long long p0 = before_s + (long long)h * C;
-  const int c_lo = runs.owner(p0), c_hi = runs.owner(p0 + C - 1);
+  if (C <= 2 * kSnap) return;
+  int c_lo = (int)((p0 + kSnap) * runs.grid / runs.total);  // the last run that begins at p0 + kSnap or before
+  while (c_lo + 1 < runs.grid && runs.raw(c_lo + 1) <= p0 + kSnap) ++c_lo;
+  while (c_lo > 0 && runs.raw(c_lo) > p0 + kSnap) --c_lo;
+  int c_hi = c_lo;
+  while (c_hi + 1 < runs.grid && runs.raw(c_hi + 1) < p0 + C - kSnap) ++c_hi;
   if (c_lo == c_hi) return;
   const int rows = sp.n * G, np = c_hi - c_lo + 1;
-  auto piece = [&](int k) {  // a CTA's first pair is its slot 0 if it began in an earlier CTA's run, else 1
-    return (const float*)a.ws + (size_t)(2 * (c_lo + k) + (p0 < runs.begin(c_lo + k) ? 0 : 1)) * kRowsD * (D + 2);
-  };
+  // A CTA's first pair is its slot 0 if an earlier run begins it, else slot 1.
+  auto piece = [&](int k) { return (const float*)a.ws + (size_t)(2 * (c_lo + k) + (k > 0 ? 0 : 1)) * kRowsD * (D + 2); };
   for (int i = tid; i < rows * np; i += 128) fac[i / np][i % np] = __ldcg(piece(i % np) + (i / np) * (D + 2));
   __syncthreads();
   if (tid < rows) {
@@ -665,8 +729,10 @@ cudaError_t launch_decode(const PagedAttnArgs& a, cudaStream_t s) {
   }
   const int rows = row_cap(a);
   const DecodeLayout<D, E4> lay(rows, a.batch.B);
+  // An even ring: a stage always belongs to the same warp group, whose waits
+  // then see every phase of its barriers.
   int stages = kMaxStagesD;
-  while (stages > 2 && lay.bytes(stages) > kSmemD) --stages;
+  while (stages > 2 && lay.bytes(stages) > kSmemD) stages -= 2;
   if (lay.bytes(stages) > kSmemD) return cudaErrorInvalidValue;
   const int grid = decode_grid(a);
   cudaError_t e = launch_pdl(kernel, dim3(grid), dim3(kThreadsD), lay.bytes(stages), s, maps, a, stages, rows);
