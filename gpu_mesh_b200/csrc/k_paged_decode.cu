@@ -4,13 +4,15 @@
 //
 // The cache is read once and every byte feeds at most 32 query rows' worth of
 // FLOPs, so memory is the bound.  What the kernel does about it:
-//   * Work split.  The units are (sequence, KV head, 128-key chunk) of the
-//     lengths as they are on the device; each persistent CTA counts them and
-//     takes a contiguous run of equal length.  A run's end that lies near the
-//     end of a (sequence, head) moves there; one that cuts it leaves (max,
-//     sum, O) in the workspace, and a second kernel joins the pieces in order:
-//     no counters to initialise, so a captured call can be replayed and its
-//     result does not depend on timing.
+//   * Work split.  The units are (sequence, KV head, block of 32 keys, 16 over
+//     bf16 pages) of the lengths as they are on the device.  Every CTA (one per
+//     SM) takes an equal contiguous run of them, whose ends move to the end of
+//     a (sequence, head) where one is near, and deals it to its warps the same
+//     way; each warp streams its part by itself, without a barrier.  Then the
+//     CTA joins what its warps' ends cut, once, in shared memory.  A (sequence,
+//     head) that CTAs' ends cut leaves (max, sum, O) in the workspace, and a
+//     second kernel joins those pieces in order: no counters to initialise, so
+//     a captured call can be replayed and its result does not depend on timing.
 //   * Loads.  Keys and values go from memory straight into the registers that
 //     the MMAs read.  The order of the dims inside a score product is free,
 //     so a thread's K fragments are 16 consecutive bytes of its keys; the
@@ -19,8 +21,7 @@
 //     instruction covers whole 64- or 128-byte rows whatever the page size
 //     (16-token pages cost one table lookup more, not more requests), and
 //     each warp has the next block's loads in flight while it computes.
-//   * Compute.  Eight warps take 32-key (bf16: 16-key) blocks in turn.
-//     Transposed products, so that the query rows sit on the MMA's N = 8
+//   * Compute.  Transposed products, so that the query rows sit on the MMA's N = 8
 //     side: Sᵀ = K·Qᵀ (M = 16 keys), Oᵀ = Vᵀ·Pᵀ (M = 16 dims), fp32
 //     accumulators, online softmax in base 2.
 //       bf16 pages: bf16 MMAs, P split into bf16 high + low parts (2^-17).
@@ -44,30 +45,36 @@ namespace {
 using namespace attn;
 using namespace paged;
 
-constexpr int kWarps = 8;
-constexpr int kThreadsD = kWarps * 32;
-constexpr int kChunkD = 128;     // keys of a unit
-constexpr int kRowsD = 16;       // most query rows of a (sequence, head)
-constexpr int kSnap = 4;         // units a run's end moves to end with a (sequence, head)
-constexpr int kMaxPieces = 160;  // pieces of a cut pair (at most one per CTA)
+constexpr int kWarps = 8;   // of a CTA (one per SM): 255 registers each; 12 or 16 warps spill, and were slower
+constexpr int kRowsD = 16;  // most query rows of a (sequence, head)
 
-// 128-key chunks of a sequence that this kernel takes (0: none, or left to
-// the kernel for many tokens).
-__device__ __forceinline__ int decode_chunks(const SeqSpan& s, int G) {
+// Keys of a block.
+__host__ __device__ constexpr int block_keys(bool e4) { return e4 ? 32 : 16; }
+
+// Blocks of a sequence and KV head that this kernel takes (0: none, or left
+// to the kernel for many tokens).
+__device__ __forceinline__ int decode_blocks(const SeqSpan& s, int G, int bk) {
   if (s.n < 1 || s.n * G > kRowsD) return 0;
   const int len = s.past + s.n;
-  return len > 0 ? (len + kChunkD - 1) / kChunkD : 1;  // no keys at all: one unit that writes zeros
+  return len > 0 ? (len + bk - 1) / bk : 1;  // no keys at all: one block that writes zeros
 }
 
-// Runs of the `total` units over `grid` CTAs: equal ones, but for ends that
-// lie within kSnap units of a (sequence, head)'s end and move there, which
-// saves a cut (an empty run is possible then).
-struct Runs {
-  long long total;
-  int grid;
-  __device__ Runs(long long n, int most) : total(n), grid((int)(n < most ? n : most)) {}
-  __device__ long long raw(int c) const { return (long long)c * total / grid; }
+constexpr int kSnap = 8;   // blocks that a CTA's run's end moves to end with a (sequence, head)
+
+// What a CTA leaves for the join: the (sequence, head) that its run ends and
+// earlier ones began, as its first token row, KV head, query rows (0: there
+// is none) and number of pieces, this run's the last.
+struct Cut {
+  int q0, h, rows, pieces;
 };
+
+// What a warp's piece of a cut (sequence, head) is: rows 0 where there is none.
+struct PieceMeta {
+  int b, h, rows, ends;
+};
+
+// Floats of a run's piece of one (sequence, head): per row O [D], max, sum.
+__host__ __device__ constexpr int piece_floats(int rows, int D) { return rows * (D + 2); }
 
 // 16 (or 8) bytes of the cache, read once: not kept in L1.
 __device__ __forceinline__ uint4 load_once(const void* p) {
@@ -84,33 +91,30 @@ __device__ __forceinline__ uint2 load_once8(const void* p) {
 }
 
 template <int D, bool E4, int NT>
-__global__ void __launch_bounds__(kThreadsD, 1)
-    paged_decode_kernel(const __grid_constant__ PagedAttnArgs a, int merge_rows) {
+__global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __grid_constant__ PagedAttnArgs a, int row_cap) {
   constexpr int KS = D / 16;                     // k-steps of the score MMA
   constexpr int DM = D / 16;                     // dim tiles of Oᵀ
-  constexpr int SUB = E4 ? 2 : 1;                // 16-key tiles of a warp's block
-  constexpr int BK = 16 * SUB;                   // keys of a block
+  constexpr int BK = block_keys(E4), SUB = BK / 16;  // keys of a block, its 16-key tiles
   constexpr int KP = D * (E4 ? 1 : 2) / 64;      // 16-byte pieces of a key that a thread holds (four threads a key)
-  constexpr int VW = D / 8 * (E4 ? 1 : 2) / 4;   // words of a value row that a thread holds (eight threads a key)
-  using Elem = typename std::conditional<E4, uint8_t, __nv_bfloat16>::type;
+  constexpr int VW = D / 8 * (E4 ? 1 : 2) / 4;   // words of a value row that a thread holds (eight threads a row)
+  constexpr int QW = KS / 2;       // 16-byte words of a query row that a thread holds
+  constexpr int ES = E4 ? 1 : 2;
   const PagedPool& pool = a.pool;
   const PagedBatch& bt = a.batch;
   const int G = a.nq / pool.nkv, nkv = pool.nkv;
-  extern __shared__ float smem_f[];
-  float* merge = smem_f;                               // [warp][row][m, l, O(D)]
-  float* fac = merge + kWarps * merge_rows * (D + 2);  // [warp][row]
-  float* msum = fac + kWarps * 8;                      // [row] max, [row] sum
-  int* pre = (int*)(msum + 16);                        // [B + 1] units before a sequence
-  int* slen = pre + bt.B + 1;                          // [B] cached tokens
-  int* sqn = slen + bt.B;                              // [B] first token row · 32 + new tokens
+  extern __shared__ __align__(16) float held[];  // [warp][2][row][O(D), max, sum]: pieces for the CTA's join
+  __shared__ PieceMeta meta[kWarps][2];          // 0: began in an earlier warp's part, 1: goes on in the next one's
+  int* pre = (int*)(held + 2 * kWarps * piece_floats(row_cap, D));  // [B + 1] blocks before a sequence
+  int* slen = pre + bt.B + 1;                                       // [B] cached tokens
+  int* sqn = slen + bt.B;                                           // [B] first token row · 32 + new tokens
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
   pdl_wait();
-  for (int b = tid; b < bt.B; b += kThreadsD) {
+  for (int b = tid; b < bt.B; b += kWarps * 32) {
     const SeqSpan s = seq_span(bt, b, pool.ps);
     if (!s.ok && blockIdx.x == 0) flag_error(a.err, kErrPaged);
-    pre[b + 1] = decode_chunks(s, G);
+    pre[b + 1] = decode_blocks(s, G, BK);
     slen[b] = s.past + s.n;
     sqn[b] = s.q0 * 32 + (s.n & 31);
   }
@@ -118,7 +122,7 @@ __global__ void __launch_bounds__(kThreadsD, 1)
   // written before this kernel.
   pdl_trigger();
   __syncthreads();
-  if (warp == 0) {  // units before each sequence: chunks · KV heads, summed
+  if (warp == 0) {  // blocks before each sequence, over its KV heads, summed
     long long run = 0;
     for (int b0 = 0; b0 < bt.B; b0 += 32) {
       const int b = b0 + lane;
@@ -134,17 +138,14 @@ __global__ void __launch_bounds__(kThreadsD, 1)
     }
     if (lane == 0) {
       pre[0] = 0;
-      if (run >= 0x7fffffffLL) {  // 2^38 cached tokens: no pool holds them
+      if (run >= 0x7fffffffLL) {  // 2^35 cached tokens: no pool holds them
         flag_error(a.err, kErrPaged);
         pre[bt.B] = 0;
       }
     }
   }
   __syncthreads();
-  const Runs runs(pre[bt.B], (int)gridDim.x);
-  const int c = blockIdx.x;
-  if (c >= runs.grid) return;
-  // The sequence that unit u belongs to.
+  const int total = pre[bt.B], c = blockIdx.x, grid = min((int)gridDim.x, total);
   auto seq_of = [&](int u) {
     int lo = 0, hi = bt.B;  // pre[lo] <= u < pre[hi]
     while (hi - lo > 1) {
@@ -153,87 +154,125 @@ __global__ void __launch_bounds__(kThreadsD, 1)
     }
     return lo;
   };
-  auto begin = [&](int k) {
-    const int u = (int)runs.raw(k);
-    if (u >= (int)runs.total) return u;
-    const int b = seq_of(u), C = max(1, (slen[b] + kChunkD - 1) / kChunkD), off = (u - pre[b]) % C;
-    return off <= kSnap ? u - off : C - off <= kSnap ? u + C - off : u;
+  auto begin = [&](int k) {  // of CTA k's run
+    const int u = (int)((long long)k * total / grid);
+    if (u >= total) return total;
+    const int b = seq_of(u), nb = max(1, (slen[b] + BK - 1) / BK), off = (u - pre[b]) % nb;
+    return off <= kSnap ? u - off : nb - off <= kSnap ? u + nb - off : u;
   };
-  const int u0 = begin(c), u1 = begin(c + 1);
-  if (u0 >= u1) return;
+  Cut* cuts = (Cut*)((float*)a.ws + (size_t)2 * gridDim.x * piece_floats(row_cap, D));
+  if (tid == 0) cuts[c] = Cut{0, 0, 0, 0};
+  if (tid < 2 * kWarps) meta[tid >> 1][tid & 1].rows = 0;
+  if (c >= grid) return;
+  const int c0 = begin(c), c1 = begin(c + 1);
+  if (c0 >= c1) return;
+  __syncthreads();  // meta is cleared
+  // The warp's part of the run; where there are fewer blocks than warps the last ones have none.
+  const int parts = min(kWarps, c1 - c0), part_of = min(warp, parts);
+  const int u0 = c0 + (int)((long long)(c1 - c0) * part_of / parts);
+  const int u1 = c0 + (int)((long long)(c1 - c0) * min(part_of + 1, parts) / parts);
 
-  // A piece of the run: the part of one (sequence, KV head) that lies in it.
-  struct Piece {
-    int b, h, pu, C, ue, kb, ke;  // first unit of the pair, its units, the piece's end; its blocks
-  };
-  auto piece_at = [&](int u) {
-    Piece p;
-    p.b = seq_of(u);
-    const int len = slen[p.b];
-    p.C = max(1, (len + kChunkD - 1) / kChunkD);
-    p.h = (u - pre[p.b]) / p.C;
-    p.pu = pre[p.b] + p.h * p.C;
-    p.ue = min(u1, p.pu + p.C);
-    p.kb = (u - p.pu) * (kChunkD / BK);
-    p.ke = min((p.ue - p.pu) * (kChunkD / BK), (len + BK - 1) / BK);
-    return p;
-  };
-
-  // The blocks of this warp, in order, over all pieces: `ahead` runs two
-  // blocks ahead of the computation for the page lookups, one for the data.
-  // Blocks are dealt to the warps in turn across pieces.
+  // The part's blocks, in order.  Data is requested one block ahead of the
+  // computation, pages are looked up two ahead.
   struct Block {
-    int b, h, k0, len;  // len 0: none left
-    int page[SUB];
+    int b, h, k0, len;  // keys k0 .. of the sequence's len
+    int page[SUB];      // -1: no key there, or outside the pool (its keys read as zeros)
+    bool valid, first, last;  // first / last block of its piece of the part
+    bool full;          // every key of the block is there
   };
-  Piece ap = piece_at(u0);
-  int abase = 0, ablk = ap.kb + warp;
+  const int page_shift = 31 - __clz(pool.ps);
+  int cu = u0, cb, ch, cblk, cnb, clen;
+  const int32_t* ctab;
+  {
+    cb = seq_of(min(cu, total - 1));
+    clen = slen[cb];
+    cnb = max(1, (clen + BK - 1) / BK);
+    ch = (cu - pre[cb]) / cnb;
+    cblk = (cu - pre[cb]) - ch * cnb;
+    ctab = bt.table + (int64_t)cb * bt.ld;
+  }
+  bool fresh = true;
   auto next_block = [&]() {
     Block x;
-    x.len = 0;
-    x.b = x.h = x.k0 = 0;
-    while (ablk >= ap.ke) {
-      abase = (abase + max(0, ap.ke - ap.kb)) & (kWarps - 1);
-      if (ap.ue >= u1) break;
-      ap = piece_at(ap.ue);
-      ablk = ap.kb + ((warp - abase) & (kWarps - 1));
-    }
+    x.valid = cu < u1;
+    x.b = cb;
+    x.h = ch;
+    x.k0 = cblk * BK;
+    x.len = x.valid ? clen : 0;
+    x.first = fresh || cblk == 0;
+    x.last = cblk + 1 == cnb || cu + 1 == u1;
+    fresh = false;
 #pragma unroll
-    for (int i = 0; i < SUB; ++i) x.page[i] = -1;
-    if (ablk < ap.ke) {
-      x.b = ap.b;
-      x.h = ap.h;
-      x.k0 = ablk * BK;
-      x.len = slen[ap.b];
-#pragma unroll
-      for (int i = 0; i < SUB; ++i)
-        if (x.k0 + 16 * i < x.len) x.page[i] = __ldg(bt.table + (int64_t)x.b * bt.ld + (x.k0 + 16 * i) / pool.ps);
-      ablk += kWarps;
+    for (int i = 0; i < SUB; ++i)
+      x.page[i] = x.k0 + 16 * i < x.len ? __ldg(ctab + ((x.k0 + 16 * i) >> page_shift)) : -1;
+    ++cu;
+    if (++cblk == cnb && cu < u1) {
+      cblk = 0;
+      if (++ch == nkv) {
+        ch = 0;
+        do ++cb; while (pre[cb + 1] == pre[cb]);
+        clen = slen[cb];
+        cnb = max(1, (clen + BK - 1) / BK);
+        ctab = bt.table + (int64_t)cb * bt.ld;
+      }
     }
     return x;
+  };
+  // The page numbers, a block later: they have arrived by then.
+  auto check = [&](Block& x) {
+    x.full = x.k0 + BK <= x.len;
+#pragma unroll
+    for (int i = 0; i < SUB; ++i)
+      if ((unsigned)x.page[i] >= (unsigned)pool.pages) {
+        if (x.k0 + 16 * i < x.len) flag_error(a.err, kErrPaged);
+        x.page[i] = -1;
+        x.full = false;
+      }
   };
   uint4 kx[SUB][2][KP];       // keys g, g + 8 of each tile
   uint32_t vx[SUB][4][VW];    // values 2t, 2t + 1, 2t + 8, 2t + 9
   float ks[SUB], vs[SUB];
-  // A block's keys (and both scales) and values: each half is requested as soon
-  // as the registers of the block before are free.
+  uint4 qx[NT][QW];           // query row g of each 8-row tile
+  // A block's keys (both scales, and the query rows of a new piece) and values:
+  // each half is requested as soon as the registers of the block before are
+  // free.  Offsets of a thread's rows inside a tile, in bytes; the tile lies in one page.
+  const int64_t koff = (int64_t)g * pool.kt * ES + 16 * t, k8 = 8 * pool.kt * ES;
+  const int64_t voff = (int64_t)2 * t * pool.vt * ES + g * (VW * 4), v1 = pool.vt * ES, v8 = 8 * v1;
   auto load_k = [&](const Block& x) {
 #pragma unroll
     for (int i = 0; i < SUB; ++i) {
       const int k0 = x.k0 + 16 * i, page = x.page[i];
-      const bool some = k0 < x.len, good = page >= 0 && page < pool.pages;
-      if (some && !good) flag_error(a.err, kErrPaged);  // its keys read as zeros
-      const Elem* kp = (const Elem*)pool.k + (int64_t)page * pool.kp + x.h * pool.kh + (k0 % pool.ps) * pool.kt;
+      const uint8_t* kp = (const uint8_t*)pool.k + (page * pool.kp + x.h * pool.kh + (k0 & (pool.ps - 1)) * pool.kt) * ES + koff;
+      if (x.full) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const bool ok = good && k0 + g + 8 * r < x.len;
+        for (int r = 0; r < 2; ++r)
 #pragma unroll
-        for (int p = 0; p < KP; ++p)
-          kx[i][r][p] = ok ? load_once((const uint8_t*)(kp + (g + 8 * r) * pool.kt) + 64 * p + 16 * t) : make_uint4(0u, 0u, 0u, 0u);
+          for (int p = 0; p < KP; ++p) kx[i][r][p] = load_once(kp + r * k8 + 64 * p);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int p = 0; p < KP; ++p)
+            kx[i][r][p] = page >= 0 && k0 + g + 8 * r < x.len ? load_once(kp + r * k8 + 64 * p) : make_uint4(0u, 0u, 0u, 0u);
       }
       if constexpr (E4) {
-        ks[i] = some && good ? __ldg(pool.ks + (int64_t)page * pool.kse + x.h) : 0.f;
-        vs[i] = some && good ? __ldg(pool.vs + (int64_t)page * pool.vse + x.h) : 1.f;
+        ks[i] = page >= 0 ? __ldg(pool.ks + page * pool.kse + x.h) : 0.f;
+        vs[i] = page >= 0 ? __ldg(pool.vs + page * pool.vse + x.h) : 1.f;
+      }
+    }
+    if (x.valid && x.first) {
+      const int rows = (sqn[x.b] & 31) * G;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int r = nt * 8 + g;
+        const __nv_bfloat16* q = (const __nv_bfloat16*)a.q + (int64_t)((sqn[x.b] >> 5) + r / G) * a.ldq +
+                                 (int64_t)(x.h * G + r % G) * a.hdq;
+        // The dims in the order of the K fragments: a thread's 16 bytes of a
+        // key are 16 (bf16: 8) consecutive dims, k-steps of four dims each.
+#pragma unroll
+        for (int i = 0; i < QW; ++i)
+          qx[nt][i] = r < rows ? *reinterpret_cast<const uint4*>(E4 ? q + 64 * (i / 2) + 16 * t + 8 * (i % 2) : q + 32 * i + 8 * t)
+                               : make_uint4(0u, 0u, 0u, 0u);
       }
     }
   };
@@ -241,375 +280,385 @@ __global__ void __launch_bounds__(kThreadsD, 1)
 #pragma unroll
     for (int i = 0; i < SUB; ++i) {
       const int k0 = x.k0 + 16 * i, page = x.page[i];
-      const bool good = page >= 0 && page < pool.pages;
-      const Elem* vp = (const Elem*)pool.v + (int64_t)page * pool.vp + x.h * pool.vh + (k0 % pool.ps) * pool.vt;
+      const uint8_t* vp = (const uint8_t*)pool.v + (page * pool.vp + x.h * pool.vh + (k0 & (pool.ps - 1)) * pool.vt) * ES + voff;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int key = 2 * t + (r & 1) + 8 * (r >> 1);
-        const bool ok = good && k0 + key < x.len;
-        const uint8_t* at = (const uint8_t*)(vp + key * pool.vt) + g * (VW * 4);
+        const bool ok = page >= 0 && k0 + 2 * t + (r & 1) + 8 * (r >> 1) < x.len;
+        const uint8_t* at = vp + (r & 1) * v1 + (r >> 1) * v8;
         if constexpr (VW == 2) {
-          const uint2 v = ok ? load_once8(at) : make_uint2(0u, 0u);
+          uint2 v = make_uint2(0u, 0u);
+          if (x.full) v = load_once8(at);
+          else if (ok) v = load_once8(at);
           vx[i][r][0] = v.x;
           vx[i][r][1] = v.y;
         } else {
 #pragma unroll
-          for (int w = 0; w < VW / 4; ++w) {
-            const uint4 v = ok ? load_once(at + 16 * w) : make_uint4(0u, 0u, 0u, 0u);
-            vx[i][r][4 * w] = v.x;
-            vx[i][r][4 * w + 1] = v.y;
-            vx[i][r][4 * w + 2] = v.z;
-            vx[i][r][4 * w + 3] = v.w;
+          for (int p = 0; p < VW / 4; ++p) {
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (x.full) v = load_once(at + 16 * p);
+            else if (ok) v = load_once(at + 16 * p);
+            vx[i][r][4 * p] = v.x;
+            vx[i][r][4 * p + 1] = v.y;
+            vx[i][r][4 * p + 2] = v.z;
+            vx[i][r][4 * p + 3] = v.w;
           }
         }
       }
     }
   };
-  Block now = next_block(), next = next_block();
+  Block now = next_block();
+  check(now);
   load_k(now);
   load_v(now);
+  Block next = next_block();
 
   const float scale2 = a.scale * 1.4426950408889634f;
-  int base = 0;
-  for (int u = u0; u < u1;) {
-    const Piece p = piece_at(u);
-    const int len = slen[p.b], nq_tok = sqn[p.b] & 31, rows = nq_tok * G, past = len - nq_tok;
-    const bool whole = p.pu >= u0 && p.pu + p.C <= u1;
-    // Thread (g, t) holds keys g, g + 8 (dims of Oᵀ by tile) for the query
-    // rows 2t, 2t + 1 of each 8-row tile; vis: keys those rows see.
-    int vis[NT][2];
-    float mrow[NT][2], lrow[NT][2], rowf[NT][2];
-    float o[NT][DM][4];
-    uint32_t qb[NT][KS][2];
+  // Thread (g, t) holds keys g, g + 8 (dims of Oᵀ by tile) for the query
+  // rows 2t, 2t + 1 of each 8-row tile; vis: keys those rows see.
+  int rows = 0, least = 0, from = 0, vis[NT][2];
+  float mrow[NT][2], lrow[NT][2], rowf[NT][2];
+  float o[NT][DM][4];
+  uint32_t qb[NT][KS][2];
+  while (now.valid) {
+    if (now.first) {
+      const int n = sqn[now.b] & 31, past = now.len - n;
+      rows = n * G;
+      least = past + 1;  // keys that every row sees
+      from = now.k0;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+      for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r = nt * 8 + 2 * t + e;
-        vis[nt][e] = r < rows ? past + r / G + 1 : 0;
-        mrow[nt][e] = -INFINITY;
-        lrow[nt][e] = 0.f;
-        rowf[nt][e] = scale2;
-      }
+        for (int e = 0; e < 2; ++e) {
+          const int r = nt * 8 + 2 * t + e;
+          vis[nt][e] = r < rows ? past + r / G + 1 : 0;
+          mrow[nt][e] = -INFINITY;
+          lrow[nt][e] = 0.f;
+          rowf[nt][e] = scale2;
+        }
 #pragma unroll
-      for (int i = 0; i < DM; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
-      // Row g's dims in the order of the K fragments: thread t of a key's
-      // four holds 16 consecutive bytes, k-steps of four dims each.
-      const int r = nt * 8 + g;
-      const __nv_bfloat16* q = (const __nv_bfloat16*)a.q + (int64_t)((sqn[p.b] >> 5) + r / G) * a.ldq +
-                               (int64_t)(p.h * G + r % G) * a.hdq;
-      if constexpr (E4) {
-        uint4 raw[KS / 4][2];
-        float amax = 0.f;
+        for (int i = 0; i < DM; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+        if constexpr (E4) {
+          float amax = 0.f;
 #pragma unroll
-        for (int i = 0; i < KS / 4; ++i)
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            raw[i][w] = r < rows ? *reinterpret_cast<const uint4*>(q + 64 * i + 16 * t + 8 * w) : make_uint4(0u, 0u, 0u, 0u);
-            const uint32_t x[4] = {raw[i][w].x, raw[i][w].y, raw[i][w].z, raw[i][w].w};
+          for (int i = 0; i < QW; ++i) {
+            const uint32_t x[4] = {qx[nt][i].x, qx[nt][i].y, qx[nt][i].z, qx[nt][i].w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) amax = fmaxf(amax, fmaxf(fabsf(lo_bf16(x[k])), fabsf(hi_bf16(x[k]))));
           }
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        const int sh = row_shift(amax);
-        const float f = pow2i(sh);
+          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+          const int sh = row_shift(amax);
+          const float f = pow2i(sh);
 #pragma unroll
-        for (int i = 0; i < KS / 4; ++i)
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            const uint4 x = raw[i][w];
-            qb[nt][4 * i + 2 * w][0] = pack_f16(lo_bf16(x.x) * f, hi_bf16(x.x) * f);
-            qb[nt][4 * i + 2 * w][1] = pack_f16(lo_bf16(x.y) * f, hi_bf16(x.y) * f);
-            qb[nt][4 * i + 2 * w + 1][0] = pack_f16(lo_bf16(x.z) * f, hi_bf16(x.z) * f);
-            qb[nt][4 * i + 2 * w + 1][1] = pack_f16(lo_bf16(x.w) * f, hi_bf16(x.w) * f);
+          for (int i = 0; i < QW; ++i) {
+            const uint4 x = qx[nt][i];
+            qb[nt][2 * i][0] = pack_f16(lo_bf16(x.x) * f, hi_bf16(x.x) * f);
+            qb[nt][2 * i][1] = pack_f16(lo_bf16(x.y) * f, hi_bf16(x.y) * f);
+            qb[nt][2 * i + 1][0] = pack_f16(lo_bf16(x.z) * f, hi_bf16(x.z) * f);
+            qb[nt][2 * i + 1][1] = pack_f16(lo_bf16(x.w) * f, hi_bf16(x.w) * f);
           }
-        // Row g's factor is needed by the threads that hold rows 2t, 2t + 1.
+          // Row g's factor is needed by the threads that hold rows 2t, 2t + 1.
 #pragma unroll
-        for (int e = 0; e < 2; ++e) rowf[nt][e] = scale2 * pow2i(-__shfl_sync(0xffffffffu, sh, (2 * t + e) * 4));
-      } else {
+          for (int e = 0; e < 2; ++e) rowf[nt][e] = scale2 * pow2i(-__shfl_sync(0xffffffffu, sh, (2 * t + e) * 4));
+        } else {
 #pragma unroll
-        for (int i = 0; i < KS / 2; ++i) {
-          const uint4 x = r < rows ? *reinterpret_cast<const uint4*>(q + 32 * i + 8 * t) : make_uint4(0u, 0u, 0u, 0u);
-          qb[nt][2 * i][0] = x.x;
-          qb[nt][2 * i][1] = x.y;
-          qb[nt][2 * i + 1][0] = x.z;
-          qb[nt][2 * i + 1][1] = x.w;
+          for (int i = 0; i < QW; ++i) {
+            qb[nt][2 * i][0] = qx[nt][i].x;
+            qb[nt][2 * i][1] = qx[nt][i].y;
+            qb[nt][2 * i + 1][0] = qx[nt][i].z;
+            qb[nt][2 * i + 1][1] = qx[nt][i].w;
+          }
         }
       }
     }
-    const int least = past + 1;  // keys that every row sees
-    for (int blk = p.kb + ((warp - base) & (kWarps - 1)); blk < p.ke; blk += kWarps) {
-      const int j0 = blk * BK;
-      float sc[NT][SUB][4];
+    const int j0 = now.k0;
+    float sc[NT][SUB][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < SUB; ++i) sc[nt][i][0] = sc[nt][i][1] = sc[nt][i][2] = sc[nt][i][3] = 0.f;
+      for (int i = 0; i < SUB; ++i) sc[nt][i][0] = sc[nt][i][1] = sc[nt][i][2] = sc[nt][i][3] = 0.f;
 #pragma unroll
-      for (int q = 0; q < KP; ++q) {
-#pragma unroll
-        for (int i = 0; i < SUB; ++i) {
-          const uint32_t x[4] = {kx[i][0][q].x, kx[i][0][q].y, kx[i][0][q].z, kx[i][0][q].w};
-          const uint32_t y[4] = {kx[i][1][q].x, kx[i][1][q].y, kx[i][1][q].z, kx[i][1][q].w};
-          if constexpr (E4) {
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              const uint32_t a0 = e4m3x2_to_f16x2(x[w]), a1 = e4m3x2_to_f16x2(y[w]);
-              const uint32_t a2 = e4m3x2_hi_to_f16x2(x[w]), a3 = e4m3x2_hi_to_f16x2(y[w]);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma16816_f16(sc[nt][i], a0, a1, a2, a3, qb[nt][4 * q + w][0], qb[nt][4 * q + w][1]);
-            }
-          } else {
-#pragma unroll
-            for (int w = 0; w < 2; ++w)
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-                mma16816_full(sc[nt][i], x[2 * w], y[2 * w], x[2 * w + 1], y[2 * w + 1], qb[nt][2 * q + w][0], qb[nt][2 * q + w][1]);
-          }
-        }
-      }
-      float ksc[SUB];
-      int ve[SUB];
+    for (int q = 0; q < KP; ++q) {
 #pragma unroll
       for (int i = 0; i < SUB; ++i) {
-        ksc[i] = E4 ? ks[i] : 1.f;
-        ve[i] = E4 ? scale_exp(vs[i]) : 0;
-      }
-      load_k(next);
-      // Online softmax per query row (column): keys g (c0, c1), g + 8 (c2, c3) of each tile.
-      uint32_t ph[NT][SUB][2], plo[NT][SUB][2];
-      const bool clear = j0 + BK <= least;  // every key of the block is visible to every row
+        const uint32_t x[4] = {kx[i][0][q].x, kx[i][0][q].y, kx[i][0][q].z, kx[i][0][q].w};
+        const uint32_t y[4] = {kx[i][1][q].x, kx[i][1][q].y, kx[i][1][q].z, kx[i][1][q].w};
+        if constexpr (E4) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float mx[2] = {mrow[nt][0], mrow[nt][1]};
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t a0 = e4m3x2_to_f16x2(x[w]), a1 = e4m3x2_to_f16x2(y[w]);
+            const uint32_t a2 = e4m3x2_hi_to_f16x2(x[w]), a3 = e4m3x2_hi_to_f16x2(y[w]);
 #pragma unroll
-        for (int i = 0; i < SUB; ++i) {
-          float* s = sc[nt][i];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float f = rowf[nt][e] * ksc[i];
-            s[e] = E4 ? fmaf(s[e], f, (float)ve[i]) : s[e] * f;
-            s[2 + e] = E4 ? fmaf(s[2 + e], f, (float)ve[i]) : s[2 + e] * f;
-            if (!clear) {
-              s[e] = j0 + 16 * i + g < vis[nt][e] ? s[e] : -INFINITY;
-              s[2 + e] = j0 + 16 * i + g + 8 < vis[nt][e] ? s[2 + e] : -INFINITY;
-            }
-            mx[e] = fmaxf(mx[e], fmaxf(s[e], s[2 + e]));
+            for (int nt = 0; nt < NT; ++nt) mma16816_f16(sc[nt][i], a0, a1, a2, a3, qb[nt][4 * q + w][0], qb[nt][4 * q + w][1]);
           }
-        }
+        } else {
 #pragma unroll
-        for (int off = 4; off < 32; off <<= 1) {
-          mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], off));
-          mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], off));
-        }
-        if (__any_sync(0xffffffffu, mx[0] != mrow[nt][0] || mx[1] != mrow[nt][1])) {
-          float keep[2];
+          for (int w = 0; w < 2; ++w)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            keep[e] = mrow[nt][e] == -INFINITY ? 0.f : ex2(mrow[nt][e] - mx[e]);
-            mrow[nt][e] = mx[e];
-            lrow[nt][e] *= keep[e];
-          }
-#pragma unroll
-          for (int i = 0; i < DM; ++i) {
-            o[nt][i][0] *= keep[0];
-            o[nt][i][1] *= keep[1];
-            o[nt][i][2] *= keep[0];
-            o[nt][i][3] *= keep[1];
-          }
-        }
-        // A row that has seen no key yet keeps m = -inf: every weight is 0.
-        const float base0 = mx[0] == -INFINITY ? 0.f : mx[0] - (E4 ? 14.f : 0.f);
-        const float base1 = mx[1] == -INFINITY ? 0.f : mx[1] - (E4 ? 14.f : 0.f);
-#pragma unroll
-        for (int i = 0; i < SUB; ++i) {
-          float* s = sc[nt][i];
-          s[0] = ex2(s[0] - base0);
-          s[1] = ex2(s[1] - base1);
-          s[2] = ex2(s[2] - base0);
-          s[3] = ex2(s[3] - base1);
-          if constexpr (E4) {
-            const float w = pow2i(-ve[i] - 14);
-            lrow[nt][0] = fmaf(s[0] + s[2], w, lrow[nt][0]);
-            lrow[nt][1] = fmaf(s[1] + s[3], w, lrow[nt][1]);
-            // Pᵀ as the B operand of Oᵀ += Vᵀ·Pᵀ: an 8x8 (keys x rows) matrix each, transposed in registers.
-            ph[nt][i][0] = movm_trans(pack_f16(s[0], s[1]));
-            ph[nt][i][1] = movm_trans(pack_f16(s[2], s[3]));
-          } else {
-            lrow[nt][0] += s[0] + s[2];
-            lrow[nt][1] += s[1] + s[3];
-            const uint32_t h01 = pack2(s[0], s[1]), h23 = pack2(s[2], s[3]);
-            ph[nt][i][0] = movm_trans(h01);
-            ph[nt][i][1] = movm_trans(h23);
-            plo[nt][i][0] = movm_trans(pack2(s[0] - lo_bf16(h01), s[1] - hi_bf16(h01)));
-            plo[nt][i][1] = movm_trans(pack2(s[2] - lo_bf16(h23), s[3] - hi_bf16(h23)));
-          }
+            for (int nt = 0; nt < NT; ++nt)
+              mma16816_full(sc[nt][i], x[2 * w], y[2 * w], x[2 * w + 1], y[2 * w + 1], qb[nt][2 * q + w][0], qb[nt][2 * q + w][1]);
         }
       }
-      // Tile j of Oᵀ: rows g and g + 8 are the thread's dims 2j and 2j + 1.
-#pragma unroll
-      for (int j = 0; j < DM; ++j) {
-#pragma unroll
-        for (int i = 0; i < SUB; ++i) {
-          if constexpr (E4) {
-            const int sel = j & 1 ? 0x7362 : 0x5140;
-            const uint32_t y0 = __byte_perm(vx[i][0][j / 2], vx[i][1][j / 2], sel);
-            const uint32_t y1 = __byte_perm(vx[i][2][j / 2], vx[i][3][j / 2], sel);
-            const uint32_t a0 = e4m3x2_to_f16x2(y0), a1 = e4m3x2_hi_to_f16x2(y0);
-            const uint32_t a2 = e4m3x2_to_f16x2(y1), a3 = e4m3x2_hi_to_f16x2(y1);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma16816_f16(o[nt][j], a0, a1, a2, a3, ph[nt][i][0], ph[nt][i][1]);
-          } else {
-            const uint32_t a0 = __byte_perm(vx[i][0][j], vx[i][1][j], 0x5410), a1 = __byte_perm(vx[i][0][j], vx[i][1][j], 0x7632);
-            const uint32_t a2 = __byte_perm(vx[i][2][j], vx[i][3][j], 0x5410), a3 = __byte_perm(vx[i][2][j], vx[i][3][j], 0x7632);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              mma16816_full(o[nt][j], a0, a1, a2, a3, ph[nt][i][0], ph[nt][i][1]);
-              mma16816_full(o[nt][j], a0, a1, a2, a3, plo[nt][i][0], plo[nt][i][1]);
-            }
-          }
-        }
-      }
-      load_v(next);
-      next = next_block();
     }
-    base = (base + max(0, p.ke - p.kb)) & (kWarps - 1);
-
-    // End of the piece: join the warps, eight query rows at a time.
+    float ksc[SUB];
+    int ve[SUB];
+#pragma unroll
+    for (int i = 0; i < SUB; ++i) {
+      ksc[i] = E4 ? ks[i] : 1.f;
+      ve[i] = E4 ? scale_exp(vs[i]) : 0;
+    }
+    check(next);
+    load_k(next);
+    // Online softmax per query row (column): keys g (c0, c1), g + 8 (c2, c3) of each tile.
+    uint32_t ph[NT][SUB][2], plo[NT][SUB][2];
+    const bool clear = j0 + BK <= least;  // every key of the block is visible to every row
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int nr = min(8, rows - nt * 8);
-      if (nt > 0 && nr <= 0) break;
-      float* mw = merge + warp * merge_rows * (D + 2);
+      float mx[2] = {mrow[nt][0], mrow[nt][1]};
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float l = lrow[nt][e];
+      for (int i = 0; i < SUB; ++i) {
+        float* s = sc[nt][i];
 #pragma unroll
-        for (int off = 4; off < 32; off <<= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
-        const int hh = 2 * t + e;
-        if (hh < nr) {
-          if (g == 0) {
-            mw[hh * (D + 2)] = mrow[nt][e];
-            mw[hh * (D + 2) + 1] = l;
+        for (int e = 0; e < 2; ++e) {
+          const float f = rowf[nt][e] * ksc[i];
+          s[e] = E4 ? fmaf(s[e], f, (float)ve[i]) : s[e] * f;
+          s[2 + e] = E4 ? fmaf(s[2 + e], f, (float)ve[i]) : s[2 + e] * f;
+          if (!clear) {
+            s[e] = j0 + 16 * i + g < vis[nt][e] ? s[e] : -INFINITY;
+            s[2 + e] = j0 + 16 * i + g + 8 < vis[nt][e] ? s[2 + e] : -INFINITY;
           }
-#pragma unroll
-          for (int j = 0; j < DM; ++j)
-            *reinterpret_cast<float2*>(&mw[hh * (D + 2) + 2 + g * (D / 8) + 2 * j]) = make_float2(o[nt][j][e], o[nt][j][2 + e]);
+          mx[e] = fmaxf(mx[e], fmaxf(s[e], s[2 + e]));
         }
       }
-      __syncthreads();
-      if (tid < nr) {
-        float M = -INFINITY, S = 0.f;
-        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, merge[(w * merge_rows + tid) * (D + 2)]);
-        for (int w = 0; w < kWarps; ++w) {
-          const float mv = merge[(w * merge_rows + tid) * (D + 2)];
-          const float f = mv == -INFINITY ? 0.f : ex2(mv - M);
-          fac[w * 8 + tid] = f;
-          S += f * merge[(w * merge_rows + tid) * (D + 2) + 1];
-        }
-        msum[tid] = M;
-        msum[8 + tid] = S;
-      }
-      __syncthreads();
-      float* part = (float*)a.ws + (size_t)(2 * c + (p.pu < u0 ? 0 : 1)) * kRowsD * (D + 2);
-      for (int i = tid; i < nr * D; i += kThreadsD) {
-        const int hh = i / D, d = i % D, r = nt * 8 + hh;
-        float acc = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) acc += fac[w * 8 + hh] * merge[(w * merge_rows + hh) * (D + 2) + 2 + d];
-        if constexpr (E4) acc *= 1.f / 16384.f;
-        if (whole) {
-          const float S = msum[8 + hh];
-          ((__nv_bfloat16*)a.out)[(int64_t)((sqn[p.b] >> 5) + r / G) * a.ldo + (int64_t)(p.h * G + r % G) * a.hdo + d] =
-              __float2bfloat16_rn(S == 0.f ? 0.f : acc / S);
+      for (int off = 4; off < 32; off <<= 1) {
+        mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], off));
+        mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], off));
+      }
+      if (__any_sync(0xffffffffu, mx[0] != mrow[nt][0] || mx[1] != mrow[nt][1])) {
+        float keep[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          keep[e] = mrow[nt][e] == -INFINITY ? 0.f : ex2(mrow[nt][e] - mx[e]);
+          mrow[nt][e] = mx[e];
+          lrow[nt][e] *= keep[e];
+        }
+#pragma unroll
+        for (int i = 0; i < DM; ++i) {
+          o[nt][i][0] *= keep[0];
+          o[nt][i][1] *= keep[1];
+          o[nt][i][2] *= keep[0];
+          o[nt][i][3] *= keep[1];
+        }
+      }
+      // A row that has seen no key yet keeps m = -inf: every weight is 0.
+      const float base0 = mx[0] == -INFINITY ? 0.f : mx[0] - (E4 ? 14.f : 0.f);
+      const float base1 = mx[1] == -INFINITY ? 0.f : mx[1] - (E4 ? 14.f : 0.f);
+#pragma unroll
+      for (int i = 0; i < SUB; ++i) {
+        float* s = sc[nt][i];
+        s[0] = ex2(s[0] - base0);
+        s[1] = ex2(s[1] - base1);
+        s[2] = ex2(s[2] - base0);
+        s[3] = ex2(s[3] - base1);
+        if constexpr (E4) {
+          const float w = pow2i(-ve[i] - 14);
+          lrow[nt][0] = fmaf(s[0] + s[2], w, lrow[nt][0]);
+          lrow[nt][1] = fmaf(s[1] + s[3], w, lrow[nt][1]);
+          // Pᵀ as the B operand of Oᵀ += Vᵀ·Pᵀ: an 8x8 (keys x rows) matrix each, transposed in registers.
+          ph[nt][i][0] = movm_trans(pack_f16(s[0], s[1]));
+          ph[nt][i][1] = movm_trans(pack_f16(s[2], s[3]));
         } else {
-          part[r * (D + 2) + 2 + d] = acc;
-          if (d == 0) {
-            part[r * (D + 2)] = msum[hh];
-            part[r * (D + 2) + 1] = msum[8 + hh];
+          lrow[nt][0] += s[0] + s[2];
+          lrow[nt][1] += s[1] + s[3];
+          const uint32_t h01 = pack2(s[0], s[1]), h23 = pack2(s[2], s[3]);
+          ph[nt][i][0] = movm_trans(h01);
+          ph[nt][i][1] = movm_trans(h23);
+          plo[nt][i][0] = movm_trans(pack2(s[0] - lo_bf16(h01), s[1] - hi_bf16(h01)));
+          plo[nt][i][1] = movm_trans(pack2(s[2] - lo_bf16(h23), s[3] - hi_bf16(h23)));
+        }
+      }
+    }
+    // Tile j of Oᵀ: rows g and g + 8 are the thread's dims 2j and 2j + 1.
+#pragma unroll
+    for (int j = 0; j < DM; ++j) {
+#pragma unroll
+      for (int i = 0; i < SUB; ++i) {
+        if constexpr (E4) {
+          const int sel = j & 1 ? 0x7362 : 0x5140;
+          const uint32_t y0 = __byte_perm(vx[i][0][j / 2], vx[i][1][j / 2], sel);
+          const uint32_t y1 = __byte_perm(vx[i][2][j / 2], vx[i][3][j / 2], sel);
+          const uint32_t a0 = e4m3x2_to_f16x2(y0), a1 = e4m3x2_hi_to_f16x2(y0);
+          const uint32_t a2 = e4m3x2_to_f16x2(y1), a3 = e4m3x2_hi_to_f16x2(y1);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma16816_f16(o[nt][j], a0, a1, a2, a3, ph[nt][i][0], ph[nt][i][1]);
+        } else {
+          const uint32_t a0 = __byte_perm(vx[i][0][j], vx[i][1][j], 0x5410), a1 = __byte_perm(vx[i][0][j], vx[i][1][j], 0x7632);
+          const uint32_t a2 = __byte_perm(vx[i][2][j], vx[i][3][j], 0x5410), a3 = __byte_perm(vx[i][2][j], vx[i][3][j], 0x7632);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma16816_full(o[nt][j], a0, a1, a2, a3, ph[nt][i][0], ph[nt][i][1]);
+            mma16816_full(o[nt][j], a0, a1, a2, a3, plo[nt][i][0], plo[nt][i][1]);
           }
         }
       }
-      __syncthreads();  // the join area is rewritten
     }
-    u = p.ue;
+    load_v(next);
+    if (now.last) {  // end of the piece: out, or kept for the CTA's join
+      const bool ends = now.k0 + BK >= now.len, whole = from == 0 && ends;
+      const int slot = from > 0 ? 0 : 1;
+      if (!whole && lane == 0) meta[warp][slot] = PieceMeta{now.b, now.h, rows, ends};
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float l = lrow[nt][e];
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+          const int r = nt * 8 + 2 * t + e;
+          if (r >= rows) continue;
+          // The thread's D / 8 dims of the row.
+          float x[D / 8];
+#pragma unroll
+          for (int j = 0; j < DM; ++j) x[2 * j] = o[nt][j][e], x[2 * j + 1] = o[nt][j][2 + e];
+          const float unit = E4 ? 1.f / 16384.f : 1.f;
+          if (whole) {
+            const float f = l == 0.f ? 0.f : unit / l;
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) x[i] *= f;
+            __nv_bfloat16* out = (__nv_bfloat16*)a.out + (int64_t)((sqn[now.b] >> 5) + r / G) * a.ldo +
+                                 (int64_t)(now.h * G + r % G) * a.hdo + g * (D / 8);
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) store16_f<__nv_bfloat16>(out + 8 * i, x + 8 * i);
+          } else {
+            float* part = held + (size_t)(2 * warp + slot) * piece_floats(row_cap, D) + r * (D + 2);
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i)
+              *reinterpret_cast<float2*>(part + g * (D / 8) + 2 * i) = make_float2(x[2 * i] * unit, x[2 * i + 1] * unit);
+            if (g == 0) *reinterpret_cast<float2*>(part + D) = make_float2(mrow[nt][e], l);
+          }
+        }
+      }
+    }
+    now = next;
+    next = next_block();
+  }
+  __syncthreads();
+  // Chains of pieces of one (sequence, head): a slot 1, or warp 0's slot 0,
+  // and the slots 0 of the warps behind it up to the one that ends it.
+  for (int i = -1; i < kWarps; ++i) {
+    const bool begun = i < 0;  // in an earlier CTA's run
+    const PieceMeta head = begun ? meta[0][0] : meta[i][1];
+    if (head.rows == 0) continue;
+    int last = max(i, 0);
+    bool ends = begun && head.ends;
+    while (!ends && last + 1 < kWarps && meta[last + 1][0].rows > 0) ends = meta[++last][0].ends;
+    const int q0 = sqn[head.b] >> 5, np = last - i + (begun ? 0 : 1);  // pieces of the chain
+    const int lowest = begun ? 0 : i;
+    float* part = (float*)a.ws + (size_t)(2 * c + (begun ? 0 : 1)) * piece_floats(row_cap, D);
+    for (int k = tid; k < head.rows * D; k += kWarps * 32) {
+      const int r = k / D, d = k % D;
+      const float* x = held + r * (D + 2);
+      // piece j of the chain: slot 1 of its first warp unless the pair began earlier, then slots 0
+      auto at = [&](int j) { return x + (size_t)(2 * (lowest + j) + (j == 0 && !begun ? 1 : 0)) * piece_floats(row_cap, D); };
+      float M = -INFINITY, S = 0.f, acc = 0.f;
+      for (int j = 0; j < np; ++j) M = fmaxf(M, at(j)[D]);
+      for (int j = 0; j < np; ++j) {
+        const float m = at(j)[D], f = m == -INFINITY ? 0.f : ex2(m - M);
+        S += f * at(j)[D + 1];
+        acc += f * at(j)[d];
+      }
+      if (!begun && ends) {
+        ((__nv_bfloat16*)a.out)[(int64_t)(q0 + r / G) * a.ldo + (int64_t)(head.h * G + r % G) * a.hdo + d] =
+            __float2bfloat16_rn(S == 0.f ? 0.f : acc / S);
+      } else {
+        part[r * (D + 2) + d] = acc;
+        if (d == 0) *reinterpret_cast<float2*>(part + r * (D + 2) + D) = make_float2(M, S);
+      }
+    }
+    if (begun && ends && tid == 0) {  // the pair's last piece: find its first
+      const int p0 = pre[head.b] + head.h * ((slen[head.b] + BK - 1) / BK);
+      int k = min(c, (int)(((long long)p0 + 1) * grid / total));
+      while (k > 0 && begin(k) > p0) --k;
+      while (k + 1 < c && begin(k + 1) <= p0) ++k;
+      cuts[c] = Cut{q0, head.h, head.rows, c - k + 1};
+    }
   }
 }
 
-// Joins the pieces of a (sequence, KV head) that CTA runs have cut.
+// Joins the pieces of the (sequence, KV head)s that CTAs' ends have cut, in
+// order: CTA i the one that run i ends, its warps by query row, several to a
+// row where there are few rows.
+constexpr int kJoinWarps = 8;
+
 template <int D>
-__global__ void __launch_bounds__(128) paged_decode_join_kernel(PagedAttnArgs a, int grid) {
-  __shared__ long long before_s, total_s;
-  __shared__ float fac[kRowsD][kMaxPieces];
-  __shared__ float sum[kRowsD];
-  const PagedBatch& bt = a.batch;
-  const int tid = threadIdx.x, nkv = a.pool.nkv, G = a.nq / nkv;
-  const int b = blockIdx.x / nkv, h = blockIdx.x % nkv;
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(const __grid_constant__ PagedAttnArgs a,
+                                                                           int row_cap) {
+  constexpr int N = D / 32;
+  __shared__ float part[kJoinWarps][32][N + 3];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int G = a.nq / a.pool.nkv;
+  const float* ws = (const float*)a.ws;
+  const int grid = gridDim.x, last = blockIdx.x;
   pdl_trigger();
-  if (tid == 0) before_s = total_s = 0;
-  __syncthreads();
-  // Lengths were written before the attention kernel began, which allows this
-  // kernel to start only after its own wait.
-  long long before = 0, total = 0;
-  for (int i = tid; i < bt.B; i += 128) {
-    const long long x = (long long)decode_chunks(seq_span(bt, i, a.pool.ps), G) * nkv;
-    total += x;
-    if (i < b) before += x;
-  }
-  atomicAdd((unsigned long long*)&total_s, (unsigned long long)total);
-  atomicAdd((unsigned long long*)&before_s, (unsigned long long)before);
-  const SeqSpan sp = seq_span(bt, b, a.pool.ps);
-  const int C = decode_chunks(sp, G);
-  __syncthreads();
   pdl_wait();
-  if (C == 0 || total_s >= 0x7fffffffLL) return;
-  const Runs runs(total_s, grid);
-  // The ends of runs that cut this pair (none of them moved): c_lo + 1 .. c_hi.
-  const long long p0 = before_s + (long long)h * C;
-  if (C <= 2 * kSnap) return;
-  int c_lo = (int)((p0 + kSnap) * runs.grid / runs.total);  // the last run that begins at p0 + kSnap or before
-  while (c_lo + 1 < runs.grid && runs.raw(c_lo + 1) <= p0 + kSnap) ++c_lo;
-  while (c_lo > 0 && runs.raw(c_lo) > p0 + kSnap) --c_lo;
-  int c_hi = c_lo;
-  while (c_hi + 1 < runs.grid && runs.raw(c_hi + 1) < p0 + C - kSnap) ++c_hi;
-  if (c_lo == c_hi) return;
-  const int rows = sp.n * G, np = c_hi - c_lo + 1;
-  // A CTA's first pair is its slot 0 if an earlier run begins it, else slot 1.
-  auto piece = [&](int k) { return (const float*)a.ws + (size_t)(2 * (c_lo + k) + (k > 0 ? 0 : 1)) * kRowsD * (D + 2); };
-  for (int i = tid; i < rows * np; i += 128) fac[i / np][i % np] = __ldcg(piece(i % np) + (i / np) * (D + 2));
-  __syncthreads();
-  if (tid < rows) {
-    float M = -INFINITY, S = 0.f;
-    for (int k = 0; k < np; ++k) M = fmaxf(M, fac[tid][k]);
-    for (int k = 0; k < np; ++k) {
-      const float f = fac[tid][k] == -INFINITY ? 0.f : ex2(fac[tid][k] - M);
-      fac[tid][k] = f;
-      S += f * __ldcg(piece(k) + tid * (D + 2) + 1);
-    }
-    sum[tid] = S;
-  }
-  __syncthreads();
-  for (int i = tid; i < rows * D; i += 128) {
-    const int r = i / D, d = i % D;
-    float acc = 0.f;
-    for (int k0 = 0; k0 < np; k0 += 8) {
-      float v[8];
+  const int4 x = __ldcg(reinterpret_cast<const int4*>(ws + (size_t)2 * grid * piece_floats(row_cap, D)) + last);
+  const Cut cut{x.x, x.y, x.z, x.w};
+  if (cut.rows == 0) return;
+  const int per = cut.rows >= kJoinWarps ? 1 : kJoinWarps / cut.rows;  // warps of a row
+  for (int r0 = 0; r0 < cut.rows; r0 += kJoinWarps / per) {
+    const int r = r0 + warp / per, sub = warp % per;
+    const bool mine = warp / per < kJoinWarps / per && r < cut.rows;
+    float M = -INFINITY, L = 0.f, acc[N];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = k0 + k < np ? __ldcg(piece(k0 + k) + r * (D + 2) + 2 + d) : 0.f;
+    for (int i = 0; i < N; ++i) acc[i] = 0.f;
+    auto add = [&](float m, float l, const float* v) {
+      const float top = fmaxf(M, m);
+      const float keep = M == -INFINITY ? 0.f : ex2(M - top), f = m == -INFINITY ? 0.f : ex2(m - top);
+      M = top;
+      L = L * keep + f * l;
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (k0 + k < np) acc += fac[r][k0 + k] * v[k];
+      for (int i = 0; i < N; ++i) acc[i] = acc[i] * keep + f * v[i];
+    };
+    if (mine) {
+      for (int k0 = sub; k0 < cut.pieces; k0 += 8 * per) {
+        float2 ml[8];
+        float v[8][N];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {  // eight pieces' loads in flight
+          const int i = min(k0 + k * per, cut.pieces - 1);
+          // the first piece is its run's slot 1, the others their runs' slot 0
+          const float* q = ws + (size_t)(2 * (last - cut.pieces + 1 + i) + (i == 0 ? 1 : 0)) * piece_floats(row_cap, D) + (size_t)r * (D + 2);
+          ml[k] = __ldcg(reinterpret_cast<const float2*>(q + D));
+#pragma unroll
+          for (int j = 0; j < N / 2; ++j) {
+            const float2 y = __ldcg(reinterpret_cast<const float2*>(q + lane * N + 2 * j));
+            v[k][2 * j] = y.x, v[k][2 * j + 1] = y.y;
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k0 + k * per < cut.pieces) add(ml[k].x, ml[k].y, v[k]);
+      }
     }
-    ((__nv_bfloat16*)a.out)[(int64_t)(sp.q0 + r / G) * a.ldo + (int64_t)(h * G + r % G) * a.hdo + d] =
-        __float2bfloat16_rn(sum[r] == 0.f ? 0.f : acc / sum[r]);
+    if (per > 1) {  // then cut.rows < kJoinWarps: one round
+      if (mine && sub > 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) part[warp][lane][i] = acc[i];
+        part[warp][lane][N] = M;
+        part[warp][lane][N + 1] = L;
+      }
+      __syncthreads();
+      if (mine && sub == 0)
+        for (int k = 1; k < per; ++k) add(part[warp + k][lane][N], part[warp + k][lane][N + 1], part[warp + k][lane]);
+    }
+    if (mine && sub == 0) {
+      const float f = L == 0.f ? 0.f : 1.f / L;
+      __nv_bfloat16* out = (__nv_bfloat16*)a.out + (int64_t)(cut.q0 + r / G) * a.ldo + (int64_t)(cut.h * G + r % G) * a.hdo + lane * N;
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) *reinterpret_cast<uint32_t*>(out + 2 * i) = pack2(acc[2 * i] * f, acc[2 * i + 1] * f);
+    }
   }
-}
-
-int decode_grid(const PagedAttnArgs& a) {
-  const int64_t most = (int64_t)a.batch.B * a.pool.nkv *
-                       std::max<int64_t>(1, ((int64_t)a.batch.max_pages * a.pool.ps + kChunkD - 1) / kChunkD);
-  return (int)std::min<int64_t>(std::min<int64_t>(usable_sms(), kMaxPieces), most);
 }
 
 int row_cap(const PagedAttnArgs& a) {
@@ -619,22 +668,20 @@ int row_cap(const PagedAttnArgs& a) {
 template <int D, bool E4, int NT>
 cudaError_t launch_decode(const PagedAttnArgs& a, cudaStream_t s) {
   auto kernel = paged_decode_kernel<D, E4, NT>;
-  const int rows = std::min(8, row_cap(a));
-  const size_t smem = (size_t)(kWarps * rows * (D + 2) + kWarps * 8 + 16 + 3 * a.batch.B + 1) * 4;
+  auto bytes = [](int rows, int B) { return (size_t)(2 * kWarps * piece_floats(rows, D) + 3 * B + 1) * 4; };
   static bool configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (!configured[dev]) {
-    const size_t most = (size_t)(kWarps * 8 * (D + 2) + kWarps * 8 + 16 + 3 * kPagedMaxBatch + 1) * 4;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes(8 * NT, kPagedMaxBatch));
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
-  const int grid = decode_grid(a);
-  cudaError_t e = launch_pdl(kernel, dim3(grid), dim3(kThreadsD), smem, s, a, rows);
+  const int rows = row_cap(a), grid = usable_sms();
+  cudaError_t e = launch_pdl(kernel, dim3(grid), dim3(kWarps * 32), bytes(rows, a.batch.B), s, a, rows);
   if (e != cudaSuccess) return e;
-  return launch_pdl(paged_decode_join_kernel<D>, dim3((unsigned)(a.batch.B * a.pool.nkv)), dim3(128), 0, s, a, grid);
+  return launch_pdl(paged_decode_join_kernel<D>, dim3(grid), dim3(kJoinWarps * 32), 0, s, a, rows);
 }
 
 }  // namespace
@@ -645,7 +692,7 @@ bool paged_decode_applicable(const PagedAttnArgs& a) {
 }
 
 size_t paged_decode_workspace(const PagedAttnArgs& a) {
-  return (size_t)2 * decode_grid(a) * kRowsD * (a.pool.D + 2) * sizeof(float);
+  return (size_t)usable_sms() * (2 * piece_floats(row_cap(a), a.pool.D) * sizeof(float) + sizeof(Cut));
 }
 
 cudaError_t launch_paged_decode(const PagedAttnArgs& a, cudaStream_t s) {

@@ -341,7 +341,7 @@ typedef struct mg_paged_pool {
   int32_t cache_dtype; /* the activations' dtype, or MG_DTYPE_E4M3 */
 } mg_paged_pool;
 
-/* A ragged batch of at most 4096 sequences and fewer than 2^26 token rows.  Sequence b brings the token rows
+/* A ragged batch of at most 2048 sequences and fewer than 2^26 token rows.  Sequence b brings the token rows
  * q_start[b] .. q_start[b + 1] - 1 (possibly none) and holds kv_len[b] cached
  * tokens with them; its token j lies in page page_table[b table_stride +
  * j / page_size].  All three arrays are on the device and are read by the

@@ -57,7 +57,7 @@ SHARED = [
     (dict(v=BASE + 8), dict(), dict(), "16-byte"),
     (dict(), dict(batch=-1), dict(), "negative"),
     (dict(), dict(max_new=-1), dict(), "negative"),
-    (dict(), dict(batch=4097), dict(), "4096"),
+    (dict(), dict(batch=2049), dict(), "2048"),
     (dict(), dict(tokens=1 << 26), dict(), "2^26"),
     (dict(), dict(q_start=None), dict(), "null"),
     (dict(), dict(max_pages=0), dict(), "columns"),
