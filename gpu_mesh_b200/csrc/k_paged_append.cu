@@ -16,8 +16,11 @@
 // which is exact too until they reach the subnormals.
 //
 // Bound: memory, T·(2 nq + 2 nkv)·D·e bytes read or written plus the codes.
-// One thread holds 16 bytes of a head, a head's D / N lanes reduce its norm
-// and swap rotate-half partners by shuffles, so a row is read once.
+// A thread holds 16 bytes of a head, a head's D / N lanes reduce its norm and
+// swap rotate-half partners by shuffles, so a row is read once.  A warp takes
+// one token, whose table entries stay in its registers over all heads (eight
+// warps share a token where there are few); its rows are requested before the
+// sequence is looked up.
 #include <math.h>
 
 #include <algorithm>
@@ -29,44 +32,84 @@ namespace mg {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kRowVecs = 4;   // 16-byte vectors of a token row that a thread loads before it computes
+constexpr int kWarpsA = kThreads / 32;
+constexpr int kAhead = 4;     // 16-byte vectors of a token row that a thread requests at once
 constexpr int kThinNew = 8;   // most new tokens per sequence for which a token's CTA also stores its run of rows
 
 template <typename T, int D>
 struct Shape {
   static constexpr int N = 16 / sizeof(T);  // elements of a vector
   static constexpr int LPH = D / N;         // lanes of a head
+  static constexpr int HPW = 32 / LPH;      // heads that a warp holds at once
+  static constexpr int K = N < D / 2 ? N : D / 2;  // table entries of a vector's dims
   static_assert(LPH >= 1 && LPH <= 32, "a head lies inside a warp");
 };
 
-// The sequence that token row t belongs to (-1: behind the last one).  The
-// CTA's threads look at the batch's ranges side by side: one round trip to
-// memory where a bisection makes log2(B).
-__device__ __forceinline__ int find_seq(const PagedBatch& b, int t, int* found) {
-  if (threadIdx.x == 0) *found = -1;
-  __syncthreads();
-  for (int i = threadIdx.x; i < b.B; i += kThreads)
-    if (b.q_start[i] <= t && t < b.q_start[i + 1]) *found = i;
-  __syncthreads();
-  return *found;
+template <typename T>
+__device__ __forceinline__ void widen(const uint4& v, float* x) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 2) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    } else {
+      x[i] = __uint_as_float(w[i]);
+    }
+  }
+}
+
+// The sequence of token row t (-1: behind the last one) and its span, by a
+// whole warp: the lanes look at the batch's ranges side by side, one round
+// trip to memory for 32 sequences.
+__device__ __forceinline__ int find_seq(const PagedBatch& bt, int t, int ps, SeqSpan* span) {
+  const int lane = threadIdx.x & 31;
+  for (int i0 = 0; i0 < bt.B; i0 += 32) {
+    const int i = min(i0 + lane, bt.B - 1);
+    const SeqSpan s = seq_span(bt, i, ps);
+    const unsigned hit = __ballot_sync(0xffffffffu, s.ok && s.q0 <= t && t < s.q0 + s.n);
+    if (hit) {
+      const int at = __ffs(hit) - 1;
+      span->ok = true;
+      span->q0 = __shfl_sync(0xffffffffu, s.q0, at);
+      span->n = __shfl_sync(0xffffffffu, s.n, at);
+      span->past = __shfl_sync(0xffffffffu, s.past, at);
+      return min(i0 + at, bt.B - 1);
+    }
+  }
+  return -1;
 }
 
 // Rotary row of token row t at cache position j.
 __device__ __forceinline__ int64_t rope_pos(const PagedAppendArgs& a, int t, int j) {
   int64_t pos = a.positions ? a.positions[t] : (int64_t)j;
   if (pos < 0 || pos >= a.max_pos) {
-    if (a.cos) flag_error(a.err, kErrPositionRange);
+    flag_error(a.err, kErrPositionRange);
     pos = pos < 0 ? 0 : a.max_pos - 1;
   }
   return pos;
 }
 
-// Norm and rotation of the N elements at dims d0.. of a head; every lane of
-// the warp takes part in the shuffles.
+// The table entries of the dims at d0.
 template <typename T, int D>
-__device__ __forceinline__ void norm_rotate(const PagedAppendArgs& a, float* x, int d0, const T* w, bool rotate,
-                                            int64_t pos) {
-  constexpr int N = Shape<T, D>::N, LPH = Shape<T, D>::LPH, half = D / 2;
+struct Rope {
+  float c[Shape<T, D>::K], s[Shape<T, D>::K];
+  __device__ __forceinline__ void load(const PagedAppendArgs& a, int64_t pos, int d0) {
+    const size_t at = (size_t)pos * (D / 2) + d0 % (D / 2);
+#pragma unroll
+    for (int i = 0; i < Shape<T, D>::K / 4; ++i) {
+      load16_f<float>(a.cos + at + 4 * i, c + 4 * i);
+      load16_f<float>(a.sin + at + 4 * i, s + 4 * i);
+    }
+  }
+};
+
+// Norm (by the weights w, or NULL) and rotation (where `rotate`) of the N elements at dims d0 of a head; every lane of the warp
+// takes part in the shuffles.
+template <typename T, int D>
+__device__ __forceinline__ void norm_rotate(const PagedAppendArgs& a, float* x, int d0, const void* w, bool rotate,
+                                            const Rope<T, D>& rope) {
+  constexpr int N = Shape<T, D>::N, LPH = Shape<T, D>::LPH, K = Shape<T, D>::K, half = D / 2;
   if (a.q_norm || a.k_norm) {
     float ss = 0.f;
 #pragma unroll
@@ -76,7 +119,7 @@ __device__ __forceinline__ void norm_rotate(const PagedAppendArgs& a, float* x, 
     if (w) {
       const float r = 1.0f / sqrtf(ss / (float)D + a.eps);
       float g[N];
-      load16_f<T>(w + d0, g);
+      load16_f<T>((const T*)w + d0, g);
 #pragma unroll
       for (int i = 0; i < N; ++i) x[i] = x[i] * r * g[i];
     }
@@ -91,19 +134,9 @@ __device__ __forceinline__ void norm_rotate(const PagedAppendArgs& a, float* x, 
     for (int i = 0; i < N; ++i) other[i] = x[(i + N / 2) % N];
   }
   if (!rotate) return;
-  const float* c = a.cos + (size_t)pos * half;
-  const float* s = a.sin + (size_t)pos * half;
-  constexpr int K = N < half ? N : half;  // table entries of these dims
-  const int k0 = d0 % half;
-  float cv[K], sv[K];
-#pragma unroll
-  for (int i = 0; i < K / 4; ++i) {
-    load16_f<float>(c + k0 + 4 * i, cv + 4 * i);
-    load16_f<float>(s + k0 + 4 * i, sv + 4 * i);
-  }
 #pragma unroll
   for (int i = 0; i < N; ++i)
-    x[i] = fmaf(x[i], cv[i % K], d0 + i < half ? -other[i] * sv[i % K] : other[i] * sv[i % K]);
+    x[i] = fmaf(x[i], rope.c[i % K], d0 + i < half ? -other[i] * rope.s[i % K] : other[i] * rope.s[i % K]);
 }
 
 // The N values at p as e4m3 codes of scale 1 / inv.
@@ -153,180 +186,208 @@ __device__ __forceinline__ float finite_abs(float x) {
   return m <= 3.402823466e38f ? m : 0.f;  // not an infinity, not NaN
 }
 
+// One run of rows, the new tokens of a sequence in one page, for one (head, K
+// or V) of an e4m3 pool, by a whole CTA: the largest magnitude of all rows
+// gives the scale, so the rows stay in registers as they were read and the
+// norm and rotation run twice, which costs less than registers for fp32 rows
+// (they bound the loads in flight).
+template <typename T, int D>
+__device__ __forceinline__ void store_run(const PagedAppendArgs& a, int slot, int u) {
+  constexpr int N = Shape<T, D>::N, LPH = Shape<T, D>::LPH;
+  constexpr int RPI = kThreads / LPH;             // rows per round
+  constexpr int IT = RPI >= 128 ? 1 : 128 / RPI;  // rounds of the largest page
+  __shared__ float warp_amax[kWarpsA];
+  const PagedPool& pool = a.pool;
+  const PagedBatch& bt = a.batch;
+  const int tid = threadIdx.x, d0 = tid % LPH * N, r0 = tid / LPH;
+  const int h = u % pool.nkv;
+  const bool is_v = u >= pool.nkv;
+  // Sequence b's runs are the slots q_start[b] / ps + 2 b + r; it has at most
+  // n / ps + 2 of them.  Every warp looks it up by itself, as find_seq does.
+  const int lane = tid & 31;
+  SeqSpan sp;
+  int b = -1;
+  for (int i0 = 0; i0 < bt.B && b < 0; i0 += 32) {
+    const int i = min(i0 + lane, bt.B - 1);
+    const SeqSpan s = seq_span(bt, i, pool.ps);
+    const bool in = s.ok && s.q0 / pool.ps + 2 * i <= slot && slot < (s.q0 + s.n) / pool.ps + 2 * (i + 1);
+    const unsigned hit = __ballot_sync(0xffffffffu, in);
+    if (hit) {
+      const int at = __ffs(hit) - 1;
+      b = min(i0 + at, bt.B - 1);
+      sp.q0 = __shfl_sync(0xffffffffu, s.q0, at);
+      sp.n = __shfl_sync(0xffffffffu, s.n, at);
+      sp.past = __shfl_sync(0xffffffffu, s.past, at);
+    }
+  }
+  if (b < 0 || sp.past < 0) return;
+  const int pi = sp.past / pool.ps + slot - (sp.q0 / pool.ps + 2 * b);  // page of the sequence
+  const int j0 = max(sp.past, pi * pool.ps), j1 = min(sp.past + sp.n, (pi + 1) * pool.ps);
+  if (j0 >= j1) return;
+  const int nr = j1 - j0, off = j0 - pi * pool.ps, t0 = sp.q0 + j0 - sp.past;
+  const int page = bt.table[(int64_t)b * bt.ld + pi];
+  uint4 raw[IT];
+  const T* rows = (const T*)a.qkv + (int64_t)t0 * a.ldqkv + (size_t)(a.nq + u) * D + d0;
+#pragma unroll
+  for (int it = 0; it < IT; ++it) {
+    const int r = it * RPI + r0;
+    raw[it] = r < nr ? *reinterpret_cast<const uint4*>(rows + (int64_t)r * a.ldqkv) : make_uint4(0u, 0u, 0u, 0u);
+  }
+  if (page < 0 || page >= pool.pages) {
+    if (tid == 0) flag_error(a.err, kErrPaged);
+    return;
+  }
+  float* sc = is_v ? pool.vs + (int64_t)page * pool.vse + h : pool.ks + (int64_t)page * pool.kse + h;
+  const float old = off > 0 ? *sc : 0.f;
+  auto value = [&](int it, float* x) {
+    widen<T>(raw[it], x);
+    if (is_v) return;
+    const int r = min(it * RPI + r0, nr - 1);
+    Rope<T, D> rope;
+    if (a.cos) rope.load(a, rope_pos(a, t0 + r, j0 + r), d0);
+    norm_rotate<T, D>(a, x, d0, a.k_norm, true, rope);
+  };
+  float amax = 0.f;
+#pragma unroll
+  for (int it = 0; it < IT; ++it) {
+    if (it * RPI >= nr) break;  // uniform over the CTA
+    float x[N];
+    value(it, x);
+#pragma unroll
+    for (int i = 0; i < N; ++i) amax = fmaxf(amax, finite_abs(x[i]));
+  }
+  amax = warp_max(amax);
+  if ((tid & 31) == 0) warp_amax[tid >> 5] = amax;
+  __syncthreads();  // also: every thread has read the old scale
+#pragma unroll
+  for (int i = 0; i < kWarpsA; ++i) amax = fmaxf(amax, warp_amax[i]);
+  int e = e4m3_exp(amax);
+  uint8_t* base = is_v ? (uint8_t*)pool.v + page * pool.vp + h * pool.vh : (uint8_t*)pool.k + page * pool.kp + h * pool.kh;
+  const int64_t ts = is_v ? pool.vt : pool.kt;
+  if (off > 0) {
+    const int eo = scale_exp(old);
+    if (e > eo) move_codes(base, ts, D, off, pow2i(eo - e), tid, kThreads);
+    e = max(e, eo);
+  }
+  if (tid == 0) *sc = pow2i(e);
+  const float inv = pow2i(-e);
+#pragma unroll
+  for (int it = 0; it < IT; ++it) {
+    if (it * RPI >= nr) break;
+    float x[N];
+    value(it, x);
+    const int r = it * RPI + r0;
+    if (r < nr) store_codes<N>(base + (int64_t)(off + r) * ts + d0, x, inv);
+  }
+}
+
 // kMode 0: the pool holds the activation type.  1: e4m3, a token's CTA also
 // stores the run of rows (new tokens in one page) that it begins.  2: e4m3,
-// tile CTAs store the runs and token CTAs rotate the queries only.
+// CTAs below `tiles` store a run each and the others rotate the queries only.
+// `per`: warps of a token (8 in mode 1).
 template <typename T, int D, int kMode>
-__global__ void __launch_bounds__(kThreads) paged_append_kernel(PagedAppendArgs a, int slots) {
-  constexpr int N = Shape<T, D>::N, LPH = Shape<T, D>::LPH;
-  __shared__ int found;
-  __shared__ float warp_amax[kThreads / 32];
+__global__ void __launch_bounds__(kThreads, kMode == 1 ? 2 : 4)
+    paged_append_kernel(const __grid_constant__ PagedAppendArgs a, int tiles, int per) {
+  using S = Shape<T, D>;
+  constexpr int N = S::N, LPH = S::LPH, HPW = S::HPW;
   pdl_trigger();
   pdl_wait();
   const PagedPool& pool = a.pool;
   const PagedBatch& bt = a.batch;
-  const int tid = threadIdx.x;
-  const int hl = tid % LPH, d0 = hl * N;
-  const int nh = a.nq + 2 * pool.nkv;
-
-  if (kMode == 2 && blockIdx.x < (unsigned)(slots * 2 * pool.nkv)) {
-    // One run: (sequence, page) x (head, K or V).  Sequence b's runs are the
-    // slots q_start[b] / ps + 2 b + r; it has at most n / ps + 2 of them.
-    const int slot = blockIdx.x / (2 * pool.nkv), u = blockIdx.x % (2 * pool.nkv);
-    const int h = u % pool.nkv;
-    const bool is_v = u >= pool.nkv;
-    if (tid == 0) found = -1;
-    __syncthreads();
-    for (int i = tid; i < bt.B; i += kThreads) {
-      const int lo = bt.q_start[i] / pool.ps + 2 * i, hi = bt.q_start[i + 1] / pool.ps + 2 * (i + 1);
-      if (lo <= slot && slot < hi) found = i;
-    }
-    __syncthreads();
-    const int b = found;
-    if (b < 0) return;
-    const SeqSpan sp = seq_span(bt, b, pool.ps);
-    if (!sp.ok || sp.past < 0) return;
-    const int pi = sp.past / pool.ps + slot - (sp.q0 / pool.ps + 2 * b);  // page of the sequence
-    const int j0 = max(sp.past, pi * pool.ps), j1 = min(sp.past + sp.n, (pi + 1) * pool.ps);
-    if (j0 >= j1) return;
-    const int page = bt.table[(int64_t)b * bt.ld + pi];
-    if (page < 0 || page >= pool.pages) {
-      if (tid == 0) flag_error(a.err, kErrPaged);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int block = blockIdx.x;
+  if (kMode == 2) {
+    if (block < tiles) {
+      store_run<T, D>(a, block / (2 * pool.nkv), block % (2 * pool.nkv));
       return;
     }
-    constexpr int RPI = kThreads / LPH;                    // rows per round
-    constexpr int IT = RPI >= 128 ? 1 : 128 / RPI;         // rounds of the largest page
-    const int r0 = tid / LPH, nr = j1 - j0, off = j0 - pi * pool.ps;
-    float x[IT][N];
-#pragma unroll
-    for (int it = 0; it < IT; ++it) {
-      const int r = it * RPI + r0;
-      if (r < nr) {
-        load16_f<T>((const T*)a.qkv + (int64_t)(sp.q0 + j0 - sp.past + r) * a.ldqkv + (size_t)(a.nq + u) * D + d0, x[it]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[it][i] = 0.f;
-      }
-    }
-    float* sc = is_v ? pool.vs + (int64_t)page * pool.vse + h : pool.ks + (int64_t)page * pool.kse + h;
-    const float old = off > 0 ? *sc : 0.f;
-    float amax = 0.f;
-#pragma unroll
-    for (int it = 0; it < IT; ++it) {
-      if (it * RPI >= nr) break;  // uniform over the CTA
-      const int r = it * RPI + r0;
-      if (!is_v) {
-        const int t = sp.q0 + j0 - sp.past + (r < nr ? r : 0);
-        norm_rotate<T, D>(a, x[it], d0, (const T*)a.k_norm, true, a.cos ? rope_pos(a, t, j0 + (r < nr ? r : 0)) : 0);
-      }
-#pragma unroll
-      for (int i = 0; i < N; ++i) amax = fmaxf(amax, finite_abs(x[it][i]));
-    }
-    amax = warp_max(amax);
-    if ((tid & 31) == 0) warp_amax[tid >> 5] = amax;
-    __syncthreads();  // also: every thread has read the old scale
-#pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) amax = fmaxf(amax, warp_amax[w]);
-    int e = e4m3_exp(amax);
-    uint8_t* base = is_v ? (uint8_t*)pool.v + page * pool.vp + h * pool.vh : (uint8_t*)pool.k + page * pool.kp + h * pool.kh;
-    const int64_t ts = is_v ? pool.vt : pool.kt;
-    if (off > 0) {
-      const int eo = scale_exp(old);
-      if (e > eo) move_codes(base, ts, D, off, pow2i(eo - e), tid, kThreads);
-      e = max(e, eo);
-    }
-    if (tid == 0) *sc = pow2i(e);
-    const float inv = pow2i(-e);
-#pragma unroll
-    for (int it = 0; it < IT; ++it) {
-      const int r = it * RPI + r0;
-      if (r < nr) store_codes<N>(base + (int64_t)(off + r) * ts + d0, x[it], inv);
-    }
-    return;
+    block -= tiles;
   }
-
-  const int t = kMode == 2 ? blockIdx.x - slots * 2 * pool.nkv : blockIdx.x;
-  if (t == bt.T) {  // the last CTA looks the batch over: a range that does not fit may own no CTA above
+  if (block == (int)gridDim.x - tiles - 1) {  // the last CTA looks the batch over: a range that does not fit may own no row
     for (int i = tid; i < bt.B; i += kThreads) {
       const SeqSpan sp = seq_span(bt, i, pool.ps);
       if (!sp.ok || (sp.n > 0 && sp.past < 0)) flag_error(a.err, kErrPaged);
     }
     return;
   }
-  const int b = find_seq(bt, t, &found);
-  if (b < 0) return;  // a row behind the last sequence
-  const SeqSpan sp = seq_span(bt, b, pool.ps);
-  if (!sp.ok || sp.past < 0) return;
+  const int t = block * (kWarpsA / per) + warp / per, sub = warp % per;
+  if (t >= bt.T) return;
+  const int hl = lane % LPH, d0 = hl * N;
+  // Queries (kMode 0: keys and values too): groups of HPW heads, every per-th
+  // of them, kAhead at a time; the first are requested before the lookups.
+  const int heads = kMode == 0 ? a.nq + 2 * pool.nkv : a.nq;
+  const T* row = (const T*)a.qkv + (int64_t)t * a.ldqkv;
+  uint4 raw[kAhead];
+  auto request = [&](int g0) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int hh = (g0 + k * per) * HPW + lane / LPH;
+      raw[k] = hh < heads ? *reinterpret_cast<const uint4*>(row + (size_t)hh * D + d0) : make_uint4(0u, 0u, 0u, 0u);
+    }
+  };
+  request(sub);
+  SeqSpan sp;
+  const int b = find_seq(bt, t, pool.ps, &sp);
+  if (b < 0 || sp.past < 0) return;  // a row behind the last sequence, or of one that does not fit
   const int j = sp.past + t - sp.q0;
-  const int64_t pos = a.cos ? rope_pos(a, t, j) : 0;
   const int pi = j / pool.ps, off = j - pi * pool.ps;
   const int page = bt.table[(int64_t)b * bt.ld + pi];
+  Rope<T, D> rope;
+  if (a.cos) rope.load(a, rope_pos(a, t, j), d0);
   const bool page_ok = page >= 0 && page < pool.pages;
-  if (!page_ok && tid == 0) flag_error(a.err, kErrPaged);
+  if (!page_ok && lane == 0) flag_error(a.err, kErrPaged);
 
-  // Queries (kMode 0: keys and values too), vector by vector.
-  const int vecs = (kMode == 0 ? nh : a.nq) * LPH;
-  const T* row = (const T*)a.qkv + (int64_t)t * a.ldqkv;
-  for (int v0 = 0; v0 < vecs; v0 += kRowVecs * kThreads) {
-    float x[kRowVecs][N];
+  for (int g0 = sub; g0 * HPW < heads; g0 += kAhead * per) {
 #pragma unroll
-    for (int k = 0; k < kRowVecs; ++k) {
-      const int v = v0 + k * kThreads + tid;
-      if (v < vecs) {
-        load16_f<T>(row + (size_t)v * N, x[k]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[k][i] = 0.f;
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < kRowVecs; ++k) {
-      const int v = v0 + k * kThreads + tid;
-      if (v0 + k * kThreads >= vecs) break;  // uniform over the CTA
-      const int hh = v / LPH;
+    for (int k = 0; k < kAhead; ++k) {
+      if ((g0 + k * per) * HPW >= heads) break;  // uniform over the warp
+      const int hh = (g0 + k * per) * HPW + lane / LPH;
       const bool is_q = hh < a.nq, is_v = hh >= a.nq + pool.nkv;
-      norm_rotate<T, D>(a, x[k], d0, is_v ? nullptr : is_q ? (const T*)a.q_norm : (const T*)a.k_norm, !is_v, pos);
-      if (v >= vecs) continue;
+      float x[N];
+      widen<T>(raw[k], x);
+      norm_rotate<T, D>(a, x, d0, is_v ? nullptr : is_q ? a.q_norm : a.k_norm, !is_v, rope);
+      if (hh >= heads) continue;
       if (is_q) {
-        store16_f<T>((T*)a.q_out + (int64_t)t * a.ldq + (size_t)hh * D + d0, x[k]);
+        store16_f<T>((T*)a.q_out + (int64_t)t * a.ldq + (size_t)hh * D + d0, x);
       } else if (page_ok) {
         const int h = hh - a.nq - (is_v ? pool.nkv : 0);
         T* dst = is_v ? (T*)pool.v + page * pool.vp + h * pool.vh + off * pool.vt
                       : (T*)pool.k + page * pool.kp + h * pool.kh + off * pool.kt;
-        store16_f<T>(dst + d0, x[k]);
+        store16_f<T>(dst + d0, x);
       }
     }
+    if ((g0 + kAhead * per) * HPW < heads) request(g0 + kAhead * per);
   }
   if constexpr (kMode == 1) {
     // A run begins at the sequence's first new token and at each page's start.
     if (!page_ok || (t != sp.q0 && off != 0)) return;
     const int nr = min(min(sp.n - (t - sp.q0), pool.ps - off), kThinNew);
-    constexpr int UPR = kThreads / LPH;  // units (head, K or V) per round
-    for (int u0 = 0; u0 < 2 * pool.nkv; u0 += UPR) {
-      const int u = u0 + tid / LPH;
+    for (int u0 = warp * HPW; u0 < 2 * pool.nkv; u0 += kWarpsA * HPW) {  // units: (head, K or V)
+      const int u = u0 + lane / LPH;
       const bool valid = u < 2 * pool.nkv;
       const bool is_v = valid && u >= pool.nkv;
       const int h = is_v ? u - pool.nkv : u;
-      float x[kThinNew][N];
+      uint4 rw[kThinNew];
 #pragma unroll
-      for (int r = 0; r < kThinNew; ++r) {
-        if (valid && r < nr) {
-          load16_f<T>((const T*)a.qkv + (int64_t)(t + r) * a.ldqkv + (size_t)(a.nq + u) * D + d0, x[r]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < N; ++i) x[r][i] = 0.f;
-        }
-      }
+      for (int r = 0; r < kThinNew; ++r)
+        rw[r] = valid && r < nr ? *reinterpret_cast<const uint4*>(row + (int64_t)r * a.ldqkv + (size_t)(a.nq + u) * D + d0)
+                                : make_uint4(0u, 0u, 0u, 0u);
       float* sc = is_v ? pool.vs + (int64_t)page * pool.vse + h : pool.ks + (int64_t)page * pool.kse + h;
       const float old = valid && off > 0 ? *sc : 0.f;
+      auto value = [&](int r, float* x) {
+        widen<T>(rw[r], x);
+        Rope<T, D> at = rope;
+        if (a.cos && r > 0) at.load(a, rope_pos(a, t + r, j + r), d0);
+        norm_rotate<T, D>(a, x, d0, valid && !is_v ? a.k_norm : nullptr, valid && !is_v, at);
+      };
       float amax = 0.f;
 #pragma unroll
       for (int r = 0; r < kThinNew; ++r) {
         if (r >= nr) break;  // uniform over the CTA
-        norm_rotate<T, D>(a, x[r], d0, valid && !is_v ? (const T*)a.k_norm : nullptr, valid && !is_v,
-                          a.cos ? rope_pos(a, t + r, j + r) : 0);
+        float x[N];
+        value(r, x);
 #pragma unroll
-        for (int i = 0; i < N; ++i) amax = fmaxf(amax, finite_abs(x[r][i]));
+        for (int i = 0; i < N; ++i) amax = fmaxf(amax, finite_abs(x[i]));
       }
 #pragma unroll
       for (int o = LPH / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
@@ -346,28 +407,35 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(PagedAppendArgs 
         const int src = __ffs(grew) - 1;
         uint8_t* bs = (uint8_t*)__shfl_sync(0xffffffffu, (unsigned long long)base, src);
         const int64_t st = (int64_t)__shfl_sync(0xffffffffu, (long long)ts, src);
-        move_codes(bs, st, D, off, pow2i(__shfl_sync(0xffffffffu, shift, src)), tid & 31, 32);
+        move_codes(bs, st, D, off, pow2i(__shfl_sync(0xffffffffu, shift, src)), lane, 32);
       }
-      if (!valid) continue;
-      if (hl == 0) *sc = pow2i(e);
+      if (valid && hl == 0) *sc = pow2i(e);
       const float inv = pow2i(-e);
 #pragma unroll
-      for (int r = 0; r < kThinNew; ++r)
-        if (r < nr) store_codes<N>(base + (int64_t)(off + r) * ts + d0, x[r], inv);
+      for (int r = 0; r < kThinNew; ++r) {
+        if (r >= nr) break;
+        float x[N];
+        value(r, x);
+        if (valid) store_codes<N>(base + (int64_t)(off + r) * ts + d0, x, inv);
+      }
     }
   }
 }
 
 template <typename T, int D>
 cudaError_t launch_d(const PagedAppendArgs& a, cudaStream_t s) {
-  const int T_rows = a.batch.T;
+  const int rows = a.batch.T;
+  // As many warps per token as 16 warps per SM allow (32 rows: 8, 1000 rows: 2
+  // warps were fastest of 1, 2, 4 and 8).
+  int per = kWarpsA;
+  while (per > 1 && (int64_t)rows * per > 16 * usable_sms()) per /= 2;
+  const int blocks = (rows + kWarpsA / per - 1) / (kWarpsA / per) + 1;
   if (a.pool.cdtype != kE4M3)
-    return launch_pdl(paged_append_kernel<T, D, 0>, dim3(T_rows + 1), dim3(kThreads), 0, s, a, 0);
+    return launch_pdl(paged_append_kernel<T, D, 0>, dim3(blocks), dim3(kThreads), 0, s, a, 0, per);
   if (a.batch.max_new <= kThinNew)
-    return launch_pdl(paged_append_kernel<T, D, 1>, dim3(T_rows + 1), dim3(kThreads), 0, s, a, 0);
-  const int slots = T_rows / a.pool.ps + 2 * a.batch.B;
-  return launch_pdl(paged_append_kernel<T, D, 2>, dim3((unsigned)(slots * 2 * a.pool.nkv + T_rows + 1)), dim3(kThreads), 0,
-                    s, a, slots);
+    return launch_pdl(paged_append_kernel<T, D, 1>, dim3(rows + 1), dim3(kThreads), 0, s, a, 0, kWarpsA);
+  const int tiles = (rows / a.pool.ps + 2 * a.batch.B) * 2 * a.pool.nkv;
+  return launch_pdl(paged_append_kernel<T, D, 2>, dim3((unsigned)(tiles + blocks)), dim3(kThreads), 0, s, a, tiles, per);
 }
 
 template <typename T>
