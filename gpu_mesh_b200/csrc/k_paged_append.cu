@@ -187,24 +187,30 @@ __device__ __forceinline__ float finite_abs(float x) {
 }
 
 // One run of rows, the new tokens of a sequence in one page, for one (head, K
-// or V) of an e4m3 pool, by a whole CTA: the largest magnitude of all rows
-// gives the scale, so the rows stay in registers as they were read and the
-// norm and rotation run twice, which costs less than registers for fp32 rows
-// (they bound the loads in flight).
+// or V) of an e4m3 pool, or several where the pages are small, by a whole
+// CTA: the largest magnitude of all rows gives the scale, so the rows stay in
+// registers as they were read and the norm and rotation run twice, which
+// costs less than registers for fp32 rows (they bound the loads in flight).
 template <typename T, int D>
-__device__ __forceinline__ void store_run(const PagedAppendArgs& a, int slot, int u) {
-  constexpr int N = Shape<T, D>::N, LPH = Shape<T, D>::LPH;
-  constexpr int RPI = kThreads / LPH;             // rows per round
-  constexpr int IT = RPI >= 128 ? 1 : 128 / RPI;  // rounds of the largest page
-  __shared__ float warp_amax[kWarpsA];
+struct RunShape {
+  static constexpr int RPI = kThreads / Shape<T, D>::LPH;  // rows per round
+  static constexpr int IT = RPI >= 128 ? 1 : 128 / RPI;    // rounds of a CTA: the largest page
+  __host__ __device__ static constexpr int rounds(int ps) { return (ps + RPI - 1) / RPI; }  // of one unit
+  // (Head, K or V)s of a CTA: four of 16-token pages, of 64-token pages one.
+  __host__ __device__ static constexpr int units(int ps) { return ps >= 64 ? 1 : IT / rounds(ps) < 64 / ps ? IT / rounds(ps) : 64 / ps; }
+};
+
+// `rounds` and `IT` (the rounds of all units) are the page size's.
+template <typename T, int D, int rounds, int IT>
+__device__ __forceinline__ void store_run(const PagedAppendArgs& a, int slot, int u0) {
+  constexpr int N = Shape<T, D>::N, LPH = Shape<T, D>::LPH, RPI = RunShape<T, D>::RPI;
+  __shared__ float run_amax[IT], run_old[IT];
   const PagedPool& pool = a.pool;
   const PagedBatch& bt = a.batch;
-  const int tid = threadIdx.x, d0 = tid % LPH * N, r0 = tid / LPH;
-  const int h = u % pool.nkv;
-  const bool is_v = u >= pool.nkv;
+  const int tid = threadIdx.x, lane = tid & 31, d0 = tid % LPH * N, r0 = tid / LPH;
+  const int units = min(IT / rounds, 2 * pool.nkv - u0);
   // Sequence b's runs are the slots q_start[b] / ps + 2 b + r; it has at most
   // n / ps + 2 of them.  Every warp looks it up by itself, as find_seq does.
-  const int lane = tid & 31;
   SeqSpan sp;
   int b = -1;
   for (int i0 = 0; i0 < bt.B && b < 0; i0 += 32) {
@@ -226,64 +232,74 @@ __device__ __forceinline__ void store_run(const PagedAppendArgs& a, int slot, in
   if (j0 >= j1) return;
   const int nr = j1 - j0, off = j0 - pi * pool.ps, t0 = sp.q0 + j0 - sp.past;
   const int page = bt.table[(int64_t)b * bt.ld + pi];
+  // Round `it` is rows (it % rounds)·RPI .. of unit u0 + it / rounds.
   uint4 raw[IT];
-  const T* rows = (const T*)a.qkv + (int64_t)t0 * a.ldqkv + (size_t)(a.nq + u) * D + d0;
+  const T* rows = (const T*)a.qkv + (int64_t)t0 * a.ldqkv + (size_t)(a.nq + u0) * D + d0;
 #pragma unroll
   for (int it = 0; it < IT; ++it) {
-    const int r = it * RPI + r0;
-    raw[it] = r < nr ? *reinterpret_cast<const uint4*>(rows + (int64_t)r * a.ldqkv) : make_uint4(0u, 0u, 0u, 0u);
+    const int u = it / rounds, r = (it - u * rounds) * RPI + r0;
+    raw[it] = r < nr && u < units ? *reinterpret_cast<const uint4*>(rows + (int64_t)r * a.ldqkv + u * D) : make_uint4(0u, 0u, 0u, 0u);
   }
   if (page < 0 || page >= pool.pages) {
     if (tid == 0) flag_error(a.err, kErrPaged);
     return;
   }
-  float* sc = is_v ? pool.vs + (int64_t)page * pool.vse + h : pool.ks + (int64_t)page * pool.kse + h;
-  const float old = off > 0 ? *sc : 0.f;
+  auto scale_at = [&](int u) {
+    return u >= pool.nkv ? pool.vs + (int64_t)page * pool.vse + u - pool.nkv : pool.ks + (int64_t)page * pool.kse + u;
+  };
+  auto codes_at = [&](int u) {
+    return u >= pool.nkv ? (uint8_t*)pool.v + page * pool.vp + (u - pool.nkv) * pool.vh
+                         : (uint8_t*)pool.k + page * pool.kp + u * pool.kh;
+  };
+  if (tid < units) {
+    run_amax[tid] = 0.f;
+    run_old[tid] = off > 0 ? *scale_at(u0 + tid) : 0.f;
+  }
+  __syncthreads();
   auto value = [&](int it, float* x) {
+    const int u = it / rounds, r = min((it - u * rounds) * RPI + r0, nr - 1);
     widen<T>(raw[it], x);
-    if (is_v) return;
-    const int r = min(it * RPI + r0, nr - 1);
+    if (u0 + u >= pool.nkv) return;  // values: as they are
     Rope<T, D> rope;
     if (a.cos) rope.load(a, rope_pos(a, t0 + r, j0 + r), d0);
     norm_rotate<T, D>(a, x, d0, a.k_norm, true, rope);
   };
-  float amax = 0.f;
+#pragma unroll
+  for (int u = 0; u < IT / rounds; ++u) {
+    if (u >= units) break;  // uniform over the CTA
+    float amax = 0.f;
+#pragma unroll
+    for (int it = u * rounds; it < (u + 1) * rounds; ++it) {
+      if ((it - u * rounds) * RPI >= nr) break;
+      float x[N];
+      value(it, x);
+#pragma unroll
+      for (int i = 0; i < N; ++i) amax = fmaxf(amax, finite_abs(x[i]));
+    }
+    amax = warp_max(amax);
+    if (lane == 0) atomicMax((int*)&run_amax[u], __float_as_int(amax));  // magnitudes order as integers
+  }
+  __syncthreads();
+  for (int u = 0; u < units && off > 0; ++u) {
+    const int e = e4m3_exp(run_amax[u]), eo = scale_exp(run_old[u]);
+    if (e > eo) move_codes(codes_at(u0 + u), u0 + u >= pool.nkv ? pool.vt : pool.kt, D, off, pow2i(eo - e), tid, kThreads);
+  }
 #pragma unroll
   for (int it = 0; it < IT; ++it) {
-    if (it * RPI >= nr) break;  // uniform over the CTA
+    const int u = it / rounds, r = (it - u * rounds) * RPI + r0;
+    if ((it - u * rounds) * RPI >= nr || u >= units) continue;
+    int e = e4m3_exp(run_amax[u]);
+    if (off > 0) e = max(e, scale_exp(run_old[u]));
+    if (r == 0 && d0 == 0) *scale_at(u0 + u) = pow2i(e);
     float x[N];
     value(it, x);
-#pragma unroll
-    for (int i = 0; i < N; ++i) amax = fmaxf(amax, finite_abs(x[i]));
-  }
-  amax = warp_max(amax);
-  if ((tid & 31) == 0) warp_amax[tid >> 5] = amax;
-  __syncthreads();  // also: every thread has read the old scale
-#pragma unroll
-  for (int i = 0; i < kWarpsA; ++i) amax = fmaxf(amax, warp_amax[i]);
-  int e = e4m3_exp(amax);
-  uint8_t* base = is_v ? (uint8_t*)pool.v + page * pool.vp + h * pool.vh : (uint8_t*)pool.k + page * pool.kp + h * pool.kh;
-  const int64_t ts = is_v ? pool.vt : pool.kt;
-  if (off > 0) {
-    const int eo = scale_exp(old);
-    if (e > eo) move_codes(base, ts, D, off, pow2i(eo - e), tid, kThreads);
-    e = max(e, eo);
-  }
-  if (tid == 0) *sc = pow2i(e);
-  const float inv = pow2i(-e);
-#pragma unroll
-  for (int it = 0; it < IT; ++it) {
-    if (it * RPI >= nr) break;
-    float x[N];
-    value(it, x);
-    const int r = it * RPI + r0;
-    if (r < nr) store_codes<N>(base + (int64_t)(off + r) * ts + d0, x, inv);
+    if (r < nr) store_codes<N>(codes_at(u0 + u) + (int64_t)(off + r) * (u0 + u >= pool.nkv ? pool.vt : pool.kt) + d0, x, pow2i(-e));
   }
 }
 
 // kMode 0: the pool holds the activation type.  1: e4m3, a token's CTA also
 // stores the run of rows (new tokens in one page) that it begins.  2: e4m3,
-// CTAs below `tiles` store a run each and the others rotate the queries only.
+// CTAs below `tiles` store a run's units each and the others rotate the queries only.
 // `per`: warps of a token (8 in mode 1).
 template <typename T, int D, int kMode>
 __global__ void __launch_bounds__(kThreads, kMode == 1 ? 2 : 4)
@@ -298,7 +314,15 @@ __global__ void __launch_bounds__(kThreads, kMode == 1 ? 2 : 4)
   int block = blockIdx.x;
   if (kMode == 2) {
     if (block < tiles) {
-      store_run<T, D>(a, block / (2 * pool.nkv), block % (2 * pool.nkv));
+      const int units = RunShape<T, D>::units(pool.ps), per_slot = (2 * pool.nkv + units - 1) / units;
+      const int slot = block / per_slot, u0 = block % per_slot * units;
+      using RS = RunShape<T, D>;
+      switch (pool.ps) {
+        case 16: store_run<T, D, RS::rounds(16), RS::rounds(16) * RS::units(16)>(a, slot, u0); break;
+        case 32: store_run<T, D, RS::rounds(32), RS::rounds(32) * RS::units(32)>(a, slot, u0); break;
+        case 64: store_run<T, D, RS::rounds(64), RS::rounds(64) * RS::units(64)>(a, slot, u0); break;
+        default: store_run<T, D, RS::rounds(128), RS::rounds(128) * RS::units(128)>(a, slot, u0); break;
+      }
       return;
     }
     block -= tiles;
@@ -434,7 +458,8 @@ cudaError_t launch_d(const PagedAppendArgs& a, cudaStream_t s) {
     return launch_pdl(paged_append_kernel<T, D, 0>, dim3(blocks), dim3(kThreads), 0, s, a, 0, per);
   if (a.batch.max_new <= kThinNew)
     return launch_pdl(paged_append_kernel<T, D, 1>, dim3(rows + 1), dim3(kThreads), 0, s, a, 0, kWarpsA);
-  const int tiles = (rows / a.pool.ps + 2 * a.batch.B) * 2 * a.pool.nkv;
+  const int units = RunShape<T, D>::units(a.pool.ps);
+  const int tiles = (rows / a.pool.ps + 2 * a.batch.B) * ((2 * a.pool.nkv + units - 1) / units);
   return launch_pdl(paged_append_kernel<T, D, 2>, dim3((unsigned)(tiles + blocks)), dim3(kThreads), 0, s, a, tiles, per);
 }
 
