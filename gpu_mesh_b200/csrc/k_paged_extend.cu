@@ -260,6 +260,31 @@ __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
   return r;
 }
 
+// Two fp32 operations in one instruction; a pair is two consecutive registers.
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ void split_pair(uint64_t p, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 template <int D, bool E4>
 __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
     paged_extend_kernel(const __grid_constant__ PoolMaps maps, const __grid_constant__ CUtensorMap tm_q,
@@ -386,37 +411,40 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
         const int nv = vis - k0;  // visible keys of this chunk for this row
         const bool clear = __all_sync(0xffffffffu, nv >= kChunkE);
         const uint32_t tS = tmem + lanes + kColSE + 128 * x;
-        // Half a chunk's scores, in base 2.  e4m3: with the page's K scale and
-        // V exponent, 16 keys at a time; bf16: the factor is left to the
-        // exponential (it is positive and commutes with the maximum).
-        auto scores = [&](int hf, float* sc) {
+        auto scores = [&](int hf, float* sc) {  // half a chunk's, -inf where the row does not see the key
           tmem_ld64(tS + 64 * hf, sc);
-          if constexpr (E4) {
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const float f = rowf * sks[(pos & 1) * 8 + 4 * hf + g], e = (float)sve[(pos & 1) * 8 + 4 * hf + g];
-#pragma unroll
-              for (int i = 0; i < 16; ++i) sc[16 * g + i] = fmaf(sc[16 * g + i], f, e);
-            }
-          }
           if (!clear) {
 #pragma unroll
             for (int k = 0; k < 64; ++k) sc[k] = 64 * hf + k < nv ? sc[k] : -INFINITY;
           }
         };
-        // The maximum first, then the weights: the scores are read from TMEM
-        // twice, 64 at a time, which keeps the kernel's warps within their registers.
-        float t8[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) t8[i] = -INFINITY;
+        // Score k in base 2 is sc·f + e with f > 0 and e the same for 16 keys
+        // (a page's K scale and V exponent; bf16: the softmax scale and 0), so
+        // the maximum is taken of the raw scores, 16 at a time.  The scores
+        // are read from TMEM twice, 64 at a time, which keeps the kernel's
+        // warps within their registers.
+        auto factor = [&](int at) { return fmaxf(rowf * sks[at], 1.17549435e-38f); };  // never 0: -inf · 0 is NaN
+        float mt = -INFINITY;
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
           float sc[64];
           scores(hf, sc);
 #pragma unroll
-          for (int k = 0; k < 64; ++k) t8[k & 7] = fmaxf(t8[k & 7], sc[k]);
+          for (int g = 0; g < 4; ++g) {
+            float x = max3(sc[16 * g], sc[16 * g + 1], sc[16 * g + 2]), y = max3(sc[16 * g + 3], sc[16 * g + 4], sc[16 * g + 5]);
+            x = max3(x, sc[16 * g + 6], sc[16 * g + 7]);
+            y = max3(y, sc[16 * g + 8], sc[16 * g + 9]);
+            x = max3(x, sc[16 * g + 10], sc[16 * g + 11]);
+            y = max3(y, sc[16 * g + 12], sc[16 * g + 13]);
+            x = max3(x, sc[16 * g + 14], sc[16 * g + 15]);
+            if constexpr (E4) {
+              const int at = (pos & 1) * 8 + 4 * hf + g;
+              mt = fmaxf(mt, fmaf(fmaxf(x, y), factor(at), (float)sve[at]));
+            } else {
+              mt = max3(mt, x, y);
+            }
+          }
         }
-        float mt = fmaxf(fmaxf(fmaxf(t8[0], t8[1]), fmaxf(t8[2], t8[3])), fmaxf(fmaxf(t8[4], t8[5]), fmaxf(t8[6], t8[7])));
         if constexpr (!E4) mt *= scale2;
         float m_new = m;
         bool moved = false;
@@ -436,16 +464,22 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
           scores(hf, sc);
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
-            float s0 = 0.f, s1 = 0.f;
+            const int at = (pos & 1) * 8 + 4 * hf + g;
+            const float f = E4 ? factor(at) : scale2, e = E4 ? (float)sve[at] - mb : -mb;
+            const uint64_t ff = pair_of(f, f), ee = pair_of(e, e);
+            uint64_t sum = 0;  // two zeros
 #pragma unroll
             for (int i = 16 * g; i < 16 * g + 16; i += 2) {
-              sc[i] = ex2(E4 ? sc[i] - mb : fmaf(sc[i], scale2, -mb));
-              sc[i + 1] = ex2(E4 ? sc[i + 1] - mb : fmaf(sc[i + 1], scale2, -mb));
-              s0 += sc[i];
-              s1 += sc[i + 1];
-              sc[i / 2] = __uint_as_float(E4 ? pack_f16(sc[i], sc[i + 1]) : bf16_pair(sc[i], sc[i + 1]));
+              float y0, y1;
+              split_pair(fma_pair(pair_of(sc[i], sc[i + 1]), ff, ee), y0, y1);
+              y0 = ex2(y0);
+              y1 = ex2(y1);
+              sum = add_pair(sum, pair_of(y0, y1));
+              sc[i / 2] = __uint_as_float(E4 ? pack_f16(y0, y1) : bf16_pair(y0, y1));
             }
-            add = E4 ? fmaf(s0 + s1, pow2i(-7 - sve[(pos & 1) * 8 + 4 * hf + g]), add) : add + (s0 + s1);
+            float s0, s1;
+            split_pair(sum, s0, s1);
+            add = E4 ? fmaf(s0 + s1, pow2i(-7 - sve[at]), add) : add + (s0 + s1);
           }
           tmem_st32(tS + 32 * hf, sc);  // P over scores that have been read for good
         }
@@ -537,7 +571,7 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
     int n = 0;
     bool ok = true;
     uint4 kx[NI], vx[NI];
-    float ks = 0.f, vs = 1.f;
+    float ks = 1.f, vs = 1.f;
     // Codes of chunk `chunk` of the walk's sequence and head (zeros behind its end).
     auto load = [&](const Walk& w, int chunk) {
       const int len = w.p.s.past + w.p.s.n;
@@ -557,8 +591,7 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
           }
         }
       }
-      ks = 0.f;
-      vs = 1.f;
+      ks = vs = 1.f;
       const int j = chunk * kChunkE + dt * 16;  // threads 0-7: the scales of 16 keys
       if (dt < 8 && j < len) {
         const int page = __ldg(tab + j / pool.ps);
