@@ -564,62 +564,69 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
     }
     if (!ok) *abort_flag = 1;
   } else if (E4 && warp < R::kProducer) {
-    // Converters: thread dt takes 16 codes (piece pc) of rows rr + RPI·i.
+    // Converters: a thread takes 16 codes (piece pc of a row) of rows rr +
+    // RPI·i.  Eight lanes hold four pieces of two rows, so that their halves
+    // go to eight different groups of banks.
     constexpr int PPR = D / 16, RPI = 128 / PPR, NI = kChunkE / RPI;
-    const int dt = threadIdx.x - R::kSoft * 32;
-    const int rr = dt / PPR, pc = dt % PPR;
+    const int dt = threadIdx.x - R::kSoft * 32, cw = dt >> 5;
+    const int pc = D == 128 ? (lane & 3) + 4 * ((lane >> 3) & 1) : lane & 3;
+    const int rr = D == 128 ? cw * 4 + ((lane >> 2) & 1) + 2 * (lane >> 4) : cw * 8 + (lane >> 2);
+    const int page_shift = 31 - __clz(pool.ps), page_mask = pool.ps - 1;
     int n = 0;
     bool ok = true;
     uint4 kx[NI], vx[NI];
     float ks = 1.f, vs = 1.f;
+    int page = -1;  // lanes 0-7: the page of 16 keys of the chunk after the one in registers
+    // Looks up the pages of a chunk, a chunk before load() needs them.
+    auto look_up = [&](const Walk& w, int chunk) {
+      const int j = chunk * kChunkE + (lane & 7) * 16;
+      page = j < w.p.s.past + w.p.s.n ? __ldg(bt.table + (int64_t)w.at.b * bt.ld + (j >> page_shift)) : -1;
+    };
     // Codes of chunk `chunk` of the walk's sequence and head (zeros behind its end).
     auto load = [&](const Walk& w, int chunk) {
-      const int len = w.p.s.past + w.p.s.n;
-      const int32_t* tab = bt.table + (int64_t)w.at.b * bt.ld;
+      const int len = w.p.s.past + w.p.s.n, k0 = chunk * kChunkE;
+      if ((unsigned)page >= (unsigned)pool.pages) {
+        if (k0 + (lane & 7) * 16 < len) flag_error(a.err, kErrPaged);
+        page = -1;
+      }
+      const uint8_t* kb = (const uint8_t*)pool.k + w.at.h * pool.kh + pc * 16;
+      const uint8_t* vb = (const uint8_t*)pool.v + w.at.h * pool.vh + pc * 16;
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        const int j = chunk * kChunkE + rr + RPI * i;
+        const int r = rr + RPI * i, pg = __shfl_sync(0xffffffffu, page, r >> 4);
+        const int o = (k0 + r) & page_mask;
         kx[i] = vx[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (j < len) {
-          const int page = __ldg(tab + j / pool.ps);
-          if (page >= 0 && page < pool.pages) {
-            const int o = j % pool.ps;
-            kx[i] = *reinterpret_cast<const uint4*>((const uint8_t*)pool.k + page * pool.kp + w.at.h * pool.kh + o * pool.kt + pc * 16);
-            vx[i] = *reinterpret_cast<const uint4*>((const uint8_t*)pool.v + page * pool.vp + w.at.h * pool.vh + o * pool.vt + pc * 16);
-          } else {
-            flag_error(a.err, kErrPaged);
-          }
+        if (pg >= 0 && k0 + r < len) {
+          kx[i] = *reinterpret_cast<const uint4*>(kb + pg * pool.kp + o * pool.kt);
+          vx[i] = *reinterpret_cast<const uint4*>(vb + pg * pool.vp + o * pool.vt);
         }
       }
       ks = vs = 1.f;
-      const int j = chunk * kChunkE + dt * 16;  // threads 0-7: the scales of 16 keys
-      if (dt < 8 && j < len) {
-        const int page = __ldg(tab + j / pool.ps);
-        if (page >= 0 && page < pool.pages) {
-          ks = pool.ks[(int64_t)page * pool.kse + w.at.h];
-          vs = pool.vs[(int64_t)page * pool.vse + w.at.h];
-        }
+      if (dt < 8 && page >= 0) {
+        ks = pool.ks[page * pool.kse + w.at.h];
+        vs = pool.vs[page * pool.vse + w.at.h];
       }
     };
-    auto put = [&](uint8_t* tile, int row, const uint4& v) {
-      const uint32_t cw[4] = {v.x, v.y, v.z, v.w};
+    // 16 codes are 32 bytes of halves: two pieces of the row's 64-dim block.
+    const uint32_t at0 = (pc >> 2) * kBoxE + rr * 128 + ((((pc & 3) * 2) ^ (rr & 7)) << 4), at1 = at0 ^ 16;
+    auto put = [&](uint8_t* tile, int i, const uint4& v) {
+      const uint32_t cw4[4] = {v.x, v.y, v.z, v.w};
       uint32_t f[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        f[2 * i] = e4m3x2_to_f16x2(cw[i]);
-        f[2 * i + 1] = e4m3x2_hi_to_f16x2(cw[i]);
+      for (int k = 0; k < 4; ++k) {
+        f[2 * k] = e4m3x2_to_f16x2(cw4[k]);
+        f[2 * k + 1] = e4m3x2_hi_to_f16x2(cw4[k]);
       }
-      uint8_t* base = tile + (pc >> 2) * kBoxE + row * 128;
-      const int p0 = (pc & 3) * 2;
-      const uint4 lo = make_uint4(f[0], f[1], f[2], f[3]), hi = make_uint4(f[4], f[5], f[6], f[7]);
-      // The second block's lanes write their odd piece first: eight lanes then cover eight banks' groups.
-      const bool odd = (pc >> 2) & 1;
-      *reinterpret_cast<uint4*>(base + (((p0 + odd) ^ (row & 7)) << 4)) = odd ? hi : lo;
-      *reinterpret_cast<uint4*>(base + (((p0 + 1 - odd) ^ (row & 7)) << 4)) = odd ? lo : hi;
+      *reinterpret_cast<uint4*>(tile + at0 + i * RPI * 128) = make_uint4(f[0], f[1], f[2], f[3]);
+      *reinterpret_cast<uint4*>(tile + at1 + i * RPI * 128) = make_uint4(f[4], f[5], f[6], f[7]);
     };
     Walk w(a, pre, u0, u1);
     while (!w.done() && w.nch == 0) w.next();
-    if (!w.done()) load(w, w.lo);
+    if (!w.done()) {
+      look_up(w, w.lo);
+      load(w, w.lo);
+      look_up(w, w.lo + 1);
+    }
     while (!w.done() && ok) {
       for (int ch = 0; ch < w.nch; ++ch, ++n) {
         const int s = n & 1;
@@ -632,21 +639,28 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
         uint8_t* st = skv + s * 2 * L::kKV;
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-          put(st, rr + RPI * i, kx[i]);
-          put(st + L::kKV, rr + RPI * i, vx[i]);
+          put(st, i, kx[i]);
+          put(st + L::kKV, i, vx[i]);
         }
-        if (dt < 8) {
+        if (dt < 8) {  // the chunk's scales, as load() left them
           sks[s * 8 + dt] = ks;
           sve[s * 8 + dt] = scale_exp(vs);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive(&kvfull[s]);
-        if (ch + 1 < w.nch) load(w, w.lo + ch + 1);
+        if (ch + 1 < w.nch) {
+          load(w, w.lo + ch + 1);
+          look_up(w, w.lo + ch + 2);
+        }
       }
       if (!ok) break;
       do w.next(); while (!w.done() && w.nch == 0);
-      if (!w.done()) load(w, w.lo);
+      if (!w.done()) {
+        look_up(w, w.lo);
+        load(w, w.lo);
+        look_up(w, w.lo + 1);
+      }
     }
     if (!ok) *abort_flag = 1;
   } else if (warp == R::kProducer) {
