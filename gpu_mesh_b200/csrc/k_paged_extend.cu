@@ -12,21 +12,30 @@
 // workspace, and a second kernel joins the pieces in order.
 //
 // Warp roles:
-//   * softmax (4 warps per tile): one thread per query row (its TMEM lane).
-//     Online softmax in base 2; the maximum moves only when a row's scores
-//     outgrow it by 2^8, and only then is the row of O in TMEM rescaled.  P
-//     goes back into TMEM over the scores.
+//   * softmax (8 warps per tile): two threads per query row (its TMEM lane),
+//     half of the chunk's keys each; they exchange maxima through shared
+//     memory.  Online softmax in base 2; the maximum moves only when a row's
+//     scores outgrow it by 2^8, and only then is the row of O in TMEM rescaled.
+//     P goes back into TMEM over the scores.  The time from scores to P is
+//     what a tile waits for, with one thread per row twice as long.
 //   * MMA issuer: S_X = Q_X·Kᵀ and O_X += P_X·V per tile X, ping-ponging, P
 //     read from TMEM, V read MN-major.
-//   * producer: the tiles' query rows by 3-D TMA over {dim, head, token};
-//     bf16 pages by 4-D TMA, looked up four chunks at a time.
-//   * e4m3 pages, four converter warps: 16 codes per load, a chunk ahead in
-//     registers, to halves (exact) in the tiles' swizzled layout; rows behind
-//     the sequence become zeros.  Q becomes halves scaled by a power of two
-//     per row (exact), K's scale multiplies the fp32 scores, V's scale 2^e
-//     joins the exponent: P' = 2^(s + e - m + 7) in half (2^-11 relative, down
-//     to 2^-21 of the largest, and within 2^-31 of it below), while the sum
-//     adds 2^(s - m) in fp32.  fp8 MMAs would need P in e4m3: 2^-4.
+//   * producer: the tiles' query rows by 3-D TMA over {dim, head, token}; the
+//     chunks' keys and values, each with a ring of its own (keys are free for
+//     the next chunk long before values), by 4-D TMA over the pages, looked up
+//     four chunks at a time.
+// e4m3 pages:
+//   * Scores by fp8 MMAs straight on the codes.  Q, brought to [128, 256) per
+//     row by a power of two, is the sum of two e4m3 numbers: a bf16 has eight
+//     significant bits, and the nearest e4m3 leaves a remainder of at most
+//     four.  That is exact for elements down to 2^-10 of the row's largest; a
+//     smaller one is off by at most 2^-17 of it (the remainder is subnormal).
+//   * K's scale multiplies the fp32 scores; V's scale 2^e joins the exponent:
+//     P' = 2^(s + e - m + 7) in half (2^-11 relative, down to 2^-21 of the
+//     largest, and within 2^-31 of it below), while the sum adds 2^(s - m) in
+//     fp32.  P in e4m3 would be 2^-4, so the values are not multiplied as
+//     codes: two converter warps turn them into halves (exact), MN-major;
+//     rows behind the sequence become zeros.
 // P is bf16 over bf16 pages (2^-8 half step at most 2^-9 relative): the
 // precision in which the stage's own prefill multiplies the values.
 //
@@ -55,25 +64,33 @@ constexpr int kColSE = 0;        // TMEM: tile X's scores (then P) at 128·X, it
 constexpr int kColOE = 256;
 constexpr int kSmemE = 227 * 1024;
 
+// Warps of a CTA.
 template <bool E4>
 struct Roles {
-  static constexpr int kSoft = 8;                   // warps 0-3 tile A, 4-7 tile B
-  static constexpr int kConv = E4 ? 4 : 0;          // warps 8-11
+  static constexpr int kTileWarps = 8;          // softmax warps of a tile: two threads of a query row
+  static constexpr int kSoft = 2 * kTileWarps;
+  static constexpr int kConv = E4 ? 2 : 0;
   static constexpr int kProducer = kSoft + kConv;
   static constexpr int kMma = kProducer + 1;
   static constexpr int kThreads = 32 * (kMma + 1);
 };
 
-template <int D>
+template <int D, bool E4>
 struct ExtendLayout {
+  using Row = PoolRow<D, E4>;
   static constexpr int kDB = D / 64;
-  static constexpr int kQ = kDB * kBoxE;   // one tile's query rows
-  static constexpr int kKV = kDB * kBoxE;  // keys (or values) of a chunk, as 16-bit
+  static constexpr int kQ = kDB * kBoxE;                       // one tile's query rows (e4m3: as bf16, then as two code tiles)
+  static constexpr int kCodes = kChunkE * D;                   // a chunk's keys (or values, or a tile's rows) as codes
+  static constexpr int kK = E4 ? kCodes : kDB * kBoxE;         // a chunk's keys
+  static constexpr int kV = kDB * kBoxE;                       // a chunk's values, 16-bit
   static constexpr int kOffQ = 0;
-  static constexpr int kOffKV = 2 * kQ;
-  static constexpr int kOffBar = kOffKV + 2 * 2 * kKV;
-  static constexpr int kOffScale = kOffBar + 256;     // [stage][8] K scales, [stage][8] V exponents
-  static constexpr int kOffPre = kOffScale + 128;     // [B + 1] units before a sequence
+  static constexpr int kOffK = 2 * kQ;
+  static constexpr int kOffV = kOffK + 2 * kK;
+  static constexpr int kOffRaw = kOffV + 2 * kV;               // e4m3: the values' codes, two chunks
+  static constexpr int kOffBar = kOffRaw + (E4 ? 2 * kCodes : 0);
+  static constexpr int kOffScale = kOffBar + 256;              // [4][8] K scales, [4][8] V exponents
+  static constexpr int kOffRow = kOffScale + 256;              // [2][tile][half][row] what a row's two threads exchange
+  static constexpr int kOffPre = kOffRow + 2 * 2 * 2 * kTile * 4;  // [B + 1] units before a sequence
   static int bytes(int B) { return kOffPre + (B + 1 + 3) / 4 * 16 + 1024; }
 };
 
@@ -242,6 +259,24 @@ __device__ __forceinline__ void mma_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_
       "r"(tmem_a), "l"(b), "r"(idesc), "r"(acc));
 }
 
+// D (fp32) += A·Bᵀ, both e4m3 codes in shared memory, K = 32.
+__device__ __forceinline__ void mma_codes(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+
+// Shared-memory descriptor of a K-major tile of codes: rows of 128 bytes
+// swizzled over 128, or of 64 over 64; eight rows to a group (SBO).
+template <int D>
+__device__ __forceinline__ uint64_t desc_codes(const void* p) {
+  const uint64_t addr = smem_u32(p);
+  return ((addr & 0x3FFFFull) >> 4) | (1ull << 16) | ((uint64_t)(8 * D >> 4) << 32) | (1ull << 46) |
+         ((D == 128 ? 2ull : 4ull) << 61);
+}
+
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* tm, uint64_t* bar, int x, int y, int z) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
@@ -252,6 +287,21 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* tm, ui
 
 __device__ __forceinline__ bool warp_waits(uint64_t* bar, uint32_t parity, int* err) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, err));
+}
+
+// Barrier over the (eight) softmax warps of tile x that returns the OR of
+// `pred`, so that they all take the same branch afterwards.
+__device__ __forceinline__ bool tile_any(int x, bool pred) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.red.or.pred q, %2, 256, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)pred), "r"(1 + x)
+      : "memory");
+  return r != 0;
 }
 
 __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
@@ -289,7 +339,7 @@ template <int D, bool E4>
 __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
     paged_extend_kernel(const __grid_constant__ PoolMaps maps, const __grid_constant__ CUtensorMap tm_q,
                         const __grid_constant__ PagedAttnArgs a) {
-  using L = ExtendLayout<D>;
+  using L = ExtendLayout<D, E4>;
   using R = Roles<E4>;
   const PagedPool& pool = a.pool;
   const PagedBatch& bt = a.batch;
@@ -297,39 +347,55 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* sq = smem + L::kOffQ;    // tile X's query rows at sq + X·kQ
-  uint8_t* skv = smem + L::kOffKV;  // stage s: keys at skv + 2·s·kKV, values kKV after them
+  uint8_t* sk = smem + L::kOffK;    // stage s: a chunk's keys at sk + s·kK
+  uint8_t* sv = smem + L::kOffV;    // its values at sv + s·kV
+  uint8_t* sraw = smem + L::kOffRaw;  // e4m3: its values' codes at sraw + s·kCodes
   uint64_t* bars = (uint64_t*)(smem + L::kOffBar);
-  uint64_t* kvfull = bars;        // [2] chunk in shared memory
-  uint64_t* kvempty = bars + 2;   // [2] chunk's products done
-  uint64_t* sfull = bars + 4;     // [tile] scores ready in TMEM
-  uint64_t* pready = bars + 6;    // [tile] P written, O rescaled
-  uint64_t* odone = bars + 8;     // [tile] value product done
-  uint64_t* qfull = bars + 10;    // [tile] query rows landed
-  uint64_t* qempty = bars + 12;   // [tile] the piece's score products read them
-  uint64_t* qconv = bars + 14;    // [tile] query rows are halves (e4m3)
-  uint64_t* drain = bars + 16;    // every MMA finished
-  uint32_t* tmem_holder = (uint32_t*)(bars + 17);
+  uint64_t* kfull = bars;         // [2] a chunk's keys in shared memory
+  uint64_t* kempty = bars + 2;    // [2] its score products done
+  uint64_t* vfull = bars + 4;     // [2] its values in shared memory
+  uint64_t* vempty = bars + 6;    // [2] its value products done
+  uint64_t* sfull = bars + 8;     // [tile] scores ready in TMEM
+  uint64_t* pready = bars + 10;   // [tile] P written, O rescaled
+  uint64_t* odone = bars + 12;    // [tile] value product done
+  uint64_t* qfull = bars + 14;    // [tile] query rows landed
+  uint64_t* qempty = bars + 16;   // [tile] the piece's score products read them
+  uint64_t* qconv = bars + 18;    // [tile] query rows are halves (e4m3)
+  uint64_t* sready = bars + 20;   // [4] a chunk's scales written (e4m3)
+  uint64_t* rfull = bars + 24;    // [2] a chunk's values as codes landed (e4m3)
+  uint64_t* rempty = bars + 26;   // [2] converted
+  uint64_t* drain = bars + 28;    // every MMA finished
+  uint32_t* tmem_holder = (uint32_t*)(bars + 29);
   volatile int* abort_flag = (volatile int*)(tmem_holder + 1);
-  float* sks = (float*)(smem + L::kOffScale);  // [stage][8]
-  int* sve = (int*)(sks + 16);                 // [stage][8]
+  // The scales of chunk n in slot n & 3: the keys' stage is free again before
+  // the softmax of the chunk has ended, but chunk n + 4 is not converted before.
+  float* sks = (float*)(smem + L::kOffScale);  // [4][8]
+  int* sve = (int*)(sks + 32);                 // [4][8]
+  float* srow = (float*)(smem + L::kOffRow);
   int* pre = (int*)(smem + L::kOffPre);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&kvfull[s], E4 ? 4 : 1);
-      mbar_init(&kvempty[s], 1);
+      mbar_init(&kfull[s], 1);
+      mbar_init(&kempty[s], 1);
+      mbar_init(&vfull[s], E4 ? R::kConv : 1);
+      mbar_init(&vempty[s], 1);
+      mbar_init(&rfull[s], 1);
+      mbar_init(&rempty[s], E4 ? R::kConv : 1);
       mbar_init(&sfull[s], 1);
-      mbar_init(&pready[s], 4);
+      mbar_init(&pready[s], R::kTileWarps);
       mbar_init(&odone[s], 1);
       mbar_init(&qfull[s], 1);
       mbar_init(&qempty[s], 1);
-      mbar_init(&qconv[s], 4);
+      mbar_init(&qconv[s], R::kTileWarps);
     }
+    for (int s = 0; s < 4; ++s) mbar_init(&sready[s], 1);
     mbar_init(drain, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (E4 && threadIdx.x < 64) ((int*)sks)[threadIdx.x] = 0;  // sks and sve: finite where no page writes them
   pdl_wait();
   pdl_trigger();  // the join kernel reads, before its own wait, only what was written before this kernel
   count_units(a, pre, blockIdx.x == 0);
@@ -346,17 +412,28 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
   const uint32_t tmem = *tmem_holder;
   const int u0 = runs.begin(c), u1 = runs.begin(c + 1);
 
-  int issued = 0;         // chunks requested by TMA (bf16 producer)
+  int issued = 0, issued_v = 0;  // chunks whose keys, values were requested (producer)
   int qn[2] = {0, 0};     // query tiles requested (producer)
   if (warp < R::kSoft) {
-    const int x = warp >> 2, q4 = warp & 3;
+    const int x = warp / R::kTileWarps, hf = (warp >> 2) & 1, q4 = warp & 3;
     const int r = q4 * 32 + lane;
     const uint32_t lanes = (uint32_t)(q4 * 32) << 16;
+    const uint32_t tS = tmem + lanes + kColSE + 128 * x;
     const float scale2 = a.scale * 1.4426950408889634f;
-    int n = 0;    // ring position of the piece's first chunk
-    int cnt = 0;  // this tile's chunks so far (its sfull / pready / odone phases)
-    int qm = 0;   // query tiles so far
-    bool ok = true;
+    int n = 0;     // ring position of the piece's first chunk
+    int cnt = 0;   // this tile's chunks so far (its sfull / pready / odone phases)
+    int qm = 0;    // query tiles so far
+    int turn = 0;  // exchanges so far: they alternate between two slots, with a barrier in each
+    bool ok = true;  // of this warp; the tile's warps stop together, after a vote
+    // Exchanges v with the row's other thread; false if any of the tile's warps gave up a wait.
+    auto exchange = [&](float v, float& other) -> bool {
+      float* slot = srow + ((turn & 1) * 2 + x) * 2 * kTile;
+      ++turn;
+      slot[hf * kTile + r] = v;
+      const bool bad = tile_any(x, !ok);
+      other = slot[(1 - hf) * kTile + r];
+      return !bad;
+    };
     for (Walk w(a, pre, u0, u1); !w.done() && ok; w.next()) {
       const int qt = 2 * w.at.j + x;
       const int s_tok = qt * w.p.tq + r / G;  // this row's token
@@ -366,86 +443,90 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
       const int nchx = w.c(x);
       float rowf = scale2;
       if (E4 && nchx > 0) {
-        // The tile's rows, one per thread: to halves, scaled to [128, 256).
+        // The tile's rows, half a row per thread: scaled to [128, 256) and
+        // split into two codes per element, over the bf16 rows (all of which
+        // have been read at the exchange).
         ok = warp_waits(&qfull[x], qm & 1, a.err);
         ++qm;
-        if (!ok) break;
-        uint8_t* row = sq + x * L::kQ + r * 128;
-        float amax = 0.f;
+        constexpr int NP = D / 16;  // 16-byte pieces of half a row
+        uint8_t* tile = sq + x * L::kQ;
+        uint4 v[NP];
+        float amax = 0.f, other;
 #pragma unroll
-        for (int p = 0; p < D / 8; ++p) {
-          const uint4 v = *reinterpret_cast<const uint4*>(row + (p >> 3) * kBoxE + (((p & 7) ^ (r & 7)) << 4));
-          const uint32_t wv[4] = {v.x, v.y, v.z, v.w};
+        for (int p = 0; p < NP; ++p) {
+          const int k = hf * NP + p;
+          v[p] = *reinterpret_cast<const uint4*>(tile + (k >> 3) * kBoxE + r * 128 + (((k & 7) ^ (r & 7)) << 4));
+          const uint32_t wv[4] = {v[p].x, v[p].y, v[p].z, v[p].w};
 #pragma unroll
           for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fmaxf(fabsf(lo_bf16(wv[i])), fabsf(hi_bf16(wv[i]))));
         }
-        const int sh = row_shift(amax);
+        if (!exchange(amax, other)) {
+          ok = false;
+          break;
+        }
+        const int sh = row_shift(fmaxf(amax, other));
         const float f = pow2i(sh);
         rowf = scale2 * pow2i(-sh);
 #pragma unroll
-        for (int p = 0; p < D / 8; ++p) {
-          uint4* at = reinterpret_cast<uint4*>(row + (p >> 3) * kBoxE + (((p & 7) ^ (r & 7)) << 4));
-          const uint4 v = *at;
-          *at = make_uint4(pack_f16(lo_bf16(v.x) * f, hi_bf16(v.x) * f), pack_f16(lo_bf16(v.y) * f, hi_bf16(v.y) * f),
-                           pack_f16(lo_bf16(v.z) * f, hi_bf16(v.z) * f), pack_f16(lo_bf16(v.w) * f, hi_bf16(v.w) * f));
+        for (int p = 0; p < NP / 2; ++p) {  // 16 elements: a 16-byte piece of codes
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint4 q = v[2 * p + i / 2];
+            const uint32_t w0 = i % 2 ? q.z : q.x, w1 = i % 2 ? q.w : q.y;
+            const float e0 = lo_bf16(w0) * f, e1 = hi_bf16(w0) * f, e2 = lo_bf16(w1) * f, e3 = hi_bf16(w1) * f;
+            hi[i] = to_e4m3x2(e0, e1) | (to_e4m3x2(e2, e3) << 16);
+            const float2 a01 = from_e4m3x2(hi[i]), a23 = from_e4m3x2(hi[i] >> 16);
+            lo[i] = to_e4m3x2(e0 - a01.x, e1 - a01.y) | (to_e4m3x2(e2 - a23.x, e3 - a23.y) << 16);
+          }
+          const uint32_t at = L::Row::at(r, hf * (NP / 2) + p);
+          *reinterpret_cast<uint4*>(tile + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<uint4*>(tile + L::kCodes + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive(&qconv[x]);
       }
 
-      float m = -INFINITY, l = 0.f;  // base-2 maximum that P is taken against, sum
+      float m = -INFINITY, l = 0.f;  // base-2 maximum that P is taken against, sum of this thread's keys
       for (int ch = 0; ch < nchx; ++ch, ++cnt) {
         const int pos = n + ch, k0 = (w.lo + ch) * kChunkE;
-        if (!warp_waits(&sfull[x], (int)(cnt & 1), a.err)) {
-          ok = false;
-          break;
-        }
+        ok = warp_waits(&sfull[x], (int)(cnt & 1), a.err);
+        if constexpr (E4) ok = ok && warp_waits(&sready[pos & 3], (int)(pos >> 2) & 1, a.err);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        if constexpr (E4) {
-          if (!warp_waits(&kvfull[pos & 1], (int)(pos >> 1) & 1, a.err)) {
-            ok = false;
-            break;
-          }
-        }
-        const int nv = vis - k0;  // visible keys of this chunk for this row
-        const bool clear = __all_sync(0xffffffffu, nv >= kChunkE);
-        const uint32_t tS = tmem + lanes + kColSE + 128 * x;
-        auto scores = [&](int hf, float* sc) {  // half a chunk's, -inf where the row does not see the key
-          tmem_ld64(tS + 64 * hf, sc);
-          if (!clear) {
+        const int nv = vis - k0 - 64 * hf;  // visible keys of this half chunk for this row
+        float sc[64];
+        tmem_ld64(tS + 64 * hf, sc);
+        if (!__all_sync(0xffffffffu, nv >= 64)) {
 #pragma unroll
-            for (int k = 0; k < 64; ++k) sc[k] = 64 * hf + k < nv ? sc[k] : -INFINITY;
-          }
-        };
+          for (int k = 0; k < 64; ++k) sc[k] = k < nv ? sc[k] : -INFINITY;
+        }
         // Score k in base 2 is sc·f + e with f > 0 and e the same for 16 keys
         // (a page's K scale and V exponent; bf16: the softmax scale and 0), so
-        // the maximum is taken of the raw scores, 16 at a time.  The scores
-        // are read from TMEM twice, 64 at a time, which keeps the kernel's
-        // warps within their registers.
-        auto factor = [&](int at) { return fmaxf(rowf * sks[at], 1.17549435e-38f); };  // never 0: -inf · 0 is NaN
-        float mt = -INFINITY;
+        // the maximum is taken of the raw scores, 16 at a time.
+        const int at0 = (pos & 3) * 8 + 4 * hf;
+        auto factor = [&](int g) { return fmaxf(rowf * sks[at0 + g], 1.17549435e-38f); };  // never 0: -inf · 0 is NaN
+        float mt = -INFINITY, other;
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          float sc[64];
-          scores(hf, sc);
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            float x = max3(sc[16 * g], sc[16 * g + 1], sc[16 * g + 2]), y = max3(sc[16 * g + 3], sc[16 * g + 4], sc[16 * g + 5]);
-            x = max3(x, sc[16 * g + 6], sc[16 * g + 7]);
-            y = max3(y, sc[16 * g + 8], sc[16 * g + 9]);
-            x = max3(x, sc[16 * g + 10], sc[16 * g + 11]);
-            y = max3(y, sc[16 * g + 12], sc[16 * g + 13]);
-            x = max3(x, sc[16 * g + 14], sc[16 * g + 15]);
-            if constexpr (E4) {
-              const int at = (pos & 1) * 8 + 4 * hf + g;
-              mt = fmaxf(mt, fmaf(fmaxf(x, y), factor(at), (float)sve[at]));
-            } else {
-              mt = max3(mt, x, y);
-            }
+        for (int g = 0; g < 4; ++g) {
+          float v = max3(sc[16 * g], sc[16 * g + 1], sc[16 * g + 2]), y = max3(sc[16 * g + 3], sc[16 * g + 4], sc[16 * g + 5]);
+          v = max3(v, sc[16 * g + 6], sc[16 * g + 7]);
+          y = max3(y, sc[16 * g + 8], sc[16 * g + 9]);
+          v = max3(v, sc[16 * g + 10], sc[16 * g + 11]);
+          y = max3(y, sc[16 * g + 12], sc[16 * g + 13]);
+          v = max3(v, sc[16 * g + 14], sc[16 * g + 15]);
+          if constexpr (E4) {
+            mt = fmaxf(mt, fmaf(fmaxf(v, y), factor(g), (float)sve[at0 + g]));
+          } else {
+            mt = max3(mt, v, y);
           }
         }
         if constexpr (!E4) mt *= scale2;
+        if (!exchange(mt, other)) {
+          ok = false;
+          break;
+        }
+        mt = fmaxf(mt, other);
         float m_new = m;
         bool moved = false;
         if (m == -INFINITY) {
@@ -459,56 +540,52 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
         m = m_new;
         float add = 0.f;
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          float sc[64];
-          scores(hf, sc);
+        for (int g = 0; g < 4; ++g) {
+          const float f = E4 ? factor(g) : scale2, e = E4 ? (float)sve[at0 + g] - mb : -mb;
+          const uint64_t ff = pair_of(f, f), ee = pair_of(e, e);
+          uint64_t sum = 0;  // two zeros
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const int at = (pos & 1) * 8 + 4 * hf + g;
-            const float f = E4 ? factor(at) : scale2, e = E4 ? (float)sve[at] - mb : -mb;
-            const uint64_t ff = pair_of(f, f), ee = pair_of(e, e);
-            uint64_t sum = 0;  // two zeros
-#pragma unroll
-            for (int i = 16 * g; i < 16 * g + 16; i += 2) {
-              float y0, y1;
-              split_pair(fma_pair(pair_of(sc[i], sc[i + 1]), ff, ee), y0, y1);
-              y0 = ex2(y0);
-              y1 = ex2(y1);
-              sum = add_pair(sum, pair_of(y0, y1));
-              sc[i / 2] = __uint_as_float(E4 ? pack_f16(y0, y1) : bf16_pair(y0, y1));
-            }
-            float s0, s1;
-            split_pair(sum, s0, s1);
-            add = E4 ? fmaf(s0 + s1, pow2i(-7 - sve[at]), add) : add + (s0 + s1);
+          for (int k = 16 * g; k < 16 * g + 16; k += 2) {
+            float y0, y1;
+            split_pair(fma_pair(pair_of(sc[k], sc[k + 1]), ff, ee), y0, y1);
+            y0 = ex2(y0);
+            y1 = ex2(y1);
+            sum = add_pair(sum, pair_of(y0, y1));
+            sc[k / 2] = __uint_as_float(E4 ? pack_f16(y0, y1) : bf16_pair(y0, y1));
           }
-          tmem_st32(tS + 32 * hf, sc);  // P over scores that have been read for good
+          float s0, s1;
+          split_pair(sum, s0, s1);
+          add = E4 ? fmaf(s0 + s1, pow2i(-7 - sve[at0 + g]), add) : add + (s0 + s1);
         }
+        // P over the scores, two keys per column: both threads of the row have
+        // read theirs (the exchange).
+        tmem_st32(tS + 32 * hf, sc);
         l = l * alpha + add;
         // The previous value product of this tile has finished (the score
         // product just read was issued after it).
         if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll 1
-          for (int c4 = 0; c4 < D / 32; ++c4) {
+          for (int c4 = 0; c4 < D / 64; ++c4) {
+            const uint32_t tO = tmem + lanes + kColOE + D * x + (D / 2) * hf + c4 * 32;
             float o[32];
-            tmem_ld32(tmem + lanes + kColOE + D * x + c4 * 32, o);
+            tmem_ld32(tO, o);
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] *= alpha;
-            tmem_st32(tmem + lanes + kColOE + D * x + c4 * 32, o);
+            tmem_st32(tO, o);
           }
         }
         // bf16: value rows behind the sequence were not loaded (P is 0 there,
-        // but 0 · NaN is not): cleared before the value products.
+        // but 0 · NaN is not): cleared before the value products.  (A wait that
+        // runs out is voted on at the next exchange.)
         if constexpr (!E4) {
           if (k0 + kChunkE > len && k0 + r >= len) {
-            if (!mbar_wait(&kvfull[pos & 1], (int)(pos >> 1) & 1, a.err)) ok = false;
-            uint8_t* v = skv + (pos & 1) * 2 * L::kKV + L::kKV;
+            if (!mbar_wait(&vfull[pos & 1], (int)(pos >> 1) & 1, a.err)) *abort_flag = 1;
+            uint8_t* v = sv + (pos & 1) * L::kV;
 #pragma unroll
-            for (int p = 0; p < D / 8; ++p)
-              *reinterpret_cast<uint4*>(v + (p >> 3) * kBoxE + r * 128 + (p & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-          }
-          if (!__all_sync(0xffffffffu, ok)) {
-            ok = false;
-            break;
+            for (int p = 0; p < D / 16; ++p) {
+              const int k = hf * (D / 16) + p;
+              *reinterpret_cast<uint4*>(v + (k >> 3) * kBoxE + r * 128 + (k & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
@@ -518,12 +595,15 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
       }
       if (!ok) break;
       if (nchx > 0) {
-        if (!warp_waits(&odone[x], (int)((cnt - 1) & 1), a.err)) {
-          ok = false;
-          break;
-        }
+        ok = warp_waits(&odone[x], (int)((cnt - 1) & 1), a.err);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       }
+      float other;
+      if (!exchange(l, other)) {
+        ok = false;
+        break;
+      }
+      l = hf == 0 ? l + other : other + l;
       {
         const float unit = E4 ? 1.f / 128.f : 1.f;
         const float f = !w.whole ? unit : l == 0.f ? 0.f : unit / l;
@@ -531,10 +611,11 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
         float* part = (float*)a.ws + (size_t)(2 * c + (w.lo > 0 ? 0 : 1)) * partial_floats<D>();
         const int row = x * kTile + r;
 #pragma unroll
-        for (int c4 = 0; c4 < D / 32; ++c4) {
+        for (int c4 = 0; c4 < D / 64; ++c4) {
+          const int d0 = (D / 2) * hf + c4 * 32;
           float o[32];
           if (nchx > 0) {
-            tmem_ld32(tmem + lanes + kColOE + D * x + c4 * 32, o);
+            tmem_ld32(tmem + lanes + kColOE + D * x + d0, o);
           } else {
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = 0.f;
@@ -544,17 +625,17 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
           if (!w.whole) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-              *reinterpret_cast<float4*>(part + (size_t)row * D + 32 * c4 + 4 * e) =
+              *reinterpret_cast<float4*>(part + (size_t)row * D + d0 + 4 * e) =
                   make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
           } else if (valid) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              *reinterpret_cast<uint4*>(out + 32 * c4 + 8 * e) =
+              *reinterpret_cast<uint4*>(out + d0 + 8 * e) =
                   make_uint4(bf16_pair(o[8 * e], o[8 * e + 1]), bf16_pair(o[8 * e + 2], o[8 * e + 3]),
                              bf16_pair(o[8 * e + 4], o[8 * e + 5]), bf16_pair(o[8 * e + 6], o[8 * e + 7]));
           }
         }
-        if (!w.whole) {
+        if (!w.whole && hf == 0) {
           part[2 * kTile * D + row] = m;
           part[2 * kTile * D + 2 * kTile + row] = l;
         }
@@ -565,101 +646,50 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
     if (!ok) *abort_flag = 1;
   } else if (E4 && warp < R::kProducer) {
     // Converters: a thread takes 16 codes (piece pc of a row) of rows rr +
-    // RPI·i.  Eight lanes hold four pieces of two rows, so that their halves
-    // go to eight different groups of banks.
-    constexpr int PPR = D / 16, RPI = 128 / PPR, NI = kChunkE / RPI;
-    const int dt = threadIdx.x - R::kSoft * 32, cw = dt >> 5;
+    // RPI·i of a chunk's values.  Eight lanes hold four pieces of two rows, so
+    // that their halves go to eight different groups of banks.
+    constexpr int PPR = D / 16, RPI = 32 * (E4 ? R::kConv : 2) / PPR, NI = kChunkE / RPI;
+    const int cw = warp - R::kSoft;
     const int pc = D == 128 ? (lane & 3) + 4 * ((lane >> 3) & 1) : lane & 3;
     const int rr = D == 128 ? cw * 4 + ((lane >> 2) & 1) + 2 * (lane >> 4) : cw * 8 + (lane >> 2);
-    const int page_shift = 31 - __clz(pool.ps), page_mask = pool.ps - 1;
+    // 16 codes are 32 bytes of halves: two pieces of the row's 64-dim block.
+    const uint32_t from = L::Row::at(rr, pc);
+    const uint32_t to0 = (pc >> 2) * kBoxE + rr * 128 + ((((pc & 3) * 2) ^ (rr & 7)) << 4), to1 = to0 ^ 16;
     int n = 0;
     bool ok = true;
-    uint4 kx[NI], vx[NI];
-    float ks = 1.f, vs = 1.f;
-    int page = -1;  // lanes 0-7: the page of 16 keys of the chunk after the one in registers
-    // Looks up the pages of a chunk, a chunk before load() needs them.
-    auto look_up = [&](const Walk& w, int chunk) {
-      const int j = chunk * kChunkE + (lane & 7) * 16;
-      page = j < w.p.s.past + w.p.s.n ? __ldg(bt.table + (int64_t)w.at.b * bt.ld + (j >> page_shift)) : -1;
-    };
-    // Codes of chunk `chunk` of the walk's sequence and head (zeros behind its end).
-    auto load = [&](const Walk& w, int chunk) {
-      const int len = w.p.s.past + w.p.s.n, k0 = chunk * kChunkE;
-      if ((unsigned)page >= (unsigned)pool.pages) {
-        if (k0 + (lane & 7) * 16 < len) flag_error(a.err, kErrPaged);
-        page = -1;
-      }
-      const uint8_t* kb = (const uint8_t*)pool.k + w.at.h * pool.kh + pc * 16;
-      const uint8_t* vb = (const uint8_t*)pool.v + w.at.h * pool.vh + pc * 16;
-#pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int r = rr + RPI * i, pg = __shfl_sync(0xffffffffu, page, r >> 4);
-        const int o = (k0 + r) & page_mask;
-        kx[i] = vx[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (pg >= 0 && k0 + r < len) {
-          kx[i] = *reinterpret_cast<const uint4*>(kb + pg * pool.kp + o * pool.kt);
-          vx[i] = *reinterpret_cast<const uint4*>(vb + pg * pool.vp + o * pool.vt);
-        }
-      }
-      ks = vs = 1.f;
-      if (dt < 8 && page >= 0) {
-        ks = pool.ks[page * pool.kse + w.at.h];
-        vs = pool.vs[page * pool.vse + w.at.h];
-      }
-    };
-    // 16 codes are 32 bytes of halves: two pieces of the row's 64-dim block.
-    const uint32_t at0 = (pc >> 2) * kBoxE + rr * 128 + ((((pc & 3) * 2) ^ (rr & 7)) << 4), at1 = at0 ^ 16;
-    auto put = [&](uint8_t* tile, int i, const uint4& v) {
-      const uint32_t cw4[4] = {v.x, v.y, v.z, v.w};
-      uint32_t f[8];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        f[2 * k] = e4m3x2_to_f16x2(cw4[k]);
-        f[2 * k + 1] = e4m3x2_hi_to_f16x2(cw4[k]);
-      }
-      *reinterpret_cast<uint4*>(tile + at0 + i * RPI * 128) = make_uint4(f[0], f[1], f[2], f[3]);
-      *reinterpret_cast<uint4*>(tile + at1 + i * RPI * 128) = make_uint4(f[4], f[5], f[6], f[7]);
-    };
-    Walk w(a, pre, u0, u1);
-    while (!w.done() && w.nch == 0) w.next();
-    if (!w.done()) {
-      look_up(w, w.lo);
-      load(w, w.lo);
-      look_up(w, w.lo + 1);
-    }
-    while (!w.done() && ok) {
+    for (Walk w(a, pre, u0, u1); !w.done() && ok; w.next()) {
+      const int len = w.p.s.past + w.p.s.n;
       for (int ch = 0; ch < w.nch; ++ch, ++n) {
-        const int s = n & 1;
-        if (n >= 2 && !warp_waits(&kvempty[s], (int)((n >> 1) - 1) & 1, a.err)) ok = false;
+        const int s = n & 1, left = len - (w.lo + ch) * kChunkE;  // keys from this chunk on
+        ok = warp_waits(&rfull[s], (int)(n >> 1) & 1, a.err);
+        if (ok && n >= 2) ok = warp_waits(&vempty[s], (int)((n >> 1) - 1) & 1, a.err);
         if (*abort_flag) ok = false;
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
           break;
         }
-        uint8_t* st = skv + s * 2 * L::kKV;
+        const uint8_t* src = sraw + s * L::kCodes + from;
+        uint8_t* dst = sv + s * L::kV;
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-          put(st, i, kx[i]);
-          put(st + L::kKV, i, vx[i]);
-        }
-        if (dt < 8) {  // the chunk's scales, as load() left them
-          sks[s * 8 + dt] = ks;
-          sve[s * 8 + dt] = scale_exp(vs);
+          uint4 v = *reinterpret_cast<const uint4*>(src + i * RPI * D);  // RPI is a multiple of 8: the swizzle is the same
+          if (rr + RPI * i >= left) v = make_uint4(0u, 0u, 0u, 0u);
+          const uint32_t c4[4] = {v.x, v.y, v.z, v.w};
+          uint32_t f[8];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            f[2 * k] = e4m3x2_to_f16x2(c4[k]);
+            f[2 * k + 1] = e4m3x2_hi_to_f16x2(c4[k]);
+          }
+          *reinterpret_cast<uint4*>(dst + to0 + i * RPI * 128) = make_uint4(f[0], f[1], f[2], f[3]);
+          *reinterpret_cast<uint4*>(dst + to1 + i * RPI * 128) = make_uint4(f[4], f[5], f[6], f[7]);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (lane == 0) mbar_arrive(&kvfull[s]);
-        if (ch + 1 < w.nch) {
-          load(w, w.lo + ch + 1);
-          look_up(w, w.lo + ch + 2);
+        if (lane == 0) {
+          mbar_arrive(&rempty[s]);
+          mbar_arrive(&vfull[s]);
         }
-      }
-      if (!ok) break;
-      do w.next(); while (!w.done() && w.nch == 0);
-      if (!w.done()) {
-        look_up(w, w.lo);
-        load(w, w.lo);
-        look_up(w, w.lo + 1);
       }
     }
     if (!ok) *abort_flag = 1;
@@ -684,7 +714,7 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
         ok = __shfl_sync(0xffffffffu, (int)ok, 0);
         if (ok) ++qn[x];
       }
-      if constexpr (!E4) {
+      {
         const int len = w.p.s.past + w.p.s.n;
         for (int c0 = 0; c0 < w.nch && ok; c0 += 4) {
           // Lane (j, i): page i of chunk c0 + j.
@@ -699,36 +729,50 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
               page = -1;  // outside the pool: the box is filled with zeros
             }
           }
+          float ks = 1.f, vs = 1.f;
+          if (E4 && page >= 0) {
+            ks = pool.ks[page * pool.kse + w.at.h];
+            vs = pool.vs[page * pool.vse + w.at.h];
+          }
           const int nsl = (keys + kSlice - 1) / kSlice;
           for (int j = 0; j < 4 && c0 + j < w.nch; ++j, ++n) {
             const int s = n & 1;
-            if (n >= 2 && lane == 0) ok = mbar_wait(&kvempty[s], (int)((n >> 1) - 1) & 1, a.err);
-            ok = __shfl_sync(0xffffffffu, (int)(ok && !*abort_flag), 0);
-            if (!ok) break;
             const bool mine = (lane >> 3) == j && keys > 0;
-            uint32_t bytes = mine ? 2u * nsl * kSlice * D * 2 : 0u;
+            uint32_t bytes = mine ? (uint32_t)nsl * kSlice * L::Row::kRowBytes : 0u;
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) bytes += __shfl_xor_sync(0xffffffffu, bytes, o);
-            if (lane == 0) mbar_expect_tx(&kvfull[s], bytes);
-            __syncwarp();
-            if (mine) {
-              uint8_t* kd = skv + s * 2 * L::kKV + i * pool.ps * 128;
-              if (nsl * kSlice >= pool.ps) {
-                for (int db = 0; db < L::kDB; ++db) {
-                  tma_load_4d(kd + db * kBoxE, &maps.k, &kvfull[s], db * 64, 0, w.at.h, page);
-                  tma_load_4d(kd + L::kKV + db * kBoxE, &maps.v, &kvfull[s], db * 64, 0, w.at.h, page);
-                }
-              } else {
-                for (int q = 0; q < nsl; ++q)
-                  for (int db = 0; db < L::kDB; ++db) {
-                    tma_load_4d(kd + q * kSlice * 128 + db * kBoxE, &maps.k_tail, &kvfull[s], db * 64, q * kSlice,
-                                w.at.h, page);
-                    tma_load_4d(kd + q * kSlice * 128 + L::kKV + db * kBoxE, &maps.v_tail, &kvfull[s], db * 64,
-                                q * kSlice, w.at.h, page);
-                  }
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv) {  // the chunk's keys, then its values (e4m3: their codes)
+              uint64_t* full = kv == 0 ? &kfull[s] : E4 ? &rfull[s] : &vfull[s];
+              uint64_t* empty = kv == 0 ? &kempty[s] : E4 ? &rempty[s] : &vempty[s];
+              if (n >= 2 && lane == 0) ok = mbar_wait(empty, (int)((n >> 1) - 1) & 1, a.err);
+              ok = __shfl_sync(0xffffffffu, (int)(ok && !*abort_flag), 0);
+              if (!ok) break;
+              if (lane == 0) mbar_expect_tx(full, bytes);
+              __syncwarp();
+              if (mine) {
+                uint8_t* st = kv == 0 ? sk + s * L::kK : E4 ? sraw + s * L::kCodes : sv + s * L::kV;
+                st += i * pool.ps * L::Row::kBytes;
+                const CUtensorMap* tm = nsl * kSlice >= pool.ps ? (kv ? &maps.v : &maps.k) : (kv ? &maps.v_tail : &maps.k_tail);
+                const int boxes = nsl * kSlice >= pool.ps ? 1 : nsl;  // the whole page, or its slices that hold keys
+                for (int q = 0; q < boxes; ++q)
+#pragma unroll
+                  for (int db = 0; db < L::Row::kBlocks; ++db)
+                    tma_load_4d(st + q * kSlice * L::Row::kBytes + db * kBoxE, tm, full, db * 64, q * kSlice, w.at.h, page);
               }
+              issued += kv == 0 ? 1 : 0;
+              issued_v += kv;
             }
-            issued = n + 1;
+            if (!ok) break;
+            if constexpr (E4) {  // 16 keys at a time; groups behind the sequence keep what they had
+              if (mine)
+                for (int q = 0; q < pool.ps / 16; ++q) {
+                  sks[(n & 3) * 8 + i * (pool.ps / 16) + q] = ks;
+                  sve[(n & 3) * 8 + i * (pool.ps / 16) + q] = scale_exp(vs);
+                }
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&sready[n & 3]);
+            }
           }
         }
       }
@@ -737,32 +781,41 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
     }
     if (!ok) *abort_flag = 1;
   } else if (warp == R::kMma) {
-    // bf16 x bf16, or half x half for e4m3 pages.
-    constexpr uint32_t kTypes = E4 ? 0u : (1u << 7) | (1u << 10);
-    constexpr uint32_t idS = (instr_desc(kChunkE) & ~((1u << 7) | (1u << 10))) | kTypes;
-    constexpr uint32_t idPV = ((instr_desc(D) & ~((1u << 7) | (1u << 10))) | kTypes) | (1u << 16);  // B MN-major
-    int n = 0, kv_seen = 0;
+    // Scores: bf16, or codes; values: bf16, or halves (MN-major).
+    constexpr uint32_t kTypes = (1u << 7) | (1u << 10);
+    constexpr uint32_t idS = E4 ? instr_desc(kChunkE) & ~kTypes : instr_desc(kChunkE);
+    constexpr uint32_t idPV = (E4 ? instr_desc(D) & ~kTypes : instr_desc(D)) | (1u << 16);
+    int n = 0, k_seen = 0, v_seen = 0;  // ring positions whose keys, values this thread has waited for
     int cnt[2] = {0, 0}, qm[2] = {0, 0};
     bool ok = true;
-    auto wait_kv = [&](int upto) -> bool {
-      for (; kv_seen < upto; ++kv_seen)
-        if (!mbar_wait(&kvfull[kv_seen & 1], (int)(kv_seen >> 1) & 1, a.err)) return false;
+    auto wait_ring = [&](uint64_t* full, int& seen, int upto) -> bool {
+      for (; seen < upto; ++seen)
+        if (!mbar_wait(&full[seen & 1], (int)(seen >> 1) & 1, a.err)) return false;
       return true;
     };
     auto score = [&](int x, int pos) {
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint8_t* k = skv + (pos & 1) * 2 * L::kKV;
+      const uint8_t* k = sk + (pos & 1) * L::kK;
       const uint8_t* q = sq + x * L::kQ;
+      if constexpr (E4) {
 #pragma unroll
-      for (int kd = 0; kd < D / 16; ++kd)
-        mma_bf16(tmem + kColSE + 128 * x, smem_desc(q + (kd >> 2) * kBoxE) + (uint64_t)((kd & 3) * 2),
-                 smem_desc(k + (kd >> 2) * kBoxE) + (uint64_t)((kd & 3) * 2), idS, kd > 0 ? 1u : 0u);
+        for (int half = 0; half < 2; ++half)  // Q's codes, then its remainders'
+#pragma unroll
+          for (int kd = 0; kd < D / 32; ++kd)
+            mma_codes(tmem + kColSE + 128 * x, desc_codes<D>(q + half * L::kCodes) + (uint64_t)(2 * kd),
+                      desc_codes<D>(k) + (uint64_t)(2 * kd), idS, half + kd > 0 ? 1u : 0u);
+      } else {
+#pragma unroll
+        for (int kd = 0; kd < D / 16; ++kd)
+          mma_bf16(tmem + kColSE + 128 * x, smem_desc(q + (kd >> 2) * kBoxE) + (uint64_t)((kd & 3) * 2),
+                   smem_desc(k + (kd >> 2) * kBoxE) + (uint64_t)((kd & 3) * 2), idS, kd > 0 ? 1u : 0u);
+      }
       mma_commit(&sfull[x]);
     };
     auto value = [&](int x, int pos, bool first) -> bool {
       if (!mbar_wait(&pready[x], (int)(cnt[x] & 1), a.err)) return false;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint8_t* v = skv + (pos & 1) * 2 * L::kKV + L::kKV;
+      const uint8_t* v = sv + (pos & 1) * L::kV;
 #pragma unroll
       for (int kk = 0; kk < kChunkE / 16; ++kk)
         mma_ta(tmem + kColOE + D * x, tmem + kColSE + 128 * x + kk * 8, desc_mn(v + kk * 16 * 128, kBoxE), idPV,
@@ -775,7 +828,10 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
     };
     for (Walk w(a, pre, u0, u1); !w.done() && ok; w.next()) {
       if (lane == 0) {
-        if (w.nch > 0) ok = wait_kv(n + 1);
+        // The last tile that sees chunk ch frees its keys (after its score
+        // product) and values (after its value product).
+        auto last_of = [&](int x, int ch) { return x == (ch < w.cb ? 1 : 0); };
+        if (w.nch > 0) ok = wait_ring(kfull, k_seen, n + 1);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           if (w.c(x) == 0 || !ok) continue;
@@ -784,10 +840,15 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
             continue;
           }
           score(x, n);
+          if (last_of(x, 0)) mma_commit(&kempty[n & 1]);
           if (w.c(x) == 1) mma_commit(&qempty[x]);  // the tile's last score product
           ++qm[x];
         }
         for (int ch = 0; ch < w.nch && ok; ++ch) {
+          if (!wait_ring(vfull, v_seen, n + ch + 1)) {
+            ok = false;
+            break;
+          }
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             if (ch >= w.c(x) || !ok) continue;
@@ -795,16 +856,17 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
               ok = false;
               continue;
             }
+            if (last_of(x, ch)) mma_commit(&vempty[(n + ch) & 1]);
             if (ch + 1 < w.c(x)) {
-              if (!wait_kv(n + ch + 2)) {
+              if (!wait_ring(kfull, k_seen, n + ch + 2)) {
                 ok = false;
                 continue;
               }
               score(x, n + ch + 1);
+              if (last_of(x, ch + 1)) mma_commit(&kempty[(n + ch + 1) & 1]);
               if (ch + 2 == w.c(x)) mma_commit(&qempty[x]);
             }
           }
-          mma_commit(&kvempty[(n + ch) & 1]);  // every product reading this chunk is issued
         }
         n += w.nch;
         if (*abort_flag) ok = false;
@@ -820,7 +882,8 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
   __syncthreads();
   if (warp == R::kProducer && lane == 0 && *abort_flag) {
     // Let the loads this CTA issued land before its shared memory goes away.
-    for (int i = issued > 2 ? issued - 2 : 0; i < issued; ++i) mbar_wait(&kvfull[i & 1], (int)(i >> 1) & 1, a.err);
+    for (int i = issued > 2 ? issued - 2 : 0; i < issued; ++i) mbar_wait(&kfull[i & 1], (int)(i >> 1) & 1, a.err);
+    for (int i = issued_v > 2 ? issued_v - 2 : 0; i < issued_v; ++i) mbar_wait(E4 ? &rfull[i & 1] : &vfull[i & 1], (int)(i >> 1) & 1, a.err);
     for (int x = 0; x < 2; ++x)
       if (qn[x] > 0) mbar_wait(&qfull[x], (qn[x] - 1) & 1, a.err);
   }
@@ -902,7 +965,7 @@ int extend_grid() { return usable_sms(); }
 template <int D, bool E4>
 cudaError_t launch_extend(const PagedAttnArgs& a, cudaStream_t s) {
   PoolMaps maps{};
-  if (!E4 && !pool_maps<D, false>(&maps, a.pool)) return cudaErrorInvalidValue;
+  if (!pool_maps<D, E4>(&maps, a.pool)) return cudaErrorInvalidValue;
   const int G = a.nq / a.pool.nkv, tq = kTile / G;
   CUtensorMap tq_map;
   {
@@ -926,7 +989,7 @@ cudaError_t launch_extend(const PagedAttnArgs& a, cudaStream_t s) {
     configured[dev] = true;
   }
   const int grid = extend_grid();
-  cudaError_t e = launch_pdl(kernel, dim3(grid), dim3(Roles<E4>::kThreads), ExtendLayout<D>::bytes(a.batch.B), s, maps,
+  cudaError_t e = launch_pdl(kernel, dim3(grid), dim3(Roles<E4>::kThreads), ExtendLayout<D, E4>::bytes(a.batch.B), s, maps,
                              tq_map, a);
   if (e != cudaSuccess || grid == 1) return e;
   return launch_pdl(paged_extend_join_kernel<D>, dim3(grid - 1, 2 * kTile / 32), dim3(256),

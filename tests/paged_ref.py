@@ -53,32 +53,40 @@ def dense(pages, scale, table_row, length):
 
 
 def attend(q, k, v, past, scale):
-    """One sequence: q [n, nq, D], k / v [nkv, L, D] (64 bits) -> out, and per output the sum of p|v| and the largest
-    sum of |q||k| of its visible keys."""
+    """One sequence: q [n, nq, D], k / v [nkv, L, D] (64 bits) -> out, and per output the sum of p|v| and, over its
+    visible keys, the largest scale·Σ|q||k| and the largest scale·max|q|·Σ|k|."""
     n, nq, D = q.shape
     nkv, L = k.shape[0], k.shape[1]
     kk, vv = k.repeat_interleave(nq // nkv, 0), v.repeat_interleave(nq // nkv, 0)
     s = torch.einsum("nhd,hld->hnl", q, kk) * scale
     mag = torch.einsum("nhd,hld->hnl", q.abs(), kk.abs()) * scale
+    most = q.abs().amax(-1).transpose(0, 1)[..., None] * kk.abs().sum(-1)[:, None] * scale  # [nq, n, L]
     seen = torch.arange(L)[None] <= past + torch.arange(n)[:, None]
     s = s.masked_fill(~seen, -math.inf)
     mag = mag.masked_fill(~seen, 0.0)
+    most = most.masked_fill(~seen, 0.0)
     p = torch.exp(s - s.amax(-1, keepdim=True).clamp(min=-1e300)) if L else s
     p = p / p.sum(-1, keepdim=True).clamp(min=1e-300)
     vs = torch.where(torch.arange(L)[None, :, None] < past + n, vv, 0.0) if L else vv
     out = torch.einsum("hnl,hld->nhd", p, vs)
     weight = torch.einsum("hnl,hld->nhd", p, vs.abs())
-    top = (mag.amax(-1) if L else torch.zeros(nq, n, dtype=torch.float64)).transpose(0, 1)
+    top = torch.stack([(m.amax(-1) if L else torch.zeros(nq, n, dtype=torch.float64)).transpose(0, 1) for m in (mag, most)])
     return out, weight, top
 
 
-def attention_tolerance(out, weight, top, D, L, dtype, p_step):
+def attention_tolerance(out, weight, top, D, L, dtype, p_step, codes=False):
     """|error| of an attention row computed from fp32 scores, with P rounded to `p_step` relative (0: kept in fp32).
 
     A score is D products added in fp32, scaled: off by at most (D + 4)·2^-24·Σ|q||k|·scale, and its exponential by as
     much relatively plus 4 steps of the exponential itself; numerator and denominator each carry that, the sums over L
-    keys add L + 8 roundings (of positive terms: relative), and the result is rounded to its type."""
-    rel = 2 * ((D + 4) * F32 * top + 4 * F32) + 2 * (L + 8) * F32
+    keys add L + 8 roundings (of positive terms: relative), and the result is rounded to its type.
+
+    `codes`: bf16 queries over e4m3 pages, whose elements may be taken as the sum of two e4m3 numbers of a row scaled
+    to [128, 256) by a power of two.  The first is off by at most half a step, 2^-5 of a power of two 2^p <= |q|; the
+    remainder is a multiple of q's last bit, 2^(p - 7), and at most 2^(p - 4): four bits, exact unless that last bit
+    lies below e4m3's least step 2^-9, where it is off by at most 2^-10, that is 2^-17 of the row's largest (>= 128).
+    Its products with the key add up to at most 2^-17·max|q|·Σ|k|·scale."""
+    rel = 2 * ((D + 4) * F32 * top[0] + 4 * F32 + (2.0**-17 * top[1] if codes else 0.0)) + 2 * (L + 8) * F32
     return HALF[dtype] * out.abs() + (rel[..., None] + p_step) * 1.01 * weight + 1e-30
 
 
