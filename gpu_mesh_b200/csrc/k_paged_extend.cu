@@ -251,21 +251,38 @@ __device__ __forceinline__ uint64_t desc_mn(const void* p, uint32_t lbo) {
   return ((addr & 0x3FFFFull) >> 4) | ((uint64_t)(lbo >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
 
-__device__ __forceinline__ void mma_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// The issuing warp runs converged, its operands the same in every lane, and
+// one lane (`one`) issues: the operands then stay in uniform registers.  Inside
+// a branch of one lane each product cost about 90 cycles to issue.
+__device__ __forceinline__ void mma_16bit(bool one, uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(b), "r"(idesc), "r"(acc));
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"((uint32_t)one));
 }
-
-// D (fp32) += A·Bᵀ, both e4m3 codes in shared memory, K = 32.
-__device__ __forceinline__ void mma_codes(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ta(bool one, uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc));
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(b), "r"(idesc), "r"(acc), "r"((uint32_t)one));
+}
+// D (fp32) += A·Bᵀ, both e4m3 codes in shared memory, K = 32.
+__device__ __forceinline__ void mma_codes(bool one, uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"((uint32_t)one));
+}
+__device__ __forceinline__ void commit(bool one, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+      "r"((uint32_t)one)
+      : "memory");
 }
 
 // Shared-memory descriptor of a K-major tile of codes: rows of 128 bytes
@@ -750,15 +767,22 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
               if (!ok) break;
               if (lane == 0) mbar_expect_tx(full, bytes);
               __syncwarp();
-              if (mine) {
-                uint8_t* st = kv == 0 ? sk + s * L::kK : E4 ? sraw + s * L::kCodes : sv + s * L::kV;
-                st += i * pool.ps * L::Row::kBytes;
-                const CUtensorMap* tm = nsl * kSlice >= pool.ps ? (kv ? &maps.v : &maps.k) : (kv ? &maps.v_tail : &maps.k_tail);
-                const int boxes = nsl * kSlice >= pool.ps ? 1 : nsl;  // the whole page, or its slices that hold keys
-                for (int q = 0; q < boxes; ++q)
+              uint8_t* st = kv == 0 ? sk + s * L::kK : E4 ? sraw + s * L::kCodes : sv + s * L::kV;
+              for (int pi = 0; pi < ppc; ++pi, st += pool.ps * L::Row::kBytes) {  // the same in every lane, one issues
+                const int slices = __shfl_sync(0xffffffffu, nsl, j * 8 + pi), pg = __shfl_sync(0xffffffffu, page, j * 8 + pi);
+                if (slices == 0) break;
+                if (slices * kSlice >= pool.ps) {
 #pragma unroll
                   for (int db = 0; db < L::Row::kBlocks; ++db)
-                    tma_load_4d(st + q * kSlice * L::Row::kBytes + db * kBoxE, tm, full, db * 64, q * kSlice, w.at.h, page);
+                    if (lane == 0) tma_load_4d(st + db * kBoxE, kv ? &maps.v : &maps.k, full, db * 64, 0, w.at.h, pg);
+                } else {  // the sequence's last page: its slices that hold keys
+                  for (int q = 0; q < slices; ++q)
+#pragma unroll
+                    for (int db = 0; db < L::Row::kBlocks; ++db)
+                      if (lane == 0)
+                        tma_load_4d(st + q * kSlice * L::Row::kBytes + db * kBoxE, kv ? &maps.v_tail : &maps.k_tail, full, db * 64,
+                                    q * kSlice, w.at.h, pg);
+                }
               }
               issued += kv == 0 ? 1 : 0;
               issued_v += kv;
@@ -785,98 +809,97 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
     constexpr uint32_t kTypes = (1u << 7) | (1u << 10);
     constexpr uint32_t idS = E4 ? instr_desc(kChunkE) & ~kTypes : instr_desc(kChunkE);
     constexpr uint32_t idPV = (E4 ? instr_desc(D) & ~kTypes : instr_desc(D)) | (1u << 16);
-    int n = 0, k_seen = 0, v_seen = 0;  // ring positions whose keys, values this thread has waited for
+    const bool one = lane == 0;
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    int n = 0, k_seen = 0, v_seen = 0;  // ring positions whose keys, values this warp has waited for
     int cnt[2] = {0, 0}, qm[2] = {0, 0};
     bool ok = true;
     auto wait_ring = [&](uint64_t* full, int& seen, int upto) -> bool {
       for (; seen < upto; ++seen)
-        if (!mbar_wait(&full[seen & 1], (int)(seen >> 1) & 1, a.err)) return false;
+        if (!warp_waits(&full[seen & 1], (int)(seen >> 1) & 1, a.err)) return false;
       return true;
     };
     auto score = [&](int x, int pos) {
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint8_t* k = sk + (pos & 1) * L::kK;
+      const int st = __shfl_sync(0xffffffffu, pos & 1, 0);
+      const uint8_t* k = sk + st * L::kK;
       const uint8_t* q = sq + x * L::kQ;
       if constexpr (E4) {
 #pragma unroll
         for (int half = 0; half < 2; ++half)  // Q's codes, then its remainders'
 #pragma unroll
           for (int kd = 0; kd < D / 32; ++kd)
-            mma_codes(tmem + kColSE + 128 * x, desc_codes<D>(q + half * L::kCodes) + (uint64_t)(2 * kd),
+            mma_codes(one, tm + kColSE + 128 * x, desc_codes<D>(q + half * L::kCodes) + (uint64_t)(2 * kd),
                       desc_codes<D>(k) + (uint64_t)(2 * kd), idS, half + kd > 0 ? 1u : 0u);
       } else {
 #pragma unroll
         for (int kd = 0; kd < D / 16; ++kd)
-          mma_bf16(tmem + kColSE + 128 * x, smem_desc(q + (kd >> 2) * kBoxE) + (uint64_t)((kd & 3) * 2),
-                   smem_desc(k + (kd >> 2) * kBoxE) + (uint64_t)((kd & 3) * 2), idS, kd > 0 ? 1u : 0u);
+          mma_16bit(one, tm + kColSE + 128 * x, smem_desc(q + (kd >> 2) * kBoxE) + (uint64_t)((kd & 3) * 2),
+                    smem_desc(k + (kd >> 2) * kBoxE) + (uint64_t)((kd & 3) * 2), idS, kd > 0 ? 1u : 0u);
       }
-      mma_commit(&sfull[x]);
+      commit(one, &sfull[x]);
     };
     auto value = [&](int x, int pos, bool first) -> bool {
-      if (!mbar_wait(&pready[x], (int)(cnt[x] & 1), a.err)) return false;
+      if (!warp_waits(&pready[x], (int)(cnt[x] & 1), a.err)) return false;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint8_t* v = sv + (pos & 1) * L::kV;
+      const int st = __shfl_sync(0xffffffffu, pos & 1, 0);
+      const uint8_t* v = sv + st * L::kV;
 #pragma unroll
       for (int kk = 0; kk < kChunkE / 16; ++kk)
-        mma_ta(tmem + kColOE + D * x, tmem + kColSE + 128 * x + kk * 8, desc_mn(v + kk * 16 * 128, kBoxE), idPV,
+        mma_ta(one, tm + kColOE + D * x, tm + kColSE + 128 * x + kk * 8, desc_mn(v + kk * 16 * 128, kBoxE), idPV,
                (first && kk == 0) ? 0u : 1u);
-      mma_commit(&odone[x]);
+      commit(one, &odone[x]);
       // The next score product overwrites the columns that P is read from.
-      const bool done = mbar_wait(&odone[x], (int)(cnt[x] & 1), a.err);
+      const bool done = warp_waits(&odone[x], (int)(cnt[x] & 1), a.err);
       ++cnt[x];
       return done;
     };
     for (Walk w(a, pre, u0, u1); !w.done() && ok; w.next()) {
-      if (lane == 0) {
-        // The last tile that sees chunk ch frees its keys (after its score
-        // product) and values (after its value product).
-        auto last_of = [&](int x, int ch) { return x == (ch < w.cb ? 1 : 0); };
-        if (w.nch > 0) ok = wait_ring(kfull, k_seen, n + 1);
+      // The last tile that sees chunk ch frees its keys (after its score
+      // product) and values (after its value product).
+      auto last_of = [&](int x, int ch) { return x == (ch < w.cb ? 1 : 0); };
+      if (w.nch > 0) ok = wait_ring(kfull, k_seen, n + 1);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        if (w.c(x) == 0 || !ok) continue;
+        if (!warp_waits(E4 ? &qconv[x] : &qfull[x], qm[x] & 1, a.err)) {
+          ok = false;
+          continue;
+        }
+        score(x, n);
+        if (last_of(x, 0)) commit(one, &kempty[n & 1]);
+        if (w.c(x) == 1) commit(one, &qempty[x]);  // the tile's last score product
+        ++qm[x];
+      }
+      for (int ch = 0; ch < w.nch && ok; ++ch) {
+        if (!wait_ring(vfull, v_seen, n + ch + 1)) {
+          ok = false;
+          break;
+        }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          if (w.c(x) == 0 || !ok) continue;
-          if (!mbar_wait(E4 ? &qconv[x] : &qfull[x], qm[x] & 1, a.err)) {
+          if (ch >= w.c(x) || !ok) continue;
+          if (!value(x, n + ch, ch == 0) || __any_sync(0xffffffffu, *abort_flag)) {
             ok = false;
             continue;
           }
-          score(x, n);
-          if (last_of(x, 0)) mma_commit(&kempty[n & 1]);
-          if (w.c(x) == 1) mma_commit(&qempty[x]);  // the tile's last score product
-          ++qm[x];
-        }
-        for (int ch = 0; ch < w.nch && ok; ++ch) {
-          if (!wait_ring(vfull, v_seen, n + ch + 1)) {
-            ok = false;
-            break;
-          }
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            if (ch >= w.c(x) || !ok) continue;
-            if (!value(x, n + ch, ch == 0) || *abort_flag) {
+          if (last_of(x, ch)) commit(one, &vempty[(n + ch) & 1]);
+          if (ch + 1 < w.c(x)) {
+            if (!wait_ring(kfull, k_seen, n + ch + 2)) {
               ok = false;
               continue;
             }
-            if (last_of(x, ch)) mma_commit(&vempty[(n + ch) & 1]);
-            if (ch + 1 < w.c(x)) {
-              if (!wait_ring(kfull, k_seen, n + ch + 2)) {
-                ok = false;
-                continue;
-              }
-              score(x, n + ch + 1);
-              if (last_of(x, ch + 1)) mma_commit(&kempty[(n + ch + 1) & 1]);
-              if (ch + 2 == w.c(x)) mma_commit(&qempty[x]);
-            }
+            score(x, n + ch + 1);
+            if (last_of(x, ch + 1)) commit(one, &kempty[(n + ch + 1) & 1]);
+            if (ch + 2 == w.c(x)) commit(one, &qempty[x]);
           }
         }
-        n += w.nch;
-        if (*abort_flag) ok = false;
       }
-      ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+      n += w.nch;
+      if (__any_sync(0xffffffffu, *abort_flag)) ok = false;
     }
-    if (lane == 0) {
-      if (!ok) *abort_flag = 1;
-      mma_commit(drain);  // arrives once every MMA issued above has finished
-    }
+    if (!ok) *abort_flag = 1;
+    commit(one, drain);  // arrives once every MMA issued above has finished
   }
 
   __syncthreads();
@@ -887,7 +910,7 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
     for (int x = 0; x < 2; ++x)
       if (qn[x] > 0) mbar_wait(&qfull[x], (qn[x] - 1) & 1, a.err);
   }
-  if (warp == R::kMma && lane == 0) mbar_wait(drain, 0, a.err);
+  if (warp == R::kMma) mbar_wait(drain, 0, a.err);
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if (warp == R::kProducer) {
