@@ -246,6 +246,13 @@ __host__ __device__ constexpr size_t partial_floats() {
   return (size_t)2 * kTile * (D + 2);
 }
 
+// What a CTA leaves for the join: the item that its run ends and earlier ones
+// began, as its sequence's first token row and new tokens, its KV head and
+// tile pair, and its pieces (0: there is none), this run's the last.
+struct CutItem {
+  int q0, n, h, j, pieces, pad[3];
+};
+
 __device__ __forceinline__ uint64_t desc_mn(const void* p, uint32_t lbo) {
   const uint64_t addr = smem_u32(p);
   return ((addr & 0x3FFFFull) >> 4) | ((uint64_t)(lbo >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
@@ -418,6 +425,8 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
   count_units(a, pre, blockIdx.x == 0);
   const RunsE runs(pre[bt.B], (int)gridDim.x);
   const int c = blockIdx.x;
+  CutItem* cut = (CutItem*)((float*)a.ws + (size_t)2 * gridDim.x * partial_floats<D>()) + c;
+  if (threadIdx.x == 0) cut->pieces = 0;
   if (c >= runs.grid) return;
   if (warp == R::kProducer) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
@@ -715,6 +724,10 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
     bool ok = true;
     const int ppc = kChunkE / pool.ps;
     for (Walk w(a, pre, u0, u1); !w.done() && ok; w.next()) {
+      if (w.lo > 0 && w.hi == w.units && lane == 0) {  // the last piece of a cut item
+        const int start = w.u - w.lo, first = (int)((((long long)start + 1) * runs.grid - 1) / runs.total);
+        *cut = CutItem{w.p.s.q0, w.p.s.n, w.at.h, w.at.j, c - first + 1, {0, 0, 0}};
+      }
       // The tiles' query rows, once the previous piece's score products have read theirs.
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
@@ -918,64 +931,56 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
   }
 }
 
-// Joins the pieces of cut items: block (c, y) takes the item that CTA c's run
-// begins in the middle of, if no earlier run does, and 32 of its 256 rows.
+// Joins the pieces of cut items, in order: block (c, y) 32 of the 256 rows of
+// the item that CTA c's run ends, eight lanes per row.
 template <int D>
-__global__ void __launch_bounds__(256) paged_extend_join_kernel(const __grid_constant__ PagedAttnArgs a, int most) {
-  extern __shared__ int pre_s[];
-  __shared__ Place where;
+__global__ void __launch_bounds__(256) paged_extend_join_kernel(const __grid_constant__ PagedAttnArgs a) {
   pdl_trigger();
-  // Lengths were written before the attention kernel began, which allows this
-  // kernel to start only after its own wait.
-  count_units(a, pre_s, false);
-  const RunsE runs(pre_s[a.batch.B], most);
-  const int c = blockIdx.x + 1;  // a cut lies at the beginning of run 1 or a later one
-  if (c >= runs.grid) return;
-  const int u = runs.begin(c);
-  if (threadIdx.x < 32) {
-    const Place p = place_of(a, pre_s, u);
-    if (threadIdx.x == 0) where = p;
-  }
-  __syncthreads();
-  const Place pl = where;
-  if (pl.chunk == 0) return;               // the item begins here: nothing is cut
-  const int start = u - pl.chunk;          // the item's first unit
-  if (runs.begin(c - 1) > start) return;   // an earlier run begins inside the item too
-  const int G = a.nq / a.pool.nkv;
-  const Pairs p(seq_span(a.batch, pl.b, a.pool.ps), G);
-  const int end = start + p.units(pl.j);
-  int last = c;
-  while (last + 1 < runs.grid && runs.begin(last + 1) < end) ++last;
   pdl_wait();
-  // Eight lanes per row, each D / 8 dims.
+  const int c = blockIdx.x;
+  const CutItem* cut = (const CutItem*)((const float*)a.ws + (size_t)2 * gridDim.x * partial_floats<D>()) + c;
+  const int pieces = __ldcg(&cut->pieces);
+  if (pieces == 0) return;
+  const int4 it = __ldcg(reinterpret_cast<const int4*>(cut));  // q0, n, h, j
+  const int G = a.nq / a.pool.nkv, tq = kTile / G;
   const int row = blockIdx.y * 32 + (threadIdx.x >> 3), d0 = (threadIdx.x & 7) * (D / 8);
-  const int r = row % kTile, s_tok = (2 * pl.j + row / kTile) * p.tq + r / G;
-  if (r / G >= p.tq || s_tok >= p.s.n) return;
-  auto piece = [&](int k) {  // run k's slot: 1 if the item begins in it, 0 if it began earlier
-    return (const float*)a.ws + (size_t)(2 * k + (runs.begin(k) > start ? 0 : 1)) * partial_floats<D>();
+  const int r = row % kTile, s_tok = (2 * it.w + row / kTile) * tq + r / G;
+  if (r / G >= tq || s_tok >= it.y) return;
+  // The item's first run left it in its slot 1, the others in their slots 0.
+  auto piece = [&](int k) {
+    return (const float*)a.ws + (size_t)(2 * (c - pieces + 1 + k) + (k == 0 ? 1 : 0)) * partial_floats<D>();
   };
-  float M = -INFINITY;
-  for (int k = c - 1; k <= last; ++k) M = fmaxf(M, __ldcg(piece(k) + 2 * kTile * D + row));
-  float L = 0.f, o[D / 8];
+  float M = -INFINITY, L = 0.f, o[D / 8];
 #pragma unroll
   for (int e = 0; e < D / 8; ++e) o[e] = 0.f;
-  for (int k = c - 1; k <= last; ++k) {
-    const float* q = piece(k);
-    const float mk = __ldcg(q + 2 * kTile * D + row);
-    if (mk == -INFINITY) continue;
-    const float f = ex2(mk - M);
-    L += f * __ldcg(q + 2 * kTile * D + 2 * kTile + row);
+  for (int k0 = 0; k0 < pieces; k0 += 2) {  // two pieces' loads in flight
+    float m[2], l[2];
+    float4 v[2][D / 32];
 #pragma unroll
-    for (int e = 0; e < D / 32; ++e) {
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(q + (size_t)row * D + d0 + 4 * e));
-      o[4 * e] += f * v.x;
-      o[4 * e + 1] += f * v.y;
-      o[4 * e + 2] += f * v.z;
-      o[4 * e + 3] += f * v.w;
+    for (int k = 0; k < 2; ++k) {
+      const float* q = piece(min(k0 + k, pieces - 1));
+      m[k] = __ldcg(q + 2 * kTile * D + row);
+      l[k] = __ldcg(q + 2 * kTile * D + 2 * kTile + row);
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e) v[k][e] = __ldcg(reinterpret_cast<const float4*>(q + (size_t)row * D + d0 + 4 * e));
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (k0 + k >= pieces || m[k] == -INFINITY) continue;
+      const float top = fmaxf(M, m[k]), keep = M == -INFINITY ? 0.f : ex2(M - top), f = ex2(m[k] - top);
+      M = top;
+      L = L * keep + f * l[k];
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e) {
+        o[4 * e] = o[4 * e] * keep + f * v[k][e].x;
+        o[4 * e + 1] = o[4 * e + 1] * keep + f * v[k][e].y;
+        o[4 * e + 2] = o[4 * e + 2] * keep + f * v[k][e].z;
+        o[4 * e + 3] = o[4 * e + 3] * keep + f * v[k][e].w;
+      }
     }
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
-  bf16* out = (bf16*)a.out + (int64_t)(p.s.q0 + s_tok) * a.ldo + (int64_t)(pl.h * G + r % G) * a.hdo + d0;
+  bf16* out = (bf16*)a.out + (int64_t)(it.x + s_tok) * a.ldo + (int64_t)(it.z * G + r % G) * a.hdo + d0;
 #pragma unroll
   for (int e = 0; e < D / 64; ++e)
     *reinterpret_cast<uint4*>(out + 8 * e) =
@@ -1015,14 +1020,13 @@ cudaError_t launch_extend(const PagedAttnArgs& a, cudaStream_t s) {
   cudaError_t e = launch_pdl(kernel, dim3(grid), dim3(Roles<E4>::kThreads), ExtendLayout<D, E4>::bytes(a.batch.B), s, maps,
                              tq_map, a);
   if (e != cudaSuccess || grid == 1) return e;
-  return launch_pdl(paged_extend_join_kernel<D>, dim3(grid - 1, 2 * kTile / 32), dim3(256),
-                    (a.batch.B + 1) * sizeof(int), s, a, grid);
+  return launch_pdl(paged_extend_join_kernel<D>, dim3(grid, 2 * kTile / 32), dim3(256), 0, s, a);
 }
 
 }  // namespace
 
 size_t paged_extend_workspace(const PagedAttnArgs& a) {
-  return (size_t)2 * extend_grid() * (a.pool.D == 128 ? partial_floats<128>() : partial_floats<64>()) * sizeof(float);
+  return (size_t)extend_grid() * (2 * (a.pool.D == 128 ? partial_floats<128>() : partial_floats<64>()) * sizeof(float) + sizeof(CutItem));
 }
 
 cudaError_t launch_paged_extend(const PagedAttnArgs& a, cudaStream_t s) {
