@@ -57,7 +57,7 @@ struct Cached<uint8_t> {
 };
 
 template <typename T, typename C, int D>
-__global__ void __launch_bounds__(kSimt) paged_attn_simt_kernel(PagedAttnArgs a, int tiles, int splits) {
+__global__ void __launch_bounds__(kSimt) paged_attn_simt_kernel(const __grid_constant__ PagedAttnArgs a, int tiles, int splits) {
   constexpr int RPT = kRows * D / kSimt;          // output rows of a thread
   constexpr int P4 = Cached<C>::N;
   __shared__ float sq[kRows][D + 1];
@@ -101,32 +101,55 @@ __global__ void __launch_bounds__(kSimt) paged_attn_simt_kernel(PagedAttnArgs a,
 #pragma unroll
   for (int i = 0; i < RPT; ++i) acc[i] = 0.f;
 
+  // A round's keys and values, requested a round ahead, its pages two.
+  constexpr int NV = (kKeys * D / P4 + kSimt - 1) / kSimt;  // pieces of a thread
+  const int page_shift = 31 - __clz(pool.ps);
+  int page[NV];
+  float kx[NV][P4], vx[NV][P4];
+  auto look_up = [&](int k0) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int j = k0 + (tid + v * kSimt) / (D / P4);
+      page[v] = j < k_hi && tid + v * kSimt < kKeys * D / P4 ? bt.table[(int64_t)b * bt.ld + (j >> page_shift)] : -1;
+    }
+  };
+  auto request = [&](int k0) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int i = tid + v * kSimt, j = k0 + i / (D / P4), d = i % (D / P4) * P4, o = j & (pool.ps - 1);
+#pragma unroll
+      for (int e = 0; e < P4; ++e) kx[v][e] = vx[v][e] = 0.f;
+      if (j >= k_hi || i >= kKeys * D / P4) continue;
+      if (page[v] < 0 || page[v] >= pool.pages) {
+        flag_error(a.err, kErrPaged);
+        continue;
+      }
+      Cached<C>::load((const C*)pool.k + page[v] * pool.kp + h * pool.kh + o * pool.kt + d, kx[v]);
+      Cached<C>::load((const C*)pool.v + page[v] * pool.vp + h * pool.vh + o * pool.vt + d, vx[v]);
+      if constexpr (sizeof(C) == 1) {
+        const float fk = pool.ks[page[v] * pool.kse + h], fv = pool.vs[page[v] * pool.vse + h];
+#pragma unroll
+        for (int e = 0; e < P4; ++e) kx[v][e] *= fk, vx[v][e] *= fv;
+      }
+    }
+  };
+  look_up(k_lo);
+  request(k_lo);
+  look_up(k_lo + kKeys);
   for (int k0 = k_lo; k0 < k_hi; k0 += kKeys) {
     __syncthreads();
-    for (int i = tid; i < kKeys * D / P4; i += kSimt) {
-      const int r = i / (D / P4), d = i % (D / P4) * P4, j = k0 + r;
-      float kx[P4], vx[P4];
 #pragma unroll
-      for (int e = 0; e < P4; ++e) kx[e] = vx[e] = 0.f;
-      if (j < k_hi) {
-        const int page = bt.table[(int64_t)b * bt.ld + j / pool.ps];
-        if (page >= 0 && page < pool.pages) {
-          const int o = j % pool.ps;
-          Cached<C>::load((const C*)pool.k + page * pool.kp + h * pool.kh + o * pool.kt + d, kx);
-          Cached<C>::load((const C*)pool.v + page * pool.vp + h * pool.vh + o * pool.vt + d, vx);
-          if constexpr (sizeof(C) == 1) {
-            const float fk = pool.ks[page * pool.kse + h], fv = pool.vs[page * pool.vse + h];
+    for (int v = 0; v < NV; ++v) {
+      const int i = tid + v * kSimt, r = i / (D / P4), d = i % (D / P4) * P4;
+      if (i >= kKeys * D / P4) continue;
 #pragma unroll
-            for (int e = 0; e < P4; ++e) kx[e] *= fk, vx[e] *= fv;
-          }
-        } else {
-          flag_error(a.err, kErrPaged);
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < P4; ++e) sk[r][d + e] = kx[e], sv[r][d + e] = vx[e];
+      for (int e = 0; e < P4; ++e) sk[r][d + e] = kx[v][e], sv[r][d + e] = vx[v][e];
     }
     __syncthreads();
+    if (k0 + kKeys < k_hi) {
+      request(k0 + kKeys);
+      look_up(k0 + 2 * kKeys);
+    }
     float s[4] = {0.f, 0.f, 0.f, 0.f};
     for (int d = 0; d < D; ++d) {
       const float x = sq[qr][d];
@@ -192,35 +215,41 @@ __global__ void __launch_bounds__(kSimt) paged_attn_simt_kernel(PagedAttnArgs a,
   }
 }
 
-// Join of the key ranges of one (token, head), in their order.
+// Join of the key ranges of one (token, head), in their order: a block each,
+// a thread per dim.
 template <typename T, int D>
-__global__ void __launch_bounds__(kSimt) paged_attn_join_kernel(PagedAttnArgs a, int splits) {
+__global__ void __launch_bounds__(D < 32 ? 32 : D) paged_attn_join_kernel(const __grid_constant__ PagedAttnArgs a, int splits) {
   pdl_trigger();
   pdl_wait();
-  __shared__ int found;
   const int64_t t = blockIdx.x;
-  if (threadIdx.x == 0) found = 0;
-  __syncthreads();
-  for (int i = threadIdx.x; i < a.batch.B; i += kSimt) {  // rows of no (valid) sequence stay as they are
+  const int head = blockIdx.y, d = threadIdx.x;
+  bool found = false;  // rows of no (valid) sequence stay as they are
+  for (int i = threadIdx.x; i < a.batch.B; i += blockDim.x) {
     const SeqSpan sp = seq_span(a.batch, i, a.pool.ps);
-    if (sp.ok && sp.q0 <= t && t < sp.q0 + sp.n) found = 1;
+    found |= sp.ok && sp.q0 <= t && t < sp.q0 + sp.n;
   }
-  __syncthreads();
-  if (!found) return;
-  for (int i = threadIdx.x; i < a.nq * D; i += kSimt) {
-    const int head = i / D, d = i % D;
-    const float* w = (const float*)a.ws + (t * a.nq + head) * splits * (D + 2);
-    float mx = -INFINITY;
-    for (int z = 0; z < splits; ++z) mx = fmaxf(mx, w[z * (D + 2)]);
-    float l = 0.f, o = 0.f;
-    for (int z = 0; z < splits; ++z) {
-      const float mz = w[z * (D + 2)];
-      const float f = mz == -INFINITY ? 0.f : exp2f(mz - mx);
-      l += f * w[z * (D + 2) + 1];
-      o += f * w[z * (D + 2) + 2 + d];
+  if (!__syncthreads_or(found) || d >= D) return;
+  const float* w = (const float*)a.ws + (t * a.nq + head) * splits * (D + 2);
+  float M = -INFINITY, l = 0.f, o = 0.f;
+  for (int z0 = 0; z0 < splits; z0 += 8) {  // eight ranges' loads in flight
+    float m[8], s[8], v[8];
+#pragma unroll
+    for (int z = 0; z < 8; ++z) {
+      const float* q = w + min(z0 + z, splits - 1) * (D + 2);
+      m[z] = __ldcg(q);
+      s[z] = __ldcg(q + 1);
+      v[z] = __ldcg(q + 2 + d);
     }
-    stf<T>((T*)a.out + t * a.ldo + (int64_t)head * a.hdo + d, l == 0.f ? 0.f : o / l);
+#pragma unroll
+    for (int z = 0; z < 8; ++z) {
+      if (z0 + z >= splits || m[z] == -INFINITY) continue;
+      const float top = fmaxf(M, m[z]), keep = M == -INFINITY ? 0.f : exp2f(M - top), f = exp2f(m[z] - top);
+      M = top;
+      l = l * keep + f * s[z];
+      o = o * keep + f * v[z];
+    }
   }
+  stf<T>((T*)a.out + t * a.ldo + (int64_t)head * a.hdo + d, l == 0.f ? 0.f : o / l);
 }
 
 int simt_tiles(const PagedAttnArgs& a) {
@@ -242,7 +271,8 @@ cudaError_t launch_simt_d(const PagedAttnArgs& a, cudaStream_t s) {
   const dim3 grid((unsigned)(a.batch.B * tiles), (unsigned)a.pool.nkv, (unsigned)splits);
   cudaError_t e = launch_pdl(paged_attn_simt_kernel<T, C, D>, grid, dim3(kSimt), 0, s, a, tiles, splits);
   if (e == cudaSuccess && splits > 1)
-    e = launch_pdl(paged_attn_join_kernel<T, D>, dim3((unsigned)a.batch.T), dim3(kSimt), 0, s, a, splits);
+    e = launch_pdl(paged_attn_join_kernel<T, D>, dim3((unsigned)a.batch.T, (unsigned)a.nq), dim3(D < 32 ? 32 : D), 0, s, a,
+                   splits);
   return e;
 }
 

@@ -160,8 +160,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
     const int b = seq_of(u), nb = max(1, (slen[b] + BK - 1) / BK), off = (u - pre[b]) % nb;
     return off <= kSnap ? u - off : nb - off <= kSnap ? u + nb - off : u;
   };
+  // No workspace where no (sequence, head) can be cut.
   Cut* cuts = (Cut*)((float*)a.ws + (size_t)2 * gridDim.x * piece_floats(row_cap, D));
-  if (tid == 0) cuts[c] = Cut{0, 0, 0, 0};
+  if (a.ws && tid == 0) cuts[c] = Cut{0, 0, 0, 0};
   if (tid < 2 * kWarps) meta[tid >> 1][tid & 1].rows = 0;
   if (c >= grid) return;
   const int c0 = begin(c), c1 = begin(c + 1);
@@ -665,6 +666,12 @@ int row_cap(const PagedAttnArgs& a) {
   return (int)std::min<int64_t>(kRowsD, (int64_t)std::max(a.batch.max_new, 1) * (a.nq / a.pool.nkv));
 }
 
+// Whether a CTA's run can end inside a (sequence, head): one of at most
+// 2 kSnap blocks lies within kSnap of an end everywhere.
+bool may_cut(const PagedAttnArgs& a) {
+  return (int64_t)a.batch.max_pages * a.pool.ps > 2 * kSnap * block_keys(a.pool.cdtype == kE4M3);
+}
+
 template <int D, bool E4, int NT>
 cudaError_t launch_decode(const PagedAttnArgs& a, cudaStream_t s) {
   auto kernel = paged_decode_kernel<D, E4, NT>;
@@ -679,8 +686,10 @@ cudaError_t launch_decode(const PagedAttnArgs& a, cudaStream_t s) {
     configured[dev] = true;
   }
   const int rows = row_cap(a), grid = usable_sms();
-  cudaError_t e = launch_pdl(kernel, dim3(grid), dim3(kWarps * 32), bytes(rows, a.batch.B), s, a, rows);
-  if (e != cudaSuccess) return e;
+  PagedAttnArgs args = a;
+  if (!may_cut(a)) args.ws = nullptr;
+  cudaError_t e = launch_pdl(kernel, dim3(grid), dim3(kWarps * 32), bytes(rows, a.batch.B), s, args, rows);
+  if (e != cudaSuccess || !may_cut(a)) return e;
   return launch_pdl(paged_decode_join_kernel<D>, dim3(grid), dim3(kJoinWarps * 32), 0, s, a, rows);
 }
 
@@ -692,6 +701,7 @@ bool paged_decode_applicable(const PagedAttnArgs& a) {
 }
 
 size_t paged_decode_workspace(const PagedAttnArgs& a) {
+  if (!may_cut(a)) return 0;
   return (size_t)usable_sms() * (2 * piece_floats(row_cap(a), a.pool.D) * sizeof(float) + sizeof(Cut));
 }
 

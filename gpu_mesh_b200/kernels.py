@@ -173,7 +173,7 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     page: a page that sequences share is full, or copied first.
     """
     pool, batch = _paged(qkv, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale, max_new)
-    dev, nkv, D = qkv.device, pool.num_kv_heads, pool.head_dim
+    dev, (_, nkv, _, D) = qkv.device, k_pages.shape
     if qkv.ndim != 2 or num_q_heads < 1 or qkv.shape[1] != (num_q_heads + 2 * nkv) * D:
         raise ValueError("qkv must be [T, (num_q_heads + 2 kv heads) * head_dim]")
     T, (ld, inner) = qkv.shape[0], qkv.stride()
@@ -184,11 +184,12 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     if cos is not None or sin is not None:
         if cos is None or sin is None:
             raise ValueError("cos and sin come together")
-        for name, t in (("cos", cos), ("sin", sin)):
-            if t.dtype is not torch.float32 or t.device != dev or t.ndim != 2 or t.shape[1] * 2 != D or \
-                    t.shape != cos.shape or not t.is_contiguous():
-                raise ValueError(f"{name} must be a contiguous fp32 [positions, head_dim / 2] table on {dev}")
-        c, sn, max_pos = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
+        max_pos = cos.shape[0]
+        table = (max_pos, D // 2)
+        if not (cos.dtype is torch.float32 and sin.dtype is torch.float32 and cos.shape == table and sin.shape == table
+                and cos.device == dev and sin.device == dev and cos.is_contiguous() and sin.is_contiguous()):
+            raise ValueError(f"cos and sin must be contiguous fp32 [positions, head_dim / 2] tables on {dev}")
+        c, sn = cos.data_ptr(), sin.data_ptr()
     if q_norm is not None or k_norm is not None:
         for name, t in (("q_norm", q_norm), ("k_norm", k_norm)):
             if t is not None and (t.dtype is not qkv.dtype or t.device != dev or t.shape != (D,) or t.stride(0) != 1):
@@ -227,10 +228,11 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         raise ValueError("q must be [T, query heads, head_dim] with head_dim contiguous")
     pool, batch = _paged(q, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale, max_new)
     dev, nq = q.device, q.shape[1]
-    if q.shape[2] != pool.head_dim:
+    D = k_pages.shape[3]
+    if q.shape[2] != D:
         raise ValueError("q and the pages disagree on head_dim")
     if out is None:
-        out = q.new_empty(q.shape)
+        out = torch.empty_like(q)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1:
         raise ValueError("out must have q's shape and dtype, with head_dim contiguous")
     lib, dt, index = _lib.lib(), _DT[q.dtype], dev.index
@@ -241,7 +243,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
             scratch = q.new_empty(need, dtype=torch.uint8)
             ws = scratch.data_ptr()
         _lib.check(lib.mg_paged_attention(
-            pool, batch, dt, q.data_ptr(), ql, qh, nq, pool.head_dim ** -0.5 if scale is None else scale,
+            pool, batch, dt, q.data_ptr(), ql, qh, nq, D ** -0.5 if scale is None else scale,
             out.data_ptr(), ol, oh, ws, need, _raw_stream(index)))
     return out
 
