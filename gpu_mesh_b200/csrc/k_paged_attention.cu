@@ -27,7 +27,7 @@ namespace {
 constexpr int kRows = 16;     // query rows of a CTA
 constexpr int kKeys = 32;     // keys of a round
 constexpr int kSimt = 128;    // threads
-constexpr int kMaxSplits = 32;
+constexpr int kMaxSplits = 64;
 
 // One 16-byte (e4m3: 8-code) piece of a cached row, widened.
 template <typename C>
@@ -60,10 +60,11 @@ template <typename T, typename C, int D>
 __global__ void __launch_bounds__(kSimt) paged_attn_simt_kernel(const __grid_constant__ PagedAttnArgs a, int tiles, int splits) {
   constexpr int RPT = kRows * D / kSimt;          // output rows of a thread
   constexpr int P4 = Cached<C>::N;
-  __shared__ float sq[kRows][D + 1];
-  __shared__ float sk[kKeys][D + 1];
-  __shared__ float sv[kKeys][D];
-  __shared__ float sp[kRows][kKeys];
+  // Rows 4 floats apart in the banks: eight keys' 16-byte reads do not collide.
+  __shared__ __align__(16) float sq[kRows][D + 4];
+  __shared__ __align__(16) float sk[kKeys][D + 4];
+  __shared__ __align__(16) float sv[kKeys][D];
+  __shared__ __align__(16) float sp[kRows][kKeys];
   __shared__ float keep[kRows], sum[kRows], top[kRows];
   pdl_trigger();
   pdl_wait();
@@ -143,7 +144,10 @@ __global__ void __launch_bounds__(kSimt) paged_attn_simt_kernel(const __grid_con
       const int i = tid + v * kSimt, r = i / (D / P4), d = i % (D / P4) * P4;
       if (i >= kKeys * D / P4) continue;
 #pragma unroll
-      for (int e = 0; e < P4; ++e) sk[r][d + e] = kx[v][e], sv[r][d + e] = vx[v][e];
+      for (int e = 0; e < P4; e += 4) {
+        *reinterpret_cast<float4*>(&sk[r][d + e]) = make_float4(kx[v][e], kx[v][e + 1], kx[v][e + 2], kx[v][e + 3]);
+        *reinterpret_cast<float4*>(&sv[r][d + e]) = make_float4(vx[v][e], vx[v][e + 1], vx[v][e + 2], vx[v][e + 3]);
+      }
     }
     __syncthreads();
     if (k0 + kKeys < k_hi) {
@@ -151,10 +155,13 @@ __global__ void __launch_bounds__(kSimt) paged_attn_simt_kernel(const __grid_con
       look_up(k0 + 2 * kKeys);
     }
     float s[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int d = 0; d < D; ++d) {
-      const float x = sq[qr][d];
+    for (int d = 0; d < D; d += 4) {
+      const float4 x = *reinterpret_cast<const float4*>(&sq[qr][d]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[i] = fmaf(x, sk[kq + 8 * i][d], s[i]);
+      for (int i = 0; i < 4; ++i) {
+        const float4 y = *reinterpret_cast<const float4*>(&sk[kq + 8 * i][d]);
+        s[i] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, s[i]))));
+      }
     }
     float mx = m;
 #pragma unroll
@@ -182,12 +189,14 @@ __global__ void __launch_bounds__(kSimt) paged_attn_simt_kernel(const __grid_con
     for (int i = 0; i < RPT; ++i) acc[i] *= keep[og * RPT + i];
     // Keys that no row of the tile sees were loaded as zeros; a row's own
     // invisible keys weigh 0, but 0 · NaN is not 0, so they are left out.
-    for (int k = 0; k < kKeys; ++k) {
-      const float v = sv[k][od];
+    for (int k = 0; k < kKeys; k += 4) {
+      const float v[4] = {sv[k][od], sv[k + 1][od], sv[k + 2][od], sv[k + 3][od]};
 #pragma unroll
       for (int i = 0; i < RPT; ++i) {
-        const float p = sp[og * RPT + i][k];
-        acc[i] = p != 0.f ? fmaf(p, v, acc[i]) : acc[i];
+        const float4 p4 = *reinterpret_cast<const float4*>(&sp[og * RPT + i][k]);
+        const float p[4] = {p4.x, p4.y, p4.z, p4.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i] = p[e] != 0.f ? fmaf(p[e], v[e], acc[i]) : acc[i];
       }
     }
   }
@@ -256,12 +265,12 @@ int simt_tiles(const PagedAttnArgs& a) {
   return (int)(((int64_t)std::max(a.batch.max_new, 1) * (a.nq / a.pool.nkv) + kRows - 1) / kRows);
 }
 
-// Key ranges per row: enough CTAs for four per SM, at least 64 keys each.
+// Key ranges per row: enough CTAs for eight per SM, at least a round each.
 int simt_splits(const PagedAttnArgs& a) {
   const int64_t ctas = (int64_t)a.batch.B * simt_tiles(a) * a.pool.nkv;
   const int64_t keys = (int64_t)a.batch.max_pages * a.pool.ps;
-  int64_t n = ctas > 0 ? (4LL * usable_sms() + ctas - 1) / ctas : 1;
-  n = std::min<int64_t>(n, (keys + 63) / 64);
+  int64_t n = ctas > 0 ? (8LL * usable_sms() + ctas - 1) / ctas : 1;
+  n = std::min<int64_t>(n, (keys + kKeys - 1) / kKeys);
   return (int)std::max<int64_t>(1, std::min<int64_t>(n, kMaxSplits));
 }
 
