@@ -102,6 +102,11 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
   const PagedPool& pool = a.pool;
   const PagedBatch& bt = a.batch;
   const int G = a.nq / pool.nkv, nkv = pool.nkv;
+  // Two tiles of query rows keep their fragments in shared memory: in registers
+  // (and requested a piece ahead) they spill (16 sequences of up to 5 K keys, 2 to 4 tokens each, e4m3: 57 us
+  // against 43).
+  constexpr bool kQShared = NT == 2;
+  __shared__ uint2 qs[kQShared ? kWarps : 1][kQShared ? NT * KS : 1][32];
   extern __shared__ __align__(16) float held[];  // [warp][2][row][O(D), max, sum]: pieces for the CTA's join
   __shared__ PieceMeta meta[kWarps][2];          // 0: began in an earlier warp's part, 1: goes on in the next one's
   int* pre = (int*)(held + 2 * kWarps * piece_floats(row_cap, D));  // [B + 1] blocks before a sequence
@@ -233,7 +238,20 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
   uint4 kx[SUB][2][KP];       // keys g, g + 8 of each tile
   uint32_t vx[SUB][4][VW];    // values 2t, 2t + 1, 2t + 8, 2t + 9
   float ks[SUB], vs[SUB];
-  uint4 qx[NT][QW];           // query row g of each 8-row tile
+  uint4 qx[QW];               // query row g
+  // Query row g of 8-row tile nt, its dims in the order of the K fragments: a
+  // thread's 16 bytes of a key are 16 (bf16: 8) consecutive dims, k-steps of
+  // four dims each.
+  auto load_q = [&](const Block& x, int nt, uint4* to) {
+    const int r = nt * 8 + g;
+    const __nv_bfloat16* q = (const __nv_bfloat16*)a.q + (int64_t)((sqn[x.b] >> 5) + r / G) * a.ldq +
+                             (int64_t)(x.h * G + r % G) * a.hdq;
+#pragma unroll
+    for (int i = 0; i < QW; ++i)
+      to[i] = r < (sqn[x.b] & 31) * G
+                  ? *reinterpret_cast<const uint4*>(E4 ? q + 64 * (i / 2) + 16 * t + 8 * (i % 2) : q + 32 * i + 8 * t)
+                  : make_uint4(0u, 0u, 0u, 0u);
+  };
   // A block's keys (both scales, and the query rows of a new piece) and values:
   // each half is requested as soon as the registers of the block before are
   // free.  Offsets of a thread's rows inside a tile, in bytes; the tile lies in one page.
@@ -261,21 +279,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
         vs[i] = page >= 0 ? __ldg(pool.vs + page * pool.vse + x.h) : 1.f;
       }
     }
-    if (x.valid && x.first) {
-      const int rows = (sqn[x.b] & 31) * G;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const int r = nt * 8 + g;
-        const __nv_bfloat16* q = (const __nv_bfloat16*)a.q + (int64_t)((sqn[x.b] >> 5) + r / G) * a.ldq +
-                                 (int64_t)(x.h * G + r % G) * a.hdq;
-        // The dims in the order of the K fragments: a thread's 16 bytes of a
-        // key are 16 (bf16: 8) consecutive dims, k-steps of four dims each.
-#pragma unroll
-        for (int i = 0; i < QW; ++i)
-          qx[nt][i] = r < rows ? *reinterpret_cast<const uint4*>(E4 ? q + 64 * (i / 2) + 16 * t + 8 * (i % 2) : q + 32 * i + 8 * t)
-                               : make_uint4(0u, 0u, 0u, 0u);
-      }
-    }
+    if (!kQShared && x.valid && x.first) load_q(x, 0, qx);
   };
   auto load_v = [&](const Block& x) {
 #pragma unroll
@@ -319,7 +323,11 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
   int rows = 0, least = 0, from = 0, vis[NT][2];
   float mrow[NT][2], lrow[NT][2], rowf[NT][2];
   float o[NT][DM][4];
-  uint32_t qb[NT][KS][2];
+  uint32_t qb[KS][2];  // of the only tile
+  auto query = [&](int nt, int ks) {  // the B fragment of k-step ks
+    if constexpr (kQShared) return qs[warp][nt * KS + ks][lane];
+    return make_uint2(qb[ks][0], qb[ks][1]);
+  };
   while (now.valid) {
     if (now.first) {
       const int n = sqn[now.b] & 31, past = now.len - n;
@@ -338,11 +346,16 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
         }
 #pragma unroll
         for (int i = 0; i < DM; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+        auto keep = [&](int ks, uint32_t b0, uint32_t b1) {
+          if constexpr (kQShared) qs[warp][nt * KS + ks][lane] = make_uint2(b0, b1);
+          else qb[ks][0] = b0, qb[ks][1] = b1;
+        };
+        if constexpr (kQShared) load_q(now, nt, qx);
         if constexpr (E4) {
           float amax = 0.f;
 #pragma unroll
           for (int i = 0; i < QW; ++i) {
-            const uint32_t x[4] = {qx[nt][i].x, qx[nt][i].y, qx[nt][i].z, qx[nt][i].w};
+            const uint32_t x[4] = {qx[i].x, qx[i].y, qx[i].z, qx[i].w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) amax = fmaxf(amax, fmaxf(fabsf(lo_bf16(x[k])), fabsf(hi_bf16(x[k]))));
           }
@@ -352,11 +365,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
           const float f = pow2i(sh);
 #pragma unroll
           for (int i = 0; i < QW; ++i) {
-            const uint4 x = qx[nt][i];
-            qb[nt][2 * i][0] = pack_f16(lo_bf16(x.x) * f, hi_bf16(x.x) * f);
-            qb[nt][2 * i][1] = pack_f16(lo_bf16(x.y) * f, hi_bf16(x.y) * f);
-            qb[nt][2 * i + 1][0] = pack_f16(lo_bf16(x.z) * f, hi_bf16(x.z) * f);
-            qb[nt][2 * i + 1][1] = pack_f16(lo_bf16(x.w) * f, hi_bf16(x.w) * f);
+            const uint4 x = qx[i];
+            keep(2 * i, pack_f16(lo_bf16(x.x) * f, hi_bf16(x.x) * f), pack_f16(lo_bf16(x.y) * f, hi_bf16(x.y) * f));
+            keep(2 * i + 1, pack_f16(lo_bf16(x.z) * f, hi_bf16(x.z) * f), pack_f16(lo_bf16(x.w) * f, hi_bf16(x.w) * f));
           }
           // Row g's factor is needed by the threads that hold rows 2t, 2t + 1.
 #pragma unroll
@@ -364,10 +375,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
         } else {
 #pragma unroll
           for (int i = 0; i < QW; ++i) {
-            qb[nt][2 * i][0] = qx[nt][i].x;
-            qb[nt][2 * i][1] = qx[nt][i].y;
-            qb[nt][2 * i + 1][0] = qx[nt][i].z;
-            qb[nt][2 * i + 1][1] = qx[nt][i].w;
+            keep(2 * i, qx[i].x, qx[i].y);
+            keep(2 * i + 1, qx[i].z, qx[i].w);
           }
         }
       }
@@ -390,14 +399,20 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
             const uint32_t a0 = e4m3x2_to_f16x2(x[w]), a1 = e4m3x2_to_f16x2(y[w]);
             const uint32_t a2 = e4m3x2_hi_to_f16x2(x[w]), a3 = e4m3x2_hi_to_f16x2(y[w]);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma16816_f16(sc[nt][i], a0, a1, a2, a3, qb[nt][4 * q + w][0], qb[nt][4 * q + w][1]);
+            for (int nt = 0; nt < NT; ++nt) {
+                const uint2 b = query(nt, 4 * q + w);
+                mma16816_f16(sc[nt][i], a0, a1, a2, a3, b.x, b.y);
+              }
           }
         } else {
 #pragma unroll
           for (int w = 0; w < 2; ++w)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              mma16816_full(sc[nt][i], x[2 * w], y[2 * w], x[2 * w + 1], y[2 * w + 1], qb[nt][2 * q + w][0], qb[nt][2 * q + w][1]);
+              {
+                const uint2 b = query(nt, 2 * q + w);
+                mma16816_full(sc[nt][i], x[2 * w], y[2 * w], x[2 * w + 1], y[2 * w + 1], b.x, b.y);
+              }
         }
       }
     }
