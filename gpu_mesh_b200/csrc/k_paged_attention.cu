@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(D < 32 ? 32 : D) paged_attn_join_kernel(const 
     }
 #pragma unroll
     for (int z = 0; z < 8; ++z) {
-      if (z0 + z >= splits || m[z] == -INFINITY) continue;
+      if (z0 + z >= splits || s[z] == 0.f) continue;  // none, or it saw no key
       const float top = fmaxf(M, m[z]), keep = M == -INFINITY ? 0.f : exp2f(M - top), f = exp2f(m[z] - top);
       M = top;
       l = l * keep + f * s[z];

@@ -108,6 +108,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
   constexpr bool kQShared = NT == 2;
   __shared__ uint2 qs[kQShared ? kWarps : 1][kQShared ? NT * KS : 1][32];
   extern __shared__ __align__(16) float held[];  // [warp][2][row][O(D), max, sum]: pieces for the CTA's join
+  __shared__ int lost;                           // a row came out with NaN
   __shared__ PieceMeta meta[kWarps][2];          // 0: began in an earlier warp's part, 1: goes on in the next one's
   int* pre = (int*)(held + 2 * kWarps * piece_floats(row_cap, D));  // [B + 1] blocks before a sequence
   int* slen = pre + bt.B + 1;                                       // [B] cached tokens
@@ -169,6 +170,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
   Cut* cuts = (Cut*)((float*)a.ws + (size_t)2 * gridDim.x * piece_floats(row_cap, D));
   if (a.ws && tid == 0) cuts[c] = Cut{0, 0, 0, 0};
   if (tid < 2 * kWarps) meta[tid >> 1][tid & 1].rows = 0;
+  if (tid == 0) lost = 0;
   if (c >= grid) return;
   const int c0 = begin(c), c1 = begin(c + 1);
   if (c0 >= c1) return;
@@ -400,19 +402,18 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
             const uint32_t a2 = e4m3x2_hi_to_f16x2(x[w]), a3 = e4m3x2_hi_to_f16x2(y[w]);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                const uint2 b = query(nt, 4 * q + w);
-                mma16816_f16(sc[nt][i], a0, a1, a2, a3, b.x, b.y);
-              }
+              const uint2 b = query(nt, 4 * q + w);
+              mma16816_f16(sc[nt][i], a0, a1, a2, a3, b.x, b.y);
+            }
           }
         } else {
 #pragma unroll
           for (int w = 0; w < 2; ++w)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              {
-                const uint2 b = query(nt, 2 * q + w);
-                mma16816_full(sc[nt][i], x[2 * w], y[2 * w], x[2 * w + 1], y[2 * w + 1], b.x, b.y);
-              }
+            for (int nt = 0; nt < NT; ++nt) {
+              const uint2 b = query(nt, 2 * q + w);
+              mma16816_full(sc[nt][i], x[2 * w], y[2 * w], x[2 * w + 1], y[2 * w + 1], b.x, b.y);
+            }
         }
       }
     }
@@ -546,6 +547,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
                                  (int64_t)(now.h * G + r % G) * a.hdo + g * (D / 8);
 #pragma unroll
             for (int i = 0; i < D / 64; ++i) store16_f<__nv_bfloat16>(out + 8 * i, x + 8 * i);
+            float bad = 0.f;
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) bad = fmaf(x[i], 0.f, bad);
+            if (bad != 0.f) lost = 1;
           } else {
             float* part = held + (size_t)(2 * warp + slot) * piece_floats(row_cap, D) + r * (D + 2);
 #pragma unroll
@@ -585,8 +590,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
         acc += f * at(j)[d];
       }
       if (!begun && ends) {
-        ((__nv_bfloat16*)a.out)[(int64_t)(q0 + r / G) * a.ldo + (int64_t)(head.h * G + r % G) * a.hdo + d] =
-            __float2bfloat16_rn(S == 0.f ? 0.f : acc / S);
+        const float y = S == 0.f ? 0.f : acc / S;
+        ((__nv_bfloat16*)a.out)[(int64_t)(q0 + r / G) * a.ldo + (int64_t)(head.h * G + r % G) * a.hdo + d] = __float2bfloat16_rn(y);
+        if (y != y) lost = 1;
       } else {
         part[r * (D + 2) + d] = acc;
         if (d == 0) *reinterpret_cast<float2*>(part + r * (D + 2) + D) = make_float2(M, S);
@@ -600,6 +606,15 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
       cuts[c] = Cut{q0, head.h, head.rows, c - k + 1};
     }
   }
+  __syncthreads();
+  if (lost) {  // rows of the (sequence, head)s that lie in this run: those with NaN again
+    for (int u = c0; u < c1;) {
+      const int b = seq_of(u), nb = max(1, (slen[b] + BK - 1) / BK), h = (u - pre[b]) / nb, from = pre[b] + h * nb;
+      if (from >= c0 && from + nb <= c1)
+        for (int r = warp; r < (sqn[b] & 31) * G; r += kWarps) redo_if_nan<D, E4>(a, (sqn[b] >> 5) + r / G, h * G + r % G);
+      u = from + nb;
+    }
+  }
 }
 
 // Joins the pieces of the (sequence, KV head)s that CTAs' ends have cut, in
@@ -607,7 +622,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
 // row where there are few rows.
 constexpr int kJoinWarps = 8;
 
-template <int D>
+template <int D, bool E4>
 __global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(const __grid_constant__ PagedAttnArgs a,
                                                                            int row_cap) {
   constexpr int N = D / 32;
@@ -671,8 +686,13 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(cons
     if (mine && sub == 0) {
       const float f = L == 0.f ? 0.f : 1.f / L;
       __nv_bfloat16* out = (__nv_bfloat16*)a.out + (int64_t)(cut.q0 + r / G) * a.ldo + (int64_t)(cut.h * G + r % G) * a.hdo + lane * N;
+      float bad = 0.f;
 #pragma unroll
-      for (int i = 0; i < N / 2; ++i) *reinterpret_cast<uint32_t*>(out + 2 * i) = pack2(acc[2 * i] * f, acc[2 * i + 1] * f);
+      for (int i = 0; i < N / 2; ++i) {
+        *reinterpret_cast<uint32_t*>(out + 2 * i) = pack2(acc[2 * i] * f, acc[2 * i + 1] * f);
+        bad = fmaf(acc[2 * i] * f, 0.f, fmaf(acc[2 * i + 1] * f, 0.f, bad));
+      }
+      if (__any_sync(0xffffffffu, bad != 0.f)) redo_row<D, E4>(a, cut.q0 + r / G, cut.h * G + r % G);
     }
   }
 }
@@ -705,7 +725,7 @@ cudaError_t launch_decode(const PagedAttnArgs& a, cudaStream_t s) {
   if (!may_cut(a)) args.ws = nullptr;
   cudaError_t e = launch_pdl(kernel, dim3(grid), dim3(kWarps * 32), bytes(rows, a.batch.B), s, args, rows);
   if (e != cudaSuccess || !may_cut(a)) return e;
-  return launch_pdl(paged_decode_join_kernel<D>, dim3(grid), dim3(kJoinWarps * 32), 0, s, a, rows);
+  return launch_pdl(paged_decode_join_kernel<D, E4>, dim3(grid), dim3(kJoinWarps * 32), 0, s, a, rows);
 }
 
 }  // namespace

@@ -36,8 +36,8 @@
 //     fp32.  P in e4m3 would be 2^-4, so the values are not multiplied as
 //     codes: two converter warps turn them into halves (exact), MN-major;
 //     rows behind the sequence become zeros.
-// P is bf16 over bf16 pages (2^-8 half step at most 2^-9 relative): the
-// precision in which the stage's own prefill multiplies the values.
+// P is bf16 over bf16 pages (half a step: 2^-8 relative): the precision in
+// which the stage's own prefill multiplies the values.
 //
 // Bound: the MMA pipe and the exponentials, 4·D + 1 operations per score.
 // Every wait is bounded (code 3 in the error word on expiry); on expiry the
@@ -248,9 +248,10 @@ __host__ __device__ constexpr size_t partial_floats() {
 
 // What a CTA leaves for the join: the item that its run ends and earlier ones
 // began, as its sequence's first token row and new tokens, its KV head and
-// tile pair, and its pieces (0: there is none), this run's the last.
+// tile pair, and its pieces (0: there is none), this run's the last; and
+// whether a row of a whole item in its run came out with NaN.
 struct CutItem {
-  int q0, n, h, j, pieces, pad[3];
+  int q0, n, h, j, pieces, redo, pad[2];
 };
 
 __device__ __forceinline__ uint64_t desc_mn(const void* p, uint32_t lbo) {
@@ -391,6 +392,7 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
   uint64_t* drain = bars + 28;    // every MMA finished
   uint32_t* tmem_holder = (uint32_t*)(bars + 29);
   volatile int* abort_flag = (volatile int*)(tmem_holder + 1);
+  volatile int* redo = abort_flag + 1;  // a row came out with NaN
   // The scales of chunk n in slot n & 3: the keys' stage is free again before
   // the softmax of the chunk has ended, but chunk n + 4 is not converted before.
   float* sks = (float*)(smem + L::kOffScale);  // [4][8]
@@ -426,7 +428,7 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
   const RunsE runs(pre[bt.B], (int)gridDim.x);
   const int c = blockIdx.x;
   CutItem* cut = (CutItem*)((float*)a.ws + (size_t)2 * gridDim.x * partial_floats<D>()) + c;
-  if (threadIdx.x == 0) cut->pieces = 0;
+  if (threadIdx.x == 0) *redo = cut->pieces = cut->redo = 0;
   if (c >= runs.grid) return;
   if (warp == R::kProducer) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
@@ -490,8 +492,9 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
           ok = false;
           break;
         }
-        const int sh = row_shift(fmaxf(amax, other));
-        const float f = pow2i(sh);
+        amax = fmaxf(amax, other);
+        const int sh = row_shift(amax);
+        const float f = amax < INFINITY ? pow2i(sh) : NAN;  // a code would saturate an infinity
         rowf = scale2 * pow2i(-sh);
 #pragma unroll
         for (int p = 0; p < NP / 2; ++p) {  // 16 elements: a 16-byte piece of codes
@@ -636,6 +639,7 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
         bf16* out = (bf16*)a.out + (int64_t)(w.p.s.q0 + s_tok) * a.ldo + (int64_t)(w.at.h * G + r % G) * a.hdo;
         float* part = (float*)a.ws + (size_t)(2 * c + (w.lo > 0 ? 0 : 1)) * partial_floats<D>();
         const int row = x * kTile + r;
+        bool bad = false;
 #pragma unroll
         for (int c4 = 0; c4 < D / 64; ++c4) {
           const int d0 = (D / 2) * hf + c4 * 32;
@@ -647,7 +651,10 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
             for (int e = 0; e < 32; ++e) o[e] = 0.f;
           }
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] *= f;
+          for (int e = 0; e < 32; ++e) {
+            o[e] *= f;
+            bad |= o[e] != o[e];
+          }
           if (!w.whole) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -661,6 +668,7 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
                              bf16_pair(o[8 * e + 4], o[8 * e + 5]), bf16_pair(o[8 * e + 6], o[8 * e + 7]));
           }
         }
+        if (w.whole && valid && bad) *redo = 1;
         if (!w.whole && hf == 0) {
           part[2 * kTile * D + row] = m;
           part[2 * kTile * D + 2 * kTile + row] = l;
@@ -726,7 +734,8 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
     for (Walk w(a, pre, u0, u1); !w.done() && ok; w.next()) {
       if (w.lo > 0 && w.hi == w.units && lane == 0) {  // the last piece of a cut item
         const int start = w.u - w.lo, first = (int)((((long long)start + 1) * runs.grid - 1) / runs.total);
-        *cut = CutItem{w.p.s.q0, w.p.s.n, w.at.h, w.at.j, c - first + 1, {0, 0, 0}};
+        *reinterpret_cast<int4*>(cut) = make_int4(w.p.s.q0, w.p.s.n, w.at.h, w.at.j);
+        cut->pieces = c - first + 1;
       }
       // The tiles' query rows, once the previous piece's score products have read theirs.
 #pragma unroll
@@ -924,6 +933,7 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
       if (qn[x] > 0) mbar_wait(&qfull[x], (qn[x] - 1) & 1, a.err);
   }
   if (warp == R::kMma) mbar_wait(drain, 0, a.err);
+  if (threadIdx.x == 0 && *redo) cut->redo = 1;
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if (warp == R::kProducer) {
@@ -932,20 +942,35 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
 }
 
 // Joins the pieces of cut items, in order: block (c, y) 32 of the 256 rows of
-// the item that CTA c's run ends, eight lanes per row.
-template <int D>
+// the item that CTA c's run ends, eight lanes per row; and computes rows with
+// NaN of its run's whole items again (here, since the first kernel's roles
+// wait for one another with a limit).
+template <int D, bool E4>
 __global__ void __launch_bounds__(256) paged_extend_join_kernel(const __grid_constant__ PagedAttnArgs a) {
   pdl_trigger();
   pdl_wait();
   const int c = blockIdx.x;
   const CutItem* cut = (const CutItem*)((const float*)a.ws + (size_t)2 * gridDim.x * partial_floats<D>()) + c;
-  const int pieces = __ldcg(&cut->pieces);
+  const int2 todo = __ldcg(reinterpret_cast<const int2*>(&cut->pieces));
+  const int pieces = todo.x, G = a.nq / a.pool.nkv, tq = kTile / G;
+  if (todo.y != 0) {
+    extern __shared__ int pre[];
+    count_units(a, pre, false);
+    const RunsE runs(pre[a.batch.B], (int)gridDim.x);
+    for (Walk w(a, pre, runs.begin(c), runs.begin(c + 1)); !w.done(); w.next()) {
+      if (!w.whole) continue;
+      for (int i = threadIdx.x >> 5; i < 32; i += 8) {
+        const int row = blockIdx.y * 32 + i, r = row % kTile, s_tok = (2 * w.at.j + row / kTile) * tq + r / G;
+        if (r / G < tq && s_tok < w.p.s.n) redo_if_nan<D, E4>(a, w.p.s.q0 + s_tok, w.at.h * G + r % G);
+      }
+    }
+  }
   if (pieces == 0) return;
   const int4 it = __ldcg(reinterpret_cast<const int4*>(cut));  // q0, n, h, j
-  const int G = a.nq / a.pool.nkv, tq = kTile / G;
   const int row = blockIdx.y * 32 + (threadIdx.x >> 3), d0 = (threadIdx.x & 7) * (D / 8);
   const int r = row % kTile, s_tok = (2 * it.w + row / kTile) * tq + r / G;
-  if (r / G >= tq || s_tok >= it.y) return;
+  const bool valid = r / G < tq && s_tok < it.y;
+  if (!__any_sync(0xffffffffu, valid)) return;
   // The item's first run left it in its slot 1, the others in their slots 0.
   auto piece = [&](int k) {
     return (const float*)a.ws + (size_t)(2 * (c - pieces + 1 + k) + (k == 0 ? 1 : 0)) * partial_floats<D>();
@@ -966,7 +991,7 @@ __global__ void __launch_bounds__(256) paged_extend_join_kernel(const __grid_con
     }
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      if (k0 + k >= pieces || m[k] == -INFINITY) continue;
+      if (k0 + k >= pieces || l[k] == 0.f) continue;  // none, or it saw no key
       const float top = fmaxf(M, m[k]), keep = M == -INFINITY ? 0.f : ex2(M - top), f = ex2(m[k] - top);
       M = top;
       L = L * keep + f * l[k];
@@ -981,11 +1006,24 @@ __global__ void __launch_bounds__(256) paged_extend_join_kernel(const __grid_con
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
   bf16* out = (bf16*)a.out + (int64_t)(it.x + s_tok) * a.ldo + (int64_t)(it.z * G + r % G) * a.hdo + d0;
+  float bad = 0.f;
 #pragma unroll
-  for (int e = 0; e < D / 64; ++e)
-    *reinterpret_cast<uint4*>(out + 8 * e) =
-        make_uint4(bf16_pair(o[8 * e] * inv, o[8 * e + 1] * inv), bf16_pair(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
-                   bf16_pair(o[8 * e + 4] * inv, o[8 * e + 5] * inv), bf16_pair(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
+  for (int e = 0; e < D / 8; ++e) {
+    o[e] *= inv;
+    bad = fmaf(o[e], 0.f, bad);
+  }
+  if (valid) {
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e)
+      *reinterpret_cast<uint4*>(out + 8 * e) = make_uint4(bf16_pair(o[8 * e], o[8 * e + 1]), bf16_pair(o[8 * e + 2], o[8 * e + 3]),
+                                                          bf16_pair(o[8 * e + 4], o[8 * e + 5]), bf16_pair(o[8 * e + 6], o[8 * e + 7]));
+  }
+  unsigned again = __ballot_sync(0xffffffffu, valid && bad != 0.f);
+  while (again) {  // eight lanes are a row
+    const int lane = __ffs(again) - 1;
+    again &= ~(0xffu << (lane & ~7));
+    redo_row<D, E4>(a, __shfl_sync(0xffffffffu, it.x + s_tok, lane), __shfl_sync(0xffffffffu, it.z * G + r % G, lane));
+  }
 }
 
 int extend_grid() { return usable_sms(); }
@@ -1019,8 +1057,8 @@ cudaError_t launch_extend(const PagedAttnArgs& a, cudaStream_t s) {
   const int grid = extend_grid();
   cudaError_t e = launch_pdl(kernel, dim3(grid), dim3(Roles<E4>::kThreads), ExtendLayout<D, E4>::bytes(a.batch.B), s, maps,
                              tq_map, a);
-  if (e != cudaSuccess || grid == 1) return e;
-  return launch_pdl(paged_extend_join_kernel<D>, dim3(grid, 2 * kTile / 32), dim3(256), 0, s, a);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(paged_extend_join_kernel<D, E4>, dim3(grid, 2 * kTile / 32), dim3(256), (size_t)(a.batch.B + 1) * 4, s, a);
 }
 
 }  // namespace

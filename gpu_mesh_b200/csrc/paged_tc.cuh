@@ -99,5 +99,80 @@ __device__ __forceinline__ int row_shift(float amax) {
   return amax > 0.f ? min(7 - ((int)(__float_as_uint(amax) >> 23) - 127), 126) : 0;
 }
 
+// One (token row, query head) again, by a whole warp, key
+// by key in fp32.  The tensor-core kernels multiply all values of a block, a
+// row's invisible ones by the weight 0, and 0 times an infinity or a NaN of a
+// later token is NaN: a row that comes out with NaN is computed again from
+// what it sees.  So is one that sees such a value, which then comes out as the
+// formula has it; some 100 ns per key, paid by rows that are lost anyway.
+template <int D, bool E4>
+__device__ __noinline__ void redo_row(const PagedAttnArgs& a, int t, int head) {
+  constexpr int N = D / 32;  // dims of a lane
+  const PagedPool& pool = a.pool;
+  const int lane = threadIdx.x & 31, h = head / (a.nq / pool.nkv);
+  int b = -1, vis = 0;
+  for (int b0 = 0; b0 < a.batch.B && b < 0; b0 += 32) {
+    SeqSpan s{0, 0, 0, false};
+    if (b0 + lane < a.batch.B) s = seq_span(a.batch, b0 + lane, pool.ps);
+    const unsigned found = __ballot_sync(0xffffffffu, s.ok && s.q0 <= t && t < s.q0 + s.n);
+    if (found) {
+      b = b0 + __ffs(found) - 1;
+      vis = __shfl_sync(0xffffffffu, s.past + t - s.q0 + 1, __ffs(found) - 1);
+    }
+  }
+  if (b < 0) return;
+  float q[N], acc[N], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    q[i] = __bfloat162float(((const __nv_bfloat16*)a.q)[(int64_t)t * a.ldq + (int64_t)head * a.hdq + lane * N + i]) *
+           (a.scale * 1.4426950408889634f);
+    acc[i] = 0.f;
+  }
+#pragma unroll 1
+  for (int j = 0; j < vis; ++j) {
+    const int page = a.batch.table[(int64_t)b * a.batch.ld + j / pool.ps], o = j % pool.ps;
+    float k[N], v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) k[i] = v[i] = 0.f;
+    if (page >= 0 && page < pool.pages) {
+      const int64_t kat = page * pool.kp + h * pool.kh + o * pool.kt + lane * N;
+      const int64_t vat = page * pool.vp + h * pool.vh + o * pool.vt + lane * N;
+      const float fk = E4 ? pool.ks[page * pool.kse + h] : 1.f, fv = E4 ? pool.vs[page * pool.vse + h] : 1.f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if constexpr (E4) {
+          k[i] = from_e4m3x2(((const uint8_t*)pool.k)[kat + i]).x * fk;
+          v[i] = from_e4m3x2(((const uint8_t*)pool.v)[vat + i]).x * fv;
+        } else {
+          k[i] = __bfloat162float(((const __nv_bfloat16*)pool.k)[kat + i]);
+          v[i] = __bfloat162float(((const __nv_bfloat16*)pool.v)[vat + i]);
+        }
+      }
+    }
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) s = fmaf(q[i], k[i], s);
+#pragma unroll
+    for (int i = 16; i > 0; i >>= 1) s += __shfl_xor_sync(0xffffffffu, s, i);
+    const float top = fmaxf(m, s), keep = m == -INFINITY ? 0.f : ex2(m - top), w = ex2(s - top);
+    m = top;
+    l = l * keep + w;
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = acc[i] * keep + w * v[i];
+  }
+  __nv_bfloat16* out = (__nv_bfloat16*)a.out + (int64_t)t * a.ldo + (int64_t)head * a.hdo;
+#pragma unroll
+  for (int i = 0; i < N; ++i) out[lane * N + i] = __float2bfloat16_rn(l == 0.f ? 0.f : acc[i] / l);
+}
+
+// The same for a row that this block has written, if it holds a NaN.
+template <int D, bool E4>
+__device__ __forceinline__ void redo_if_nan(const PagedAttnArgs& a, int t, int head) {
+  const __nv_bfloat16* out = (const __nv_bfloat16*)a.out + (int64_t)t * a.ldo + (int64_t)head * a.hdo;
+  bool bad = false;
+  for (int d = threadIdx.x & 31; d < D; d += 32) bad |= __hisnan(out[d]);
+  if (__any_sync(0xffffffffu, bad)) redo_row<D, E4>(a, t, head);
+}
+
 }  // namespace paged
 }  // namespace mg

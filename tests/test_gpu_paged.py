@@ -621,3 +621,65 @@ def test_pool_past_32_bits(dtype, cache):
         small = kernels.paged_attention(q, small_k, small_v, c.table.to(DEV), *a, max_new=limit, **c.scales())
         assert torch.equal(big, small)
     kernels.paged_check_device()
+
+
+@pytest.mark.parametrize("dtype,cache", [(BF16, BF16), (BF16, E4M3), (F32, F32), (F32, E4M3)])
+@pytest.mark.parametrize("case", range(4))
+def test_attention_broken_tokens(dtype, cache, case):
+    """Infinities and NaN in keys or values reach the rows that see them, none before: not those of the same block of
+    keys, of the same tile, or of other sequences in the same page's row of the pool."""
+    new, lens = [([4, 2, 1], [700, 40, 300]), ([3, 4, 1, 2], [5000, 4000, 17, 2]), ([60, 9, 150], [60, 33, 420]),
+                 ([200, 130], [3001, 1500])][case]
+    D, nq, nkv, ps = (64, 4, 2, 32) if case % 2 else (128, 8, 2, 64)
+    c = Cache(lens, nkv, ps, D, dtype, cache, seed=case)
+    c.fill(lens)
+    q = torch.randn(sum(new), nq, D, generator=torch.Generator().manual_seed(case)).to(dtype)
+    code = cache == E4M3
+
+    def put(pages, b, j, h, d, x):
+        at = (int(c.table[b, j // ps]), h, j % ps)
+        if code:
+            pages.view(torch.uint8)[at][d] = 0x7F  # the only special value of the type
+        else:
+            pages[at][d] = x
+
+    for b, (n, L) in enumerate(zip(new, lens)):
+        if n < 2:
+            continue
+        put(c.v, b, L - 1, 0, 3, math.nan)                # seen by the last token alone
+        put(c.v, b, L - n // 2 - 1, 1, slice(0, D, 7), math.inf)
+        put(c.k, b, L - 1, 1, 5, math.nan)
+    got = torch.full_like(q, 7.0).to(DEV)
+    kernels.paged_attention(q.to(DEV), c.k, c.v, c.table.to(DEV), dev32(starts(new)), dev32(lens), out=got, **c.scales())
+    kernels.paged_check_device()
+    pools, got = c.host(), got.cpu().double()
+    for b, (t0, n, past) in enumerate(R.spans(starts(new), lens)):
+        k, v = (R.dense(*pools[key], c.table[b], lens[b]) for key in ("k", "v"))
+        for i in range(n):
+            see = past + i + 1
+            ref, weight, top = R.attend(q[t0 + i:t0 + i + 1].double(), k[:, :see], v[:, :see], past + i, D**-0.5)
+            tol = R.attention_tolerance(ref, weight, top, D, see, dtype, P_STEP[dtype], code and dtype == BF16)
+            x, ref, tol = got[t0 + i], ref[0], tol[0]
+            assert torch.equal(x.isnan(), ref.isnan()), (b, i)
+            assert torch.equal(x.isinf(), ref.isinf()) and torch.equal(x[x.isinf()], ref[ref.isinf()]), (b, i)
+            fine = ref.isfinite()
+            assert ((x - ref).abs()[fine] <= tol[fine]).all(), (b, i)
+
+
+@pytest.mark.parametrize("dtype,cache", [(BF16, BF16), (BF16, E4M3), (F32, F32), (F32, E4M3)])
+def test_attention_broken_queries(dtype, cache):
+    """An infinity or a NaN in a query row reaches that row alone, also where the keys are cut into parts."""
+    new, lens = [1, 4, 70, 1], [6000, 300, 2500, 9]
+    c = Cache(lens, 2, 32, 64, dtype, cache, seed=9)
+    c.fill(lens)
+    q = torch.randn(sum(new), 6, 64, generator=torch.Generator().manual_seed(2)).to(dtype).to(DEV)
+    bad = torch.zeros(q.shape[:2], dtype=torch.bool, device=DEV)
+    args = (c.k, c.v, c.table.to(DEV), dev32(starts(new)), dev32(lens))
+    plain = kernels.paged_attention(q, *args, **c.scales())
+    for t, h, x in ((0, 1, math.nan), (0, 4, math.inf), (2, 0, -math.inf), (20, 5, math.nan), (60, 2, math.inf)):
+        q[t, h, 7] = x
+        bad[t, h] = True
+    got = kernels.paged_attention(q, *args, **c.scales())
+    kernels.paged_check_device()
+    assert got[bad].isnan().all()
+    assert torch.equal(got[~bad], plain[~bad])
