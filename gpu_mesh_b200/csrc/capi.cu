@@ -1363,6 +1363,7 @@ int paged_args(const mg_paged_pool* p, const mg_paged_batch* b, int32_t dtype, i
   if (p->num_pages < 1 || p->num_kv_heads < 1) return fail(MG_EINVAL, "num_pages and num_kv_heads must be positive");
   if (nq < 1 || nq % p->num_kv_heads != 0 || nq / p->num_kv_heads > 16)
     return fail(MG_EINVAL, "num_q_heads must be 1 to 16 times num_kv_heads (%d and %d)", nq, p->num_kv_heads);
+  if (nq > 65535) return fail(MG_EINVAL, "num_q_heads must be at most 65535 (got %d)", nq);
   const bool e4m3 = p->cache_dtype == MG_DTYPE_E4M3;
   if (e4m3 && (!p->k_scale || !p->v_scale)) return fail(MG_EINVAL, "e4m3 pages need k_scale and v_scale");
   if (e4m3 && p->num_pages > 1 && (p->k_scale_stride < p->num_kv_heads || p->v_scale_stride < p->num_kv_heads))
@@ -1382,8 +1383,8 @@ int paged_args(const mg_paged_pool* p, const mg_paged_batch* b, int32_t dtype, i
   if (b->batch > kPagedMaxBatch) return fail(MG_EINVAL, "at most %d sequences per call (got %d)", kPagedMaxBatch, b->batch);
   if (b->batch > 0 && b->tokens > 0) {
     if (!b->page_table || !b->q_start || !b->kv_len) return fail(MG_EINVAL, "null page_table, q_start or kv_len");
-    if (b->max_pages < 1 || (int64_t)b->max_pages * ps > INT32_MAX)
-      return fail(MG_EINVAL, "the table's columns must hold 1 to 2^31 - 1 tokens");
+    if (b->max_pages < 1 || (int64_t)b->max_pages * ps > kPagedMaxLen)
+      return fail(MG_EINVAL, "the table's columns must hold 1 to 2^30 tokens");
     if (b->batch > 1 && b->table_stride < b->max_pages) return fail(MG_EINVAL, "table_stride is below max_pages");
   }
   *pool = PagedPool{p->k, p->v, p->k_scale, p->v_scale,

@@ -459,8 +459,9 @@ cudaError_t launch_d(const PagedAppendArgs& a, cudaStream_t s) {
   if (a.batch.max_new <= kThinNew)
     return launch_pdl(paged_append_kernel<T, D, 1>, dim3(rows + 1), dim3(kThreads), 0, s, a, 0, kWarpsA);
   const int units = RunShape<T, D>::units(a.pool.ps);
-  const int tiles = (rows / a.pool.ps + 2 * a.batch.B) * ((2 * a.pool.nkv + units - 1) / units);
-  return launch_pdl(paged_append_kernel<T, D, 2>, dim3((unsigned)(tiles + blocks)), dim3(kThreads), 0, s, a, tiles, per);
+  const int64_t tiles = (int64_t)(rows / a.pool.ps + 2 * a.batch.B) * ((2 * a.pool.nkv + units - 1) / units);
+  if (tiles + blocks > INT32_MAX) return cudaErrorInvalidConfiguration;
+  return launch_pdl(paged_append_kernel<T, D, 2>, dim3((unsigned)(tiles + blocks)), dim3(kThreads), 0, s, a, (int)tiles, per);
 }
 
 template <typename T>

@@ -56,6 +56,12 @@ struct Cached<uint8_t> {
   }
 };
 
+// The workspace holds a part of D + 2 floats (maximum, sum, O) per key range
+// of each (new token, head): the s-th new token of sequence b is its row
+// part_row(a, b) + s.  By the batch's bounds, not by token rows, of which a
+// padded batch may have many more.
+__device__ __forceinline__ int64_t part_row(const PagedAttnArgs& a, int b) { return (int64_t)b * max(a.batch.max_new, 1); }
+
 template <typename T, typename C, int D>
 __global__ void __launch_bounds__(kSimt) paged_attn_simt_kernel(const __grid_constant__ PagedAttnArgs a, int tiles, int splits) {
   constexpr int RPT = kRows * D / kSimt;          // output rows of a thread
@@ -214,7 +220,7 @@ __global__ void __launch_bounds__(kSimt) paged_attn_simt_kernel(const __grid_con
     if (splits == 1) {
       stf<T>((T*)a.out + t * a.ldo + (int64_t)head * a.hdo + od, sum[r] == 0.f ? 0.f : acc[i] / sum[r]);
     } else {
-      float* w = (float*)a.ws + ((t * a.nq + head) * splits + z) * (D + 2);
+      float* w = (float*)a.ws + (((part_row(a, b) - span.q0 + t) * a.nq + head) * splits + z) * (D + 2);
       w[2 + od] = acc[i];
       if (od == 0) {
         w[0] = top[r];
@@ -224,50 +230,46 @@ __global__ void __launch_bounds__(kSimt) paged_attn_simt_kernel(const __grid_con
   }
 }
 
-// Join of the key ranges of one (token, head), in their order: a block each,
-// a thread per dim.
+// Join of the key ranges of one (new token, head), in their order: block
+// (x, head) the x % max_new-th new token of sequence x / max_new, a thread per dim.
 template <typename T, int D>
 __global__ void __launch_bounds__(D < 32 ? 32 : D) paged_attn_join_kernel(const __grid_constant__ PagedAttnArgs a, int splits) {
   pdl_trigger();
   pdl_wait();
-  const int64_t t = blockIdx.x;
-  const int head = blockIdx.y, d = threadIdx.x;
-  bool found = false;  // rows of no (valid) sequence stay as they are
-  for (int i = threadIdx.x; i < a.batch.B; i += blockDim.x) {
-    const SeqSpan sp = seq_span(a.batch, i, a.pool.ps);
-    found |= sp.ok && sp.q0 <= t && t < sp.q0 + sp.n;
-  }
-  if (!__syncthreads_or(found) || d >= D) return;
-  const float* w = (const float*)a.ws + (t * a.nq + head) * splits * (D + 2);
+  const int most = max(a.batch.max_new, 1), b = blockIdx.x / most, s = blockIdx.x % most;
+  const int head = blockIdx.y, d = min((int)threadIdx.x, D - 1);
+  const SeqSpan span = seq_span(a.batch, b, a.pool.ps);  // on its way beside the parts
+  const float* w = (const float*)a.ws + ((part_row(a, b) + s) * a.nq + head) * splits * (D + 2);
   float M = -INFINITY, l = 0.f, o = 0.f;
   for (int z0 = 0; z0 < splits; z0 += 8) {  // eight ranges' loads in flight
-    float m[8], s[8], v[8];
+    float m[8], sum[8], v[8];
 #pragma unroll
     for (int z = 0; z < 8; ++z) {
       const float* q = w + min(z0 + z, splits - 1) * (D + 2);
       m[z] = __ldcg(q);
-      s[z] = __ldcg(q + 1);
+      sum[z] = __ldcg(q + 1);
       v[z] = __ldcg(q + 2 + d);
     }
 #pragma unroll
     for (int z = 0; z < 8; ++z) {
-      if (z0 + z >= splits || s[z] == 0.f) continue;  // none, or it saw no key
+      if (z0 + z >= splits || sum[z] == 0.f) continue;  // none, or it saw no key
       const float top = fmaxf(M, m[z]), keep = M == -INFINITY ? 0.f : exp2f(M - top), f = exp2f(m[z] - top);
       M = top;
-      l = l * keep + f * s[z];
+      l = l * keep + f * sum[z];
       o = o * keep + f * v[z];
     }
   }
-  stf<T>((T*)a.out + t * a.ldo + (int64_t)head * a.hdo + d, l == 0.f ? 0.f : o / l);
+  if (s >= span.n || threadIdx.x >= D) return;
+  stf<T>((T*)a.out + (int64_t)(span.q0 + s) * a.ldo + (int64_t)head * a.hdo + d, l == 0.f ? 0.f : o / l);
 }
 
-int simt_tiles(const PagedAttnArgs& a) {
-  return (int)(((int64_t)std::max(a.batch.max_new, 1) * (a.nq / a.pool.nkv) + kRows - 1) / kRows);
+int64_t simt_tiles(const PagedAttnArgs& a) {
+  return ((int64_t)std::max(a.batch.max_new, 1) * (a.nq / a.pool.nkv) + kRows - 1) / kRows;
 }
 
 // Key ranges per row: enough CTAs for eight per SM, at least a round each.
 int simt_splits(const PagedAttnArgs& a) {
-  const int64_t ctas = (int64_t)a.batch.B * simt_tiles(a) * a.pool.nkv;
+  const int64_t ctas = a.batch.B * simt_tiles(a) * a.pool.nkv;
   const int64_t keys = (int64_t)a.batch.max_pages * a.pool.ps;
   int64_t n = ctas > 0 ? (8LL * usable_sms() + ctas - 1) / ctas : 1;
   n = std::min<int64_t>(n, (keys + kKeys - 1) / kKeys);
@@ -276,12 +278,14 @@ int simt_splits(const PagedAttnArgs& a) {
 
 template <typename T, typename C, int D>
 cudaError_t launch_simt_d(const PagedAttnArgs& a, cudaStream_t s) {
-  const int tiles = simt_tiles(a), splits = simt_splits(a);
-  const dim3 grid((unsigned)(a.batch.B * tiles), (unsigned)a.pool.nkv, (unsigned)splits);
-  cudaError_t e = launch_pdl(paged_attn_simt_kernel<T, C, D>, grid, dim3(kSimt), 0, s, a, tiles, splits);
+  const int64_t tiles = simt_tiles(a), ctas = a.batch.B * tiles;
+  const int splits = simt_splits(a);
+  if (ctas > INT32_MAX) return cudaErrorInvalidConfiguration;  // (B · max_new beyond any batch that fits the GPU)
+  const dim3 grid((unsigned)ctas, (unsigned)a.pool.nkv, (unsigned)splits);
+  cudaError_t e = launch_pdl(paged_attn_simt_kernel<T, C, D>, grid, dim3(kSimt), 0, s, a, (int)tiles, splits);
   if (e == cudaSuccess && splits > 1)
-    e = launch_pdl(paged_attn_join_kernel<T, D>, dim3((unsigned)a.batch.T, (unsigned)a.nq), dim3(D < 32 ? 32 : D), 0, s, a,
-                   splits);
+    e = launch_pdl(paged_attn_join_kernel<T, D>, dim3((unsigned)(a.batch.B * std::max(a.batch.max_new, 1)), (unsigned)a.nq),
+                   dim3(D < 32 ? 32 : D), 0, s, a, splits);
   return e;
 }
 
@@ -297,13 +301,9 @@ cudaError_t launch_simt(const PagedAttnArgs& a, cudaStream_t s) {
   return cudaErrorInvalidValue;
 }
 
-}  // namespace
-
-namespace {
-
 size_t simt_workspace(const PagedAttnArgs& a) {
   const int splits = simt_splits(a);
-  return splits > 1 ? (size_t)a.batch.T * a.nq * splits * (a.pool.D + 2) * sizeof(float) : 0;
+  return splits > 1 ? (size_t)a.batch.B * std::max(a.batch.max_new, 1) * a.nq * splits * (a.pool.D + 2) * sizeof(float) : 0;
 }
 
 bool only_few(const PagedAttnArgs& a) {

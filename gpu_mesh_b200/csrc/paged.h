@@ -16,6 +16,7 @@ constexpr int kPagedMaxBatch = 2048; // sequences of one call (the kernels keep 
 constexpr int kPagedMinExp = -100;   // least exponent of a page's scale
 constexpr int kPagedMaxExp = 100;    // largest: sums weighed by 2^-e stay in fp32's range
 constexpr int kPagedMaxTokens = 1 << 26;  // token rows of one call
+constexpr int64_t kPagedMaxLen = 1 << 30; // tokens that a table row may hold: positions stay clear of 32 bits
 
 // Page p, KV head h, token o (of page_size) is the D contiguous elements at
 // k + p·kp + h·kh + o·kt (strides in elements, v likewise).  In an e4m3 pool

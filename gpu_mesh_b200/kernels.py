@@ -27,6 +27,9 @@ beside single tokens)::
 * ``max_new``: a host bound on the new tokens of one sequence (default: all rows).  A step of single tokens
   should pass 1: it chooses the kernels.
 
+Page sizes 16, 32, 64 and 128, head sizes 8, 16, 32, 64 and 128, up to 16 query heads per KV head, 2048 sequences
+and 2^26 - 1 token rows per call.  bf16 with head sizes 64 and 128 runs attention on the tensor cores.
+
 The current stream runs the work, and nothing waits for it: what only the device can see (a page id outside the
 pool, a length outside the table) leaves that sequence out and is raised by ``paged_check_device``.
 """

@@ -341,16 +341,17 @@ typedef struct mg_paged_pool {
   int32_t cache_dtype; /* the activations' dtype, or MG_DTYPE_E4M3 */
 } mg_paged_pool;
 
-/* A ragged batch of at most 2048 sequences and fewer than 2^26 token rows.  Sequence b brings the token rows
- * q_start[b] .. q_start[b + 1] - 1 (possibly none) and holds kv_len[b] cached
- * tokens with them; its token j lies in page page_table[b table_stride +
- * j / page_size].  All three arrays are on the device and are read by the
- * kernels only, so a captured call follows their contents; entries of the
- * table past a sequence's last page are not read.  Rows of the token tensors
- * behind q_start[batch] are left as they are.  A sequence whose ranges do not
- * fit (a length above max_pages page_size, more than max_new new tokens, rows
- * outside [0, tokens)) is left out, and, like a page id outside the pool,
- * reported by mg_paged_check_device. */
+/* A ragged batch of at most 2048 sequences and fewer than 2^26 token rows.
+ * Sequence b brings the token rows q_start[b] .. q_start[b + 1] - 1 (possibly
+ * none) and holds kv_len[b] cached tokens with them; its token j lies in page
+ * page_table[b table_stride + j / page_size].  All three arrays are on the
+ * device and are read by the kernels only, so a captured call follows their
+ * contents; entries of the table past a sequence's last page are not read, and
+ * its columns hold at most 2^30 tokens.  Rows of the token tensors behind
+ * q_start[batch] are left as they are.  A sequence whose ranges do not fit (a
+ * length above max_pages page_size, more than max_new new tokens, rows outside
+ * [0, tokens)) is left out, and, like a page id outside the pool, reported by
+ * mg_paged_check_device. */
 typedef struct mg_paged_batch {
   const int32_t* page_table; /* [batch, max_pages] */
   const int32_t* q_start;    /* [batch + 1] */
@@ -383,9 +384,11 @@ int mg_paged_append(const mg_paged_pool* pool, const mg_paged_batch* batch, int3
                     void* q_out, int64_t ld_q, void* stream);
 
 /* out[t, h] = softmax over the visible keys of scale q[t, h]·K, times V, with
- * num_q_heads / num_kv_heads (at most 16) query heads per KV head.  The s-th
+ * num_q_heads / num_kv_heads (at most 16) query heads per KV head (at most
+ * 65535 in all).  The s-th
  * of n new tokens sees the keys j <= kv_len - n + s; a row without any gives
- * 0.  q and out: strides of tokens and heads in elements.  `workspace` (device
+ * 0; an infinity or a NaN reaches the rows that see it alone.  q and out do
+ * not overlap; their strides of tokens and heads are in elements.  `workspace` (device
  * memory, 256-byte aligned, mg_paged_attention_workspace bytes) belongs to
  * the call until it has run on `stream`; it needs no initialisation. */
 int mg_paged_attention(const mg_paged_pool* pool, const mg_paged_batch* batch, int32_t dtype, const void* q,

@@ -683,3 +683,48 @@ def test_attention_broken_queries(dtype, cache):
     kernels.paged_check_device()
     assert got[bad].isnan().all()
     assert torch.equal(got[~bad], plain[~bad])
+
+
+@pytest.mark.parametrize("dtype,cache", [(BF16, BF16), (BF16, E4M3), (F32, E4M3)])
+@pytest.mark.parametrize("rows", [400, 800, 1400])
+def test_append_many_rows(dtype, cache, rows):
+    """Hundreds of rows of forty sequences: fewer warps per token, and a sequence that is not among the first 32."""
+    g = torch.Generator().manual_seed(rows)
+    new = (torch.rand(40, generator=g) ** 3 * rows / 20).long().tolist()
+    new[37] += rows - sum(new)
+    past = torch.randint(0, 70, (40,), generator=g).tolist()
+    lens = [p + n for p, n in zip(past, new)]
+    for D, nq, nkv, ps in ((64, 3, 1, 16), (128, 4, 2, 64)):
+        c = Cache(lens, nkv, ps, D, dtype, cache, seed=rows)
+        c.fill(past, spread=6)
+        run_append(c, new, lens, nq, norm=True, extra=5)
+
+
+@pytest.mark.parametrize("cache", [BF16, E4M3])
+def test_most_sequences(cache):
+    """The most sequences of a call, single tokens and a few with more; one more is refused."""
+    g = torch.Generator().manual_seed(8)
+    new, lens = [1] * 2048, torch.randint(1, 50, (2048,), generator=g).tolist()
+    for i, n in ((5, 30), (1200, 2), (2047, 40)):
+        new[i], lens[i] = n, max(n, lens[i])
+    c = Cache(lens, 1, 16, 64, BF16, cache)
+    c.fill([a - b for a, b in zip(lens, new)])
+    run_append(c, new, lens, 2)
+    attend(c, new, lens, 4)
+    attend(c, [1] * 2048, lens, 2, max_new=1)
+    with pytest.raises(ValueError, match="2048"):
+        kernels.paged_attention(torch.zeros(1, 2, 64, dtype=BF16, device=DEV), c.k, c.v, torch.zeros(2049, 1, dtype=torch.int32, device=DEV),
+                                dev32([0] * 2050), dev32([0] * 2049), **c.scales())
+
+
+@pytest.mark.parametrize("dtype,cache", [(BF16, BF16), (F32, F32)])
+def test_padded_batch(dtype, cache):
+    """A batch padded to a captured size: rows of no sequence, sequences without rows or tokens, a wide table."""
+    lens = [300, 45, 0, 0]
+    c = Cache(lens, 2, 16, 64, dtype, cache)
+    c.cols += 500
+    c.table = torch.cat((c.table, torch.full((4, 500), -1, dtype=torch.int32)), 1)
+    c.fill(lens)
+    attend(c, [1, 1, 0, 0], lens, 4, extra=4094, max_new=1)
+    attend(c, [1, 3, 0, 0], lens, 4, extra=600, max_new=8)
+    run_append(c, [1, 1, 0, 0], lens, 4, extra=2000, max_new=1)

@@ -62,6 +62,8 @@ SHARED = [
     (dict(), dict(q_start=None), dict(), "null"),
     (dict(), dict(max_pages=0), dict(), "columns"),
     (dict(), dict(max_pages=1 << 28, table_stride=1 << 28), dict(), "columns"),
+    (dict(page_size=128), dict(max_pages=(1 << 23) + 1, table_stride=1 << 24), dict(), "2^30"),
+    (dict(num_kv_heads=40000, page_size=16), dict(), dict(nq=80000), "65535"),
     (dict(), dict(table_stride=3), dict(), "table_stride"),
 ]
 
