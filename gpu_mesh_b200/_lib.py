@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -117,6 +118,7 @@ class Profile(ctypes.Structure):
 
 
 class PagedPool(ctypes.Structure):
+    _as_parameter_ = property(ctypes.byref)
     _fields_ = [
         ("k", _vp),
         ("v", _vp),
@@ -139,6 +141,7 @@ class PagedPool(ctypes.Structure):
 
 
 class PagedBatch(ctypes.Structure):
+    _as_parameter_ = property(ctypes.byref)
     _fields_ = [
         ("page_table", _vp),
         ("q_start", _vp),
@@ -149,6 +152,12 @@ class PagedBatch(ctypes.Structure):
         ("max_pages", _i32),
         ("max_new", _i32),
     ]
+
+
+# The same as bytes, which take a sixth of the time to make (0.15 against 0.85 us): a decode step makes both per call.
+PAGED_POOL = struct.Struct("4Q8q5i4x")
+PAGED_BATCH = struct.Struct("3Qq4i")
+assert PAGED_POOL.size == ctypes.sizeof(PagedPool) and PAGED_BATCH.size == ctypes.sizeof(PagedBatch)
 
 
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
@@ -251,7 +260,7 @@ SIGNATURES["mg_linear_noalloc"] = (
     ctypes.c_int,
     [_i32, _vp, _i64, _vp, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _i64, _vp],
 )
-_pool, _batch = ctypes.POINTER(PagedPool), ctypes.POINTER(PagedBatch)
+_pool = _batch = _vp  # a PagedPool, a PagedBatch, or either's bytes
 SIGNATURES["mg_paged_append"] = (
     ctypes.c_int,
     [_pool, _batch, _i32, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _f32, _vp, _i64, _vp],

@@ -106,45 +106,43 @@ def _refuse(x, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale) 
         raise ValueError("page_table, q_start and kv_len disagree on the number of sequences")
 
 
-def _paged(x, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale, max_new):
-    """The C structures of a pool and a batch, checked against the activations ``x``.
+def _paged(x, T, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale, max_new):
+    """The C structures of a pool and a batch as bytes, checked against the ``T`` rows of activations ``x``.
 
-    Decode steps call this twice per layer, so each tensor property is read once and the checks are one expression;
-    ``_refuse`` then names what it found."""
-    dev, kd, shape = x.device, k_pages.dtype, k_pages.shape
-    ks, vs = k_pages.stride(), v_pages.stride()
-    e4m3 = kd is torch.float8_e4m3fn
-    B = kv_len.shape[0] if kv_len.ndim == 1 else -1
-    if not (x.is_cuda and x.dtype in _DT and len(shape) == 4 and v_pages.shape == shape and v_pages.dtype is kd
-            and (e4m3 or kd is x.dtype) and k_pages.device == dev and v_pages.device == dev
+    Decode steps call this twice per layer, so each tensor property is read once and by its cheapest accessor, and
+    the checks are one expression; ``_refuse`` then names what it found."""
+    index, kd, shape = x.get_device(), k_pages.dtype, k_pages.shape
+    ks, vs, ts, table = k_pages.stride(), v_pages.stride(), page_table.stride(), page_table.shape
+    e4m3, i32, B = kd is torch.float8_e4m3fn, torch.int32, kv_len.numel()
+    if not (index >= 0 and x.dtype in _DT and len(shape) == 4 and v_pages.shape == shape and v_pages.dtype is kd
+            and (e4m3 or kd is x.dtype) and k_pages.get_device() == index and v_pages.get_device() == index
             and ks[3] == 1 and vs[3] == 1
-            and page_table.dtype is torch.int32 and q_start.dtype is torch.int32 and kv_len.dtype is torch.int32
-            and page_table.device == dev and q_start.device == dev and kv_len.device == dev
-            and page_table.ndim == 2 and page_table.shape[0] == B and page_table.stride(1) == 1
-            and q_start.shape == (B + 1,) and q_start.stride(0) == 1 and kv_len.stride(0) == 1):
+            and page_table.dtype is i32 and q_start.dtype is i32 and kv_len.dtype is i32
+            and page_table.get_device() == index and q_start.get_device() == index and kv_len.get_device() == index
+            and len(table) == 2 and table[0] == B and ts[1] == 1 and q_start.ndim == 1 and kv_len.ndim == 1
+            and q_start.numel() == B + 1 and q_start.is_contiguous() and kv_len.is_contiguous()):
         _refuse(x, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale)
     pages, nkv, ps, D = shape
+    kp = vp = kr = vr = 0
     if e4m3:
-        if not (k_scale is not None and v_scale is not None and k_scale.dtype is torch.float32
-                and v_scale.dtype is torch.float32 and k_scale.device == dev and v_scale.device == dev
-                and k_scale.shape == (pages, nkv) and v_scale.shape == (pages, nkv)
-                and k_scale.stride(1) == 1 and v_scale.stride(1) == 1):
+        good = k_scale is not None and v_scale is not None
+        if good:
+            rows, kst, vst = shape[:2], k_scale.stride(), v_scale.stride()
+            good = (k_scale.dtype is torch.float32 and v_scale.dtype is torch.float32 and k_scale.shape == rows
+                    and v_scale.shape == rows and kst[1] == 1 and vst[1] == 1
+                    and k_scale.get_device() == index and v_scale.get_device() == index)
+        if not good:
             _refuse(x, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale)
-        scales = (k_scale.data_ptr(), v_scale.data_ptr(), k_scale.stride(0), v_scale.stride(0))
-    else:
-        if k_scale is not None or v_scale is not None:
-            _refuse(x, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale)
-        scales = (None, None, 0, 0)
-    T = x.shape[0]
+        kp, vp, kr, vr = k_scale.data_ptr(), v_scale.data_ptr(), kst[0], vst[0]
+    elif k_scale is not None or v_scale is not None:
+        _refuse(x, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale)
     if max_new is None or max_new > T:
         max_new = T
     elif max_new < 0:
         raise ValueError("max_new must not be negative")
-    pool = _lib.PagedPool(k_pages.data_ptr(), v_pages.data_ptr(), scales[0], scales[1], ks[0], ks[1], ks[2],
-                          vs[0], vs[1], vs[2], scales[2], scales[3], pages, ps, nkv, D, _PAGED_DT[kd])
-    batch = _lib.PagedBatch(page_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), page_table.stride(0),
-                            B, T, page_table.shape[1], max_new)
-    return pool, batch
+    return _lib.PAGED_POOL.pack(k_pages.data_ptr(), v_pages.data_ptr(), kp, vp, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+                                kr, vr, pages, ps, nkv, D, _PAGED_DT[kd]), \
+        _lib.PAGED_BATCH.pack(page_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), ts[0], B, T, table[1], max_new)
 
 
 _HERE = contextlib.nullcontext()
@@ -175,12 +173,14 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     Rows behind ``q_start[-1]`` are left as they are in ``out``.  No two sequences of a call may append to one
     page: a page that sequences share is full, or copied first.
     """
-    pool, batch = _paged(qkv, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale, max_new)
-    dev, (_, nkv, _, D) = qkv.device, k_pages.shape
-    if qkv.ndim != 2 or num_q_heads < 1 or qkv.shape[1] != (num_q_heads + 2 * nkv) * D:
+    if qkv.ndim != 2:
         raise ValueError("qkv must be [T, (num_q_heads + 2 kv heads) * head_dim]")
-    T, (ld, inner) = qkv.shape[0], qkv.stride()
-    if inner != 1 and qkv.shape[1] > 1:
+    (T, width), (ld, inner) = qkv.shape, qkv.stride()
+    pool, batch = _paged(qkv, T, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale, max_new)
+    dev, (_, nkv, _, D) = qkv.device, k_pages.shape
+    if num_q_heads < 1 or width != (num_q_heads + 2 * nkv) * D:
+        raise ValueError("qkv must be [T, (num_q_heads + 2 kv heads) * head_dim]")
+    if inner != 1 and width > 1:
         raise ValueError("qkv rows must be contiguous")
     c = sn = qn = kn = pos = None
     max_pos = 0
@@ -195,7 +195,7 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         c, sn = cos.data_ptr(), sin.data_ptr()
     if q_norm is not None or k_norm is not None:
         for name, t in (("q_norm", q_norm), ("k_norm", k_norm)):
-            if t is not None and (t.dtype is not qkv.dtype or t.device != dev or t.shape != (D,) or t.stride(0) != 1):
+            if t is not None and (t.dtype is not qkv.dtype or t.device != dev or t.shape != (D,) or not t.is_contiguous()):
                 raise ValueError(f"{name} must be a contiguous [head_dim] tensor in the activation dtype")
         qn = None if q_norm is None else q_norm.data_ptr()
         kn = None if k_norm is None else k_norm.data_ptr()
@@ -204,16 +204,19 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
                 (T > 1 and positions.stride(0) != 1):
             raise ValueError("positions must be contiguous int64 with one entry per token row")
         pos = positions.data_ptr()
+    ldq = num_q_heads * D
     if out is None:
         out = qkv.new_empty((T, num_q_heads, D))
     elif out.shape != (T, num_q_heads, D) or out.dtype != qkv.dtype or out.device != dev or \
             out.stride(2) != 1 or (num_q_heads > 1 and out.stride(1) != D):
         raise ValueError("out must be [T, num_q_heads, head_dim] with contiguous token rows")
+    else:
+        ldq = out.stride(0)
     index = dev.index
     with _current(index):
         _lib.check(_lib.lib().mg_paged_append(
             pool, batch, _DT[qkv.dtype], qkv.data_ptr(), ld, num_q_heads, pos, c, sn, max_pos, qn, kn, eps,
-            out.data_ptr(), out.stride(0), _raw_stream(index)))
+            out.data_ptr(), ldq, _raw_stream(index)))
     return out
 
 
@@ -227,19 +230,19 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     0); ``scale`` defaults to head_dim ** -0.5.  Returns ``out`` (``[T, query heads, head_dim]``, not overlapping
     ``q``); rows behind ``q_start[-1]`` are left as they are in it.  The scratch is the call's own.
     """
-    if q.ndim != 3 or q.stride(2) != 1:
+    strides = q.stride()
+    if len(strides) != 3 or strides[2] != 1:
         raise ValueError("q must be [T, query heads, head_dim] with head_dim contiguous")
-    pool, batch = _paged(q, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale, max_new)
-    dev, nq = q.device, q.shape[1]
-    D = k_pages.shape[3]
-    if q.shape[2] != D:
+    T, nq, D = q.shape
+    pool, batch = _paged(q, T, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale, max_new)
+    if k_pages.shape[3] != D:
         raise ValueError("q and the pages disagree on head_dim")
     if out is None:
         out = torch.empty_like(q)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1:
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(2) != 1:
         raise ValueError("out must have q's shape and dtype, with head_dim contiguous")
-    lib, dt, index = _lib.lib(), _DT[q.dtype], dev.index
-    (ql, qh, _), (ol, oh, _) = q.stride(), out.stride()
+    lib, dt, index = _lib.lib(), _DT[q.dtype], q.get_device()
+    (ql, qh, _), (ol, oh, _) = strides, out.stride()
     with _current(index):
         need, ws = lib.mg_paged_attention_workspace(pool, batch, dt, nq), None
         if need:
