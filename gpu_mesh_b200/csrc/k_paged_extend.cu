@@ -400,7 +400,9 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
   float* srow = (float*)(smem + L::kOffRow);
   int* pre = (int*)(smem + L::kOffPre);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // By a shuffle, so that the compiler knows a role's branch to be the same for
+  // every lane (bf16 chunks on 5-8 K: 420 -> 411 us, e4m3: 518 -> 503 us).
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
       mbar_init(&kfull[s], 1);
