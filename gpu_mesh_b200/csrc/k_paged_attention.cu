@@ -230,36 +230,51 @@ __global__ void __launch_bounds__(kSimt) paged_attn_simt_kernel(const __grid_con
   }
 }
 
-// Join of the key ranges of one (new token, head), in their order: block
-// (x, head) the x % max_new-th new token of sequence x / max_new, a thread per dim.
+// Join of the key ranges of one (new token, head): block (x, head) the
+// x % max_new-th new token of sequence x / max_new, a thread per dim in each of
+// kJoinParts parts, which take every kJoinParts-th range in their order and
+// are then joined in theirs.
+constexpr int kJoinParts = 4;
+
 template <typename T, int D>
-__global__ void __launch_bounds__(D < 32 ? 32 : D) paged_attn_join_kernel(const __grid_constant__ PagedAttnArgs a, int splits) {
+__global__ void __launch_bounds__(kJoinParts * D) paged_attn_join_kernel(const __grid_constant__ PagedAttnArgs a, int splits) {
+  __shared__ float part[kJoinParts][D + 2];
   pdl_trigger();
   pdl_wait();
   const int most = max(a.batch.max_new, 1), b = blockIdx.x / most, s = blockIdx.x % most;
-  const int head = blockIdx.y, d = min((int)threadIdx.x, D - 1);
-  const SeqSpan span = seq_span(a.batch, b, a.pool.ps);  // on its way beside the parts
+  const int head = blockIdx.y, d = threadIdx.x % D, mine = threadIdx.x / D;
+  const SeqSpan span = seq_span(a.batch, b, a.pool.ps);  // on its way beside the ranges
   const float* w = (const float*)a.ws + ((part_row(a, b) + s) * a.nq + head) * splits * (D + 2);
   float M = -INFINITY, l = 0.f, o = 0.f;
-  for (int z0 = 0; z0 < splits; z0 += 8) {  // eight ranges' loads in flight
+  auto add = [&](float m, float sum, float v) {
+    if (sum == 0.f) return;  // it saw no key
+    const float top = fmaxf(M, m), keep = M == -INFINITY ? 0.f : exp2f(M - top), f = exp2f(m - top);
+    M = top;
+    l = l * keep + f * sum;
+    o = o * keep + f * v;
+  };
+  for (int z0 = mine; z0 < splits; z0 += 8 * kJoinParts) {  // eight ranges' loads in flight
     float m[8], sum[8], v[8];
 #pragma unroll
     for (int z = 0; z < 8; ++z) {
-      const float* q = w + min(z0 + z, splits - 1) * (D + 2);
+      const float* q = w + min(z0 + z * kJoinParts, splits - 1) * (D + 2);
       m[z] = __ldcg(q);
       sum[z] = __ldcg(q + 1);
       v[z] = __ldcg(q + 2 + d);
     }
 #pragma unroll
-    for (int z = 0; z < 8; ++z) {
-      if (z0 + z >= splits || sum[z] == 0.f) continue;  // none, or it saw no key
-      const float top = fmaxf(M, m[z]), keep = M == -INFINITY ? 0.f : exp2f(M - top), f = exp2f(m[z] - top);
-      M = top;
-      l = l * keep + f * sum[z];
-      o = o * keep + f * v[z];
-    }
+    for (int z = 0; z < 8; ++z)
+      if (z0 + z * kJoinParts < splits) add(m[z], sum[z], v[z]);
   }
-  if (s >= span.n || threadIdx.x >= D) return;
+  if (s >= span.n) return;  // (the same in the whole block)
+  part[mine][d] = o;
+  if (d == 0) {
+    part[mine][D] = M;
+    part[mine][D + 1] = l;
+  }
+  __syncthreads();
+  if (mine > 0) return;
+  for (int k = 1; k < kJoinParts; ++k) add(part[k][D], part[k][D + 1], part[k][d]);
   stf<T>((T*)a.out + (int64_t)(span.q0 + s) * a.ldo + (int64_t)head * a.hdo + d, l == 0.f ? 0.f : o / l);
 }
 
@@ -285,7 +300,7 @@ cudaError_t launch_simt_d(const PagedAttnArgs& a, cudaStream_t s) {
   cudaError_t e = launch_pdl(paged_attn_simt_kernel<T, C, D>, grid, dim3(kSimt), 0, s, a, (int)tiles, splits);
   if (e == cudaSuccess && splits > 1)
     e = launch_pdl(paged_attn_join_kernel<T, D>, dim3((unsigned)(a.batch.B * std::max(a.batch.max_new, 1)), (unsigned)a.nq),
-                   dim3(D < 32 ? 32 : D), 0, s, a, splits);
+                   dim3(kJoinParts * D), 0, s, a, splits);
   return e;
 }
 
