@@ -728,3 +728,15 @@ def test_padded_batch(dtype, cache):
     attend(c, [1, 1, 0, 0], lens, 4, extra=4094, max_new=1)
     attend(c, [1, 3, 0, 0], lens, 4, extra=600, max_new=8)
     run_append(c, [1, 1, 0, 0], lens, 4, extra=2000, max_new=1)
+
+
+@pytest.mark.parametrize("dtype,cache", [(BF16, BF16), (BF16, E4M3), (F32, E4M3)])
+@pytest.mark.parametrize("D,nkv,ps", [(8, 2, 16), (64, 3, 32), (128, 8, 16)])
+def test_append_two_to_four_tokens(dtype, cache, D, nkv, ps):
+    """A few tokens per sequence that cross a page's end, into pages whose scales grow."""
+    new = [4, 1, 3, 0, 2, 4]
+    past = [ps - 1, 0, ps - 3, 5, ps, 2 * ps - 2]
+    lens = [p + n for p, n in zip(past, new)]
+    c = Cache(lens, nkv, ps, D, dtype, cache, seed=D)
+    c.fill(past, spread=9)
+    run_append(c, new, lens, 2 * nkv, max_new=4, norm=True, extra=1)
