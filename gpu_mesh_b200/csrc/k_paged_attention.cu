@@ -13,7 +13,9 @@
 // the workspace and are joined in order by a second kernel.
 //
 // Bound: the fp32 FMA rate next to the shared-memory reads (each K and V
-// element read from memory once per 16 rows).
+// element read from memory once per 16 rows); in decode steps the round trips
+// of a CTA's few rounds.  Measured: 8 fp32 tokens on up to 2 K positions (32
+// query, 4 KV heads of 64) 25 us, chunks of up to 20 tokens on the same 100 us.
 #include <math.h>
 
 #include <algorithm>
@@ -282,7 +284,8 @@ int64_t simt_tiles(const PagedAttnArgs& a) {
   return ((int64_t)std::max(a.batch.max_new, 1) * (a.nq / a.pool.nkv) + kRows - 1) / kRows;
 }
 
-// Key ranges per row: enough CTAs for eight per SM, at least a round each.
+// Key ranges per row: enough CTAs for eight per SM, at least a round each (4, 6,
+// 8, 13 per SM: decode 26.4, 22.7, 24.8, 28.3 us, chunks 145, 117, 100, 90 us).
 int simt_splits(const PagedAttnArgs& a) {
   const int64_t ctas = a.batch.B * simt_tiles(a) * a.pool.nkv;
   const int64_t keys = (int64_t)a.batch.max_pages * a.pool.ps;

@@ -39,7 +39,16 @@
 // P is bf16 over bf16 pages (half a step: 2^-8 relative): the precision in
 // which the stage's own prefill multiplies the values.
 //
-// Bound: the MMA pipe and the exponentials, 4·D + 1 operations per score.
+// Bound: the chain of a tile, whose next score product goes over the P that
+// its value product reads: scores → softmax → value product → scores, some
+// 4,300 cycles per chunk with two tiles in flight (2,050 of them the
+// exponentials of both; the MMA pipe is 34 to 40 % busy).  Measured: chunks of
+// 700 to 1024 tokens on 5 to 8 K positions (4 sequences, 32 query, 8 KV heads
+// of 128) 411 us over bf16 pages, 830 TFLOP/s, 505 us over e4m3 ones; 8
+// prompts of 801 to 1024 (32 query, 4 KV heads of 64) 120 us.
+// Slower were steps of 64 keys with the next scores under the softmax (655 us
+// for the bf16 chunks: twice the issue and barrier work per key), an issuing
+// warp per tile (503 us), one softmax thread per row (553 us).
 // Every wait is bounded (code 3 in the error word on expiry); on expiry the
 // roles stop, issued loads and MMAs drain, and TMEM is freed.
 #include <math.h>

@@ -30,7 +30,8 @@ beside single tokens)::
 Page sizes 16, 32, 64 and 128, head sizes 8, 16, 32, 64 and 128, up to 16 query heads per KV head, 2048 sequences
 and 2^26 - 1 token rows per call.  bf16 with head sizes 64 and 128 runs attention on the tensor cores.
 
-The current stream runs the work, and nothing waits for it: what only the device can see (a page id outside the
+The current stream runs the work, and nothing waits for it (a call can be captured once one has run on its device
+outside a capture): what only the device can see (a page id outside the
 pool, a length outside the table) leaves that sequence out and is raised by ``paged_check_device``.
 """
 from __future__ import annotations
