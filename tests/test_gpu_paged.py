@@ -740,3 +740,57 @@ def test_append_two_to_four_tokens(dtype, cache, D, nkv, ps):
     c = Cache(lens, nkv, ps, D, dtype, cache, seed=D)
     c.fill(past, spread=9)
     run_append(c, new, lens, 2 * nkv, max_new=4, norm=True, extra=1)
+
+
+@pytest.mark.parametrize("dtype,cache", [(BF16, E4M3), (BF16, BF16), (F32, F32)])
+def test_captured_chunks_follow_the_device(dtype, cache):
+    """A captured batch of chunks and single tokens, replayed with other ranges, lengths and pages."""
+    lens = [700, 300, 64, 2000]
+    c = Cache(lens, 2, 16, 128, dtype, cache, seed=3)
+    c.fill(lens)
+    q = torch.randn(300, 8, 128, generator=torch.Generator().manual_seed(6)).to(dtype).to(DEV)
+    table, q_start, kv_len = c.table.to(DEV), dev32([0, 1, 2, 3, 4]), dev32([1, 1, 1, 1])
+    out = torch.full_like(q, 7.0)
+    graph = torch.cuda.CUDAGraph()
+    kernels.paged_attention(q, c.k, c.v, table, q_start, kv_len, max_new=200, **c.scales())
+    with torch.cuda.graph(graph):
+        kernels.paged_attention(q, c.k, c.v, table, q_start, kv_len, max_new=200, out=out, **c.scales())
+    for new, long, order in (([200, 1, 30, 9], lens, [0, 1, 2, 3]), ([1, 1, 1, 1], [5, 300, 64, 1999], [0, 1, 2, 3]),
+                             ([0, 150, 0, 150], [2000, 700, 300, 150], [3, 0, 1, 3])):
+        table.copy_(c.table[order])
+        q_start.copy_(dev32(starts(new)))
+        kv_len.copy_(dev32(long))
+        out.fill_(7.0)
+        graph.replay()
+        kernels.paged_check_device()
+        want = kernels.paged_attention(q, c.k, c.v, table, q_start, kv_len, max_new=200, out=torch.full_like(q, 7.0), **c.scales())
+        assert torch.equal(out, want) and (out[sum(new):] == 7.0).all()
+        t0, n = starts(new)[1], new[1]  # against the plain form: one sequence of them
+        k, v = (R.dense(*c.host()[key], c.table[order[1]], long[1]) for key in ("k", "v"))
+        ref, weight, top = R.attend(q[t0:t0 + n].cpu().double(), k, v, long[1] - n, 128**-0.5)
+        tol = R.attention_tolerance(ref, weight, top, 128, long[1], dtype, P_STEP[dtype], cache == E4M3 and dtype == BF16)
+        assert ((out[t0:t0 + n].cpu().double() - ref).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype,cache", [(BF16, E4M3), (BF16, BF16), (F32, E4M3)])
+def test_two_streams_at_once(dtype, cache):
+    """Appends and attention of two pools on two streams that run side by side."""
+    work, streams = [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for seed, (new, lens) in enumerate((([1, 90, 3], [900, 400, 33]), ([2, 1, 140], [50, 1500, 140]))):
+        c = Cache(lens, 2, 32, 64, dtype, cache, seed=seed)
+        c.fill([b - a for a, b in zip(new, lens)])
+        qkv = torch.randn(sum(new), 8 * 64, generator=torch.Generator().manual_seed(seed)).to(dtype).to(DEV)
+        args = (c.k, c.v, c.table.to(DEV), dev32(starts(new)), dev32(lens))
+        first = kernels.paged_append(qkv, *args, num_q_heads=4, **c.scales())  # the pages hold the tokens from here on
+        work.append((c, qkv, args, first, kernels.paged_attention(first, *args, **c.scales())))
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, (c, qkv, args, first, _) in enumerate(work):
+            with torch.cuda.stream(streams[i]):
+                got[i].append((kernels.paged_append(qkv, *args, num_q_heads=4, **c.scales()),
+                               kernels.paged_attention(first, *args, **c.scales())))
+    torch.cuda.synchronize()
+    kernels.paged_check_device()
+    for i, (_, _, _, first, want) in enumerate(work):
+        assert all(torch.equal(q, first) and torch.equal(out, want) for q, out in got[i])
