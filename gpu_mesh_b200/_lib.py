@@ -154,10 +154,50 @@ class PagedBatch(ctypes.Structure):
     ]
 
 
-# The same as bytes, which take a sixth of the time to make (0.15 against 0.85 us): a decode step makes both per call.
+class PagedAppendArgs(ctypes.Structure):
+    _as_parameter_ = property(ctypes.byref)
+    _fields_ = [
+        ("qkv", _vp),
+        ("positions", _vp),
+        ("cos", _vp),
+        ("sin", _vp),
+        ("q_norm", _vp),
+        ("k_norm", _vp),
+        ("q_out", _vp),
+        ("ld_qkv", _i64),
+        ("ld_q", _i64),
+        ("dtype", _i32),
+        ("num_q_heads", _i32),
+        ("max_pos", _i32),
+        ("eps", _f32),
+    ]
+
+
+class PagedAttentionArgs(ctypes.Structure):
+    _as_parameter_ = property(ctypes.byref)
+    _fields_ = [
+        ("q", _vp),
+        ("out", _vp),
+        ("workspace", _vp),
+        ("workspace_bytes", ctypes.c_uint64),
+        ("q_token_stride", _i64),
+        ("q_head_stride", _i64),
+        ("out_token_stride", _i64),
+        ("out_head_stride", _i64),
+        ("dtype", _i32),
+        ("num_q_heads", _i32),
+        ("scale", _f32),
+    ]
+
+
+# The same as bytes, which take a sixth of the time to make (a pool: 0.15 against 0.85 us): a decode step makes them
+# for every call.
 PAGED_POOL = struct.Struct("4Q8q5i4x")
 PAGED_BATCH = struct.Struct("3Qq4i")
-assert PAGED_POOL.size == ctypes.sizeof(PagedPool) and PAGED_BATCH.size == ctypes.sizeof(PagedBatch)
+PAGED_APPEND_ARGS = struct.Struct("7Q2q3if")
+PAGED_ATTENTION_ARGS = struct.Struct("4Q4q2if4x")
+assert [s.size for s in (PAGED_POOL, PAGED_BATCH, PAGED_APPEND_ARGS, PAGED_ATTENTION_ARGS)] == \
+    [ctypes.sizeof(c) for c in (PagedPool, PagedBatch, PagedAppendArgs, PagedAttentionArgs)]
 
 
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
@@ -260,14 +300,8 @@ SIGNATURES["mg_linear_noalloc"] = (
     ctypes.c_int,
     [_i32, _vp, _i64, _vp, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _i64, _vp],
 )
-_pool = _batch = _vp  # a PagedPool, a PagedBatch, or either's bytes
-SIGNATURES["mg_paged_append"] = (
-    ctypes.c_int,
-    [_pool, _batch, _i32, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _f32, _vp, _i64, _vp],
-)
-SIGNATURES["mg_paged_attention"] = (
-    ctypes.c_int,
-    [_pool, _batch, _i32, _vp, _i64, _i64, _i32, _f32, _vp, _i64, _i64, _vp, ctypes.c_uint64, _vp],
-)
-SIGNATURES["mg_paged_attention_workspace"] = (ctypes.c_uint64, [_pool, _batch, _i32, _i32])
+# Their structures come as such or as bytes.
+SIGNATURES["mg_paged_append"] = (ctypes.c_int, [_vp, _vp, _vp, _vp])
+SIGNATURES["mg_paged_attention"] = (ctypes.c_int, [_vp, _vp, _vp, _vp])
+SIGNATURES["mg_paged_attention_workspace"] = (ctypes.c_uint64, [_vp, _vp, _i32, _i32])
 SIGNATURES["mg_paged_check_device"] = (ctypes.c_int, [_vp])

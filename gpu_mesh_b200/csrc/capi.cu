@@ -1400,10 +1400,11 @@ int paged_args(const mg_paged_pool* p, const mg_paged_batch* b, int32_t dtype, i
 
 extern "C" {
 
-int mg_paged_append(const mg_paged_pool* pool, const mg_paged_batch* batch, int32_t dtype, const void* qkv,
-                    int64_t ld_qkv, int32_t num_q_heads, const int64_t* positions, const float* cos,
-                    const float* sin, int32_t max_pos, const void* q_norm, const void* k_norm, float eps,
-                    void* q_out, int64_t ld_q, void* stream) {
+int mg_paged_append(const mg_paged_pool* pool, const mg_paged_batch* batch, const mg_paged_append_args* args,
+                    void* stream) {
+  if (!args) return fail(MG_EINVAL, "null args");
+  const auto [qkv, positions, cos, sin, q_norm, k_norm, q_out, given_qkv, given_q, dtype, num_q_heads, max_pos, eps] = *args;
+  int64_t ld_qkv = given_qkv, ld_q = given_q;
   PagedAppendArgs a{};
   int rc = paged_args(pool, batch, dtype, num_q_heads, &a.pool, &a.batch);
   if (rc) return rc;
@@ -1446,10 +1447,11 @@ uint64_t mg_paged_attention_workspace(const mg_paged_pool* pool, const mg_paged_
   return paged_attention_workspace(a);
 }
 
-int mg_paged_attention(const mg_paged_pool* pool, const mg_paged_batch* batch, int32_t dtype, const void* q,
-                       int64_t q_token_stride, int64_t q_head_stride, int32_t num_q_heads, float scale, void* out,
-                       int64_t out_token_stride, int64_t out_head_stride, void* workspace, uint64_t workspace_bytes,
+int mg_paged_attention(const mg_paged_pool* pool, const mg_paged_batch* batch, const mg_paged_attention_args* args,
                        void* stream) {
+  if (!args) return fail(MG_EINVAL, "null args");
+  const auto [q, out, workspace, workspace_bytes, given_qt, given_qh, given_ot, given_oh, dtype, num_q_heads, scale] = *args;
+  int64_t q_token_stride = given_qt, q_head_stride = given_qh, out_token_stride = given_ot, out_head_stride = given_oh;
   PagedAttnArgs a{};
   int rc = paged_args(pool, batch, dtype, num_q_heads, &a.pool, &a.batch);
   if (rc) return rc;

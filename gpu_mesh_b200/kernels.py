@@ -183,8 +183,7 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         raise ValueError("qkv must be [T, (num_q_heads + 2 kv heads) * head_dim]")
     if inner != 1 and width > 1:
         raise ValueError("qkv rows must be contiguous")
-    c = sn = qn = kn = pos = None
-    max_pos = 0
+    c = sn = qn = kn = pos = max_pos = 0
     if cos is not None or sin is not None:
         if cos is None or sin is None:
             raise ValueError("cos and sin come together")
@@ -195,11 +194,13 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
             raise ValueError(f"cos and sin must be contiguous fp32 [positions, head_dim / 2] tables on {dev}")
         c, sn = cos.data_ptr(), sin.data_ptr()
     if q_norm is not None or k_norm is not None:
+        if not 0.0 < eps < 3.4e38:
+            raise ValueError("eps must be positive")
         for name, t in (("q_norm", q_norm), ("k_norm", k_norm)):
             if t is not None and (t.dtype is not qkv.dtype or t.device != dev or t.shape != (D,) or not t.is_contiguous()):
                 raise ValueError(f"{name} must be a contiguous [head_dim] tensor in the activation dtype")
-        qn = None if q_norm is None else q_norm.data_ptr()
-        kn = None if k_norm is None else k_norm.data_ptr()
+        qn = 0 if q_norm is None else q_norm.data_ptr()
+        kn = 0 if k_norm is None else k_norm.data_ptr()
     if positions is not None:
         if positions.dtype is not torch.int64 or positions.shape != (T,) or positions.device != dev or \
                 (T > 1 and positions.stride(0) != 1):
@@ -214,10 +215,10 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     else:
         ldq = out.stride(0)
     index = dev.index
+    args = _lib.PAGED_APPEND_ARGS.pack(qkv.data_ptr(), pos, c, sn, qn, kn, out.data_ptr(), ld, ldq, _DT[qkv.dtype],
+                                       num_q_heads, max_pos, eps)
     with _current(index):
-        _lib.check(_lib.lib().mg_paged_append(
-            pool, batch, _DT[qkv.dtype], qkv.data_ptr(), ld, num_q_heads, pos, c, sn, max_pos, qn, kn, eps,
-            out.data_ptr(), ldq, _raw_stream(index)))
+        _lib.check(_lib.lib().mg_paged_append(pool, batch, args, _raw_stream(index)))
     return out
 
 
@@ -242,16 +243,19 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         out = torch.empty_like(q)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(2) != 1:
         raise ValueError("out must have q's shape and dtype, with head_dim contiguous")
+    if scale is None:
+        scale = D ** -0.5
+    elif not 0.0 < scale < 3.4e38:
+        raise ValueError("scale must be positive and finite")
     lib, dt, index = _lib.lib(), _DT[q.dtype], q.get_device()
     (ql, qh, _), (ol, oh, _) = strides, out.stride()
     with _current(index):
-        need, ws = lib.mg_paged_attention_workspace(pool, batch, dt, nq), None
+        need, ws = lib.mg_paged_attention_workspace(pool, batch, dt, nq), 0
         if need:
             scratch = q.new_empty(need, dtype=torch.uint8)
             ws = scratch.data_ptr()
-        _lib.check(lib.mg_paged_attention(
-            pool, batch, dt, q.data_ptr(), ql, qh, nq, D ** -0.5 if scale is None else scale,
-            out.data_ptr(), ol, oh, ws, need, _raw_stream(index)))
+        args = _lib.PAGED_ATTENTION_ARGS.pack(q.data_ptr(), out.data_ptr(), ws, need, ql, qh, ol, oh, dt, nq, scale)
+        _lib.check(lib.mg_paged_attention(pool, batch, args, _raw_stream(index)))
     return out
 
 

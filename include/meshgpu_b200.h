@@ -363,6 +363,20 @@ typedef struct mg_paged_batch {
   int32_t max_new;   /* host bound: no sequence brings more new tokens */
 } mg_paged_batch;
 
+/* The token tensors of an append.  Optional ones are NULL. */
+typedef struct mg_paged_append_args {
+  const void* qkv;          /* [tokens, (num_q_heads + 2 num_kv_heads) head_dim], row stride ld_qkv */
+  const int64_t* positions; /* [tokens], optional */
+  const float* cos;         /* [max_pos, head_dim / 2], optional, as is sin */
+  const float* sin;
+  const void* q_norm;       /* [head_dim], optional */
+  const void* k_norm;
+  void* q_out;              /* [tokens, num_q_heads, head_dim], token stride ld_q */
+  int64_t ld_qkv, ld_q;
+  int32_t dtype, num_q_heads, max_pos;
+  float eps;
+} mg_paged_append_args;
+
 /* Append the batch's new tokens and rotate their queries: from the fused rows
  * qkv [tokens, (num_q_heads + 2 num_kv_heads) head_dim] (row stride ld_qkv),
  * q and k pass the optional per-head RMSNorm (q_norm / k_norm [head_dim],
@@ -378,22 +392,30 @@ typedef struct mg_paged_batch {
  * largest magnitude of its sign, NaN as NaN.  A position
  * outside the tables is clamped and reported.  Two sequences of a call must
  * not append to the same page. */
-int mg_paged_append(const mg_paged_pool* pool, const mg_paged_batch* batch, int32_t dtype, const void* qkv,
-                    int64_t ld_qkv, int32_t num_q_heads, const int64_t* positions, const float* cos,
-                    const float* sin, int32_t max_pos, const void* q_norm, const void* k_norm, float eps,
-                    void* q_out, int64_t ld_q, void* stream);
+int mg_paged_append(const mg_paged_pool* pool, const mg_paged_batch* batch, const mg_paged_append_args* args,
+                    void* stream);
+
+/* The token tensors [tokens, num_q_heads, head_dim] of an attention call
+ * (strides in elements, head_dim contiguous) and its scratch. */
+typedef struct mg_paged_attention_args {
+  const void* q;
+  void* out;
+  void* workspace;
+  uint64_t workspace_bytes;
+  int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+  int32_t dtype, num_q_heads;
+  float scale;
+} mg_paged_attention_args;
 
 /* out[t, h] = softmax over the visible keys of scale q[t, h]·K, times V, with
  * num_q_heads / num_kv_heads (at most 16) query heads per KV head (at most
  * 65535 in all).  The s-th
  * of n new tokens sees the keys j <= kv_len - n + s; a row without any gives
  * 0; an infinity or a NaN reaches the rows that see it alone.  q and out do
- * not overlap; their strides of tokens and heads are in elements.  `workspace` (device
+ * not overlap.  `workspace` (device
  * memory, 256-byte aligned, mg_paged_attention_workspace bytes) belongs to
  * the call until it has run on `stream`; it needs no initialisation. */
-int mg_paged_attention(const mg_paged_pool* pool, const mg_paged_batch* batch, int32_t dtype, const void* q,
-                       int64_t q_token_stride, int64_t q_head_stride, int32_t num_q_heads, float scale, void* out,
-                       int64_t out_token_stride, int64_t out_head_stride, void* workspace, uint64_t workspace_bytes,
+int mg_paged_attention(const mg_paged_pool* pool, const mg_paged_batch* batch, const mg_paged_attention_args* args,
                        void* stream);
 
 /* Workspace of mg_paged_attention for this pool and batch (0 where the

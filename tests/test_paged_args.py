@@ -28,12 +28,14 @@ def batch(**kw):
 
 def append(p, b, dtype=_lib.MG_DTYPE_BF16, qkv=BASE, ld=8 * 64, nq=4, cos=None, sin=None, max_pos=0, qn=None, eps=1e-6,
            out=BASE, ldq=4 * 64):
-    return _lib.lib().mg_paged_append(p, b, dtype, qkv, ld, nq, None, cos, sin, max_pos, qn, None, eps, out, ldq, None)
+    args = _lib.PagedAppendArgs(qkv, None, cos, sin, qn, None, out, ld, ldq, dtype, nq, max_pos, eps)
+    return _lib.lib().mg_paged_append(p, b, args, None)
 
 
 def attend(p, b, dtype=_lib.MG_DTYPE_BF16, q=BASE, qs=(256, 64), nq=4, scale=0.125, out=BASE, os=(256, 64), ws=BASE,
            nbytes=1 << 40):
-    return _lib.lib().mg_paged_attention(p, b, dtype, q, *qs, nq, scale, out, *os, ws, nbytes, None)
+    args = _lib.PagedAttentionArgs(q, out, ws, nbytes, *qs, *os, dtype, nq, scale)
+    return _lib.lib().mg_paged_attention(p, b, args, None)
 
 
 SHARED = [
@@ -102,6 +104,8 @@ def test_null_structures_and_empty_batches():
     assert attend(null_pool, batch()) == _lib.MG_EINVAL
     assert append(pool(), null_batch) == _lib.MG_EINVAL
     assert lib.mg_paged_attention_workspace(null_pool, null_batch, 1, 4) == 0
+    assert lib.mg_paged_append(pool(), batch(), None, None) == _lib.MG_EINVAL
+    assert lib.mg_paged_attention(pool(), batch(), None, None) == _lib.MG_EINVAL
     for b in (batch(batch=0), batch(tokens=0)):  # nothing to do, and nothing touched
         assert append(pool(), b) == _lib.MG_OK
         assert attend(pool(), b) == _lib.MG_OK
