@@ -6,16 +6,19 @@
 // for the s-th new token t of a sequence with `past` tokens before; a row
 // that sees no key gives 0.
 //
-// A CTA takes 16 query rows ((token, head) pairs that share a KV head) and a
-// range of keys, 32 keys at a time through shared memory in fp32, with the
-// running maximum and sum of the softmax in base 2.  Where the rows alone do
-// not fill the GPU the keys are cut into ranges, whose (max, sum, O) go to
-// the workspace and are joined in order by a second kernel.
+// A CTA takes 16 query rows ((token, head) pairs that share a KV head; 8 or 4
+// where no sequence has more) and a range of keys, 32 keys at a time through
+// shared memory in fp32, with the running maximum and sum of the softmax in
+// base 2.  Where the rows alone do not fill the GPU the keys are cut into
+// ranges, whose (max, sum, O) go to the workspace and are joined in order by a
+// second kernel.
 //
 // Bound: the fp32 FMA rate next to the shared-memory reads (each K and V
-// element read from memory once per 16 rows); in decode steps the round trips
-// of a CTA's few rounds.  Measured: 8 fp32 tokens on up to 2 K positions (32
-// query, 4 KV heads of 64) 25 us, chunks of up to 20 tokens on the same 100 us.
+// element read from memory once per CTA's rows); in decode steps the round
+// trips of a CTA's few rounds.  Measured: 8 fp32 tokens on up to 2 K positions
+// (32 query, 4 KV heads of 64) 18.6 us, 24.8 with 16 rows to a CTA; 16 tokens
+// with 8 KV heads 31 us = 2.0 TB/s, 57 with 16 rows; chunks of up to 20 tokens
+// on the same lengths 88 us.
 #include <math.h>
 
 #include <algorithm>
@@ -26,7 +29,7 @@
 namespace mg {
 namespace {
 
-constexpr int kRows = 16;     // query rows of a CTA
+constexpr int kRows = 16;     // most query rows of a CTA
 constexpr int kKeys = 32;     // keys of a round
 constexpr int kSimt = 128;    // threads
 constexpr int kMaxSplits = 64;
@@ -64,16 +67,19 @@ struct Cached<uint8_t> {
 // padded batch may have many more.
 __device__ __forceinline__ int64_t part_row(const PagedAttnArgs& a, int b) { return (int64_t)b * max(a.batch.max_new, 1); }
 
-template <typename T, typename C, int D>
+template <typename T, typename C, int D, int ROWS>
 __global__ void __launch_bounds__(kSimt) paged_attn_simt_kernel(const __grid_constant__ PagedAttnArgs a, int tiles, int splits) {
-  constexpr int RPT = kRows * D / kSimt;          // output rows of a thread
+  constexpr int RPT = ROWS * D / kSimt;           // output rows of a thread
+  constexpr int TPR = kSimt / ROWS;                // threads of a query row
+  constexpr int KPT = kKeys / TPR;                 // keys of a thread in a round
+  static_assert(RPT >= 1 && TPR <= 32, "a query row lies in a warp");
   constexpr int P4 = Cached<C>::N;
   // Rows 4 floats apart in the banks: eight keys' 16-byte reads do not collide.
-  __shared__ __align__(16) float sq[kRows][D + 4];
+  __shared__ __align__(16) float sq[ROWS][D + 4];
   __shared__ __align__(16) float sk[kKeys][D + 4];
   __shared__ __align__(16) float sv[kKeys][D];
-  __shared__ __align__(16) float sp[kRows][kKeys];
-  __shared__ float keep[kRows], sum[kRows], top[kRows];
+  __shared__ __align__(16) float sp[ROWS][kKeys];
+  __shared__ float keep[ROWS], sum[ROWS], top[ROWS];
   pdl_trigger();
   pdl_wait();
   const PagedPool& pool = a.pool;
@@ -86,15 +92,15 @@ __global__ void __launch_bounds__(kSimt) paged_attn_simt_kernel(const __grid_con
     if (tid == 0) flag_error(a.err, kErrPaged);
     return;
   }
-  const int rows = span.n * G, r0 = tile * kRows;
+  const int rows = span.n * G, r0 = tile * ROWS;
   if (r0 >= rows) return;
-  const int nr = min(kRows, rows - r0);
+  const int nr = min(ROWS, rows - r0);
   const int most = min(span.past + (r0 + nr - 1) / G + 1, span.past + span.n);  // keys the last row sees
   const int step = most > 0 ? (int)(((long long)(most + kKeys - 1) / kKeys + splits - 1) / splits) * kKeys : 0;
   const long long first = (long long)z * step;
   const int k_lo = (int)min(first, (long long)max(most, 0)), k_hi = (int)min(first + step, (long long)max(most, 0));
 
-  for (int i = tid; i < kRows * D; i += kSimt) {
+  for (int i = tid; i < ROWS * D; i += kSimt) {
     const int r = i / D, d = i % D;
     float x = 0.f;
     if (r < nr)
@@ -102,9 +108,9 @@ __global__ void __launch_bounds__(kSimt) paged_attn_simt_kernel(const __grid_con
     sq[r][d] = x;
   }
   const float scale2 = a.scale * 1.4426950408889634f;
-  const int qr = tid / 8, kq = tid % 8;                   // score row, first key
+  const int qr = tid / TPR, kq = tid % TPR;               // score row, first key
   const int vis = qr < nr ? span.past + (r0 + qr) / G + 1 : 0;
-  float m = -INFINITY, l = 0.f;                           // of row qr (the same in its 8 threads)
+  float m = -INFINITY, l = 0.f;                           // of row qr (the same in its threads)
   const int od = tid % D, og = tid / D;                   // output dim, first output row / RPT
   float acc[RPT];
 #pragma unroll
@@ -162,33 +168,35 @@ __global__ void __launch_bounds__(kSimt) paged_attn_simt_kernel(const __grid_con
       request(k0 + kKeys);
       look_up(k0 + 2 * kKeys);
     }
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    float s[KPT];
+#pragma unroll
+    for (int i = 0; i < KPT; ++i) s[i] = 0.f;
     for (int d = 0; d < D; d += 4) {
       const float4 x = *reinterpret_cast<const float4*>(&sq[qr][d]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float4 y = *reinterpret_cast<const float4*>(&sk[kq + 8 * i][d]);
+      for (int i = 0; i < KPT; ++i) {
+        const float4 y = *reinterpret_cast<const float4*>(&sk[kq + TPR * i][d]);
         s[i] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, s[i]))));
       }
     }
     float mx = m;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      s[i] = k0 + kq + 8 * i < vis ? s[i] * scale2 : -INFINITY;
+    for (int i = 0; i < KPT; ++i) {
+      s[i] = k0 + kq + TPR * i < vis ? s[i] * scale2 : -INFINITY;
       mx = fmaxf(mx, s[i]);
     }
 #pragma unroll
-    for (int o = 4; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    for (int o = TPR / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     const float alpha = m == -INFINITY ? 0.f : exp2f(m - mx);
     float part = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < KPT; ++i) {
       const float p = s[i] == -INFINITY ? 0.f : exp2f(s[i] - mx);
-      sp[qr][kq + 8 * i] = p;
+      sp[qr][kq + TPR * i] = p;
       part += p;
     }
 #pragma unroll
-    for (int o = 4; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+    for (int o = TPR / 2; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
     m = mx;
     l = l * alpha + part;
     if (kq == 0) keep[qr] = alpha;
@@ -280,16 +288,17 @@ __global__ void __launch_bounds__(kJoinParts * D) paged_attn_join_kernel(const _
   stf<T>((T*)a.out + (int64_t)(span.q0 + s) * a.ldo + (int64_t)head * a.hdo + d, l == 0.f ? 0.f : o / l);
 }
 
-int64_t simt_tiles(const PagedAttnArgs& a) {
-  return ((int64_t)std::max(a.batch.max_new, 1) * (a.nq / a.pool.nkv) + kRows - 1) / kRows;
-}
+int64_t most_rows(const PagedAttnArgs& a) { return (int64_t)std::max(a.batch.max_new, 1) * (a.nq / a.pool.nkv); }
+int64_t simt_tiles(const PagedAttnArgs& a) { return (most_rows(a) + kRows - 1) / kRows; }
 
-// Key ranges per row: enough CTAs for eight per SM, at least a round each (4, 6,
-// 8, 13 per SM: decode 26.4, 22.7, 24.8, 28.3 us, chunks 145, 117, 100, 90 us).
+// Key ranges per row: enough CTAs for nine per SM, at least a round each (with
+// 16 rows to a CTA and 4, 6, 8, 9, 10, 13 per SM: 8 tokens 26.4, 22.7, 24.8,
+// 24.8, 24.8, 28.3 us, chunks of up to 20 tokens 145, 117, 98, 88, 88, 90 us, of
+// up to 60 at 8, 9, 10: 137, 137, 148 us).
 int simt_splits(const PagedAttnArgs& a) {
   const int64_t ctas = a.batch.B * simt_tiles(a) * a.pool.nkv;
   const int64_t keys = (int64_t)a.batch.max_pages * a.pool.ps;
-  int64_t n = ctas > 0 ? (8LL * usable_sms() + ctas - 1) / ctas : 1;
+  int64_t n = ctas > 0 ? (9LL * usable_sms() + ctas - 1) / ctas : 1;
   n = std::min<int64_t>(n, (keys + kKeys - 1) / kKeys);
   return (int)std::max<int64_t>(1, std::min<int64_t>(n, kMaxSplits));
 }
@@ -300,7 +309,12 @@ cudaError_t launch_simt_d(const PagedAttnArgs& a, cudaStream_t s) {
   const int splits = simt_splits(a);
   if (ctas > INT32_MAX) return cudaErrorInvalidConfiguration;  // (B · max_new beyond any batch that fits the GPU)
   const dim3 grid((unsigned)ctas, (unsigned)a.pool.nkv, (unsigned)splits);
-  cudaError_t e = launch_pdl(paged_attn_simt_kernel<T, C, D>, grid, dim3(kSimt), 0, s, a, (int)tiles, splits);
+  // A CTA's rows: no more than a sequence has, but a thread owns at least one output.
+  constexpr int few = 4 < kSimt / D ? kSimt / D : 4, some = 8 < kSimt / D ? kSimt / D : 8;
+  const int64_t rows = most_rows(a);
+  auto kernel = rows <= few ? paged_attn_simt_kernel<T, C, D, few>
+                : rows <= some ? paged_attn_simt_kernel<T, C, D, some> : paged_attn_simt_kernel<T, C, D, kRows>;
+  cudaError_t e = launch_pdl(kernel, grid, dim3(kSimt), 0, s, a, (int)tiles, splits);
   if (e == cudaSuccess && splits > 1)
     e = launch_pdl(paged_attn_join_kernel<T, D>, dim3((unsigned)(a.batch.B * std::max(a.batch.max_new, 1)), (unsigned)a.nq),
                    dim3(kJoinParts * D), 0, s, a, splits);
