@@ -73,6 +73,12 @@ __device__ __forceinline__ int decode_blocks(const SeqSpan& s, int G, int bk) {
 // 5 K with 2 to 4 tokens 49.2, 49.6, 43.7, 46.5 us; the others within 4 %.
 constexpr int kSnap = 8;
 
+// Blocks of a CTA's run at least, where there are few: its warps take one each,
+// and the pieces to join get fewer (2 sequences of up to 1.2 K positions, 5
+// tokens, 2 KV heads: 22.6 us, with runs of one block 29.1; runs of eight take
+// one token on 130 positions from 8.5 to 11.4 us).
+constexpr int kLeast = 4;
+
 // What a CTA leaves for the join: the (sequence, head) that its run ends and
 // earlier ones began, as its first token row, KV head, query rows (0: there
 // is none) and number of pieces, this run's the last.
@@ -163,7 +169,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
     }
   }
   __syncthreads();
-  const int total = pre[bt.B], c = blockIdx.x, grid = min((int)gridDim.x, total);
+  const int total = pre[bt.B], c = blockIdx.x, grid = min((int)gridDim.x, (total + kLeast - 1) / kLeast);
   auto seq_of = [&](int u) {
     int lo = 0, hi = bt.B;  // pre[lo] <= u < pre[hi]
     while (hi - lo > 1) {
@@ -337,7 +343,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
   int rows = 0, least = 0, from = 0, vis[NT][2];
   float mrow[NT][2], lrow[NT][2], rowf[NT][2];
   float o[NT][DM][4];
-  uint32_t qb[KS][2];  // of the only tile
+  uint32_t qb[KS][2] = {};  // of the only tile
   auto query = [&](int nt, int ks) {  // the B fragment of k-step ks
     if constexpr (kQShared) return qs[warp][nt * KS + ks][lane];
     return make_uint2(qb[ks][0], qb[ks][1]);

@@ -666,7 +666,7 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
             o[e] *= f;
             bad |= o[e] != o[e];
           }
-          if (!w.whole) {
+          if (!w.whole && valid) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
               *reinterpret_cast<float4*>(part + (size_t)row * D + d0 + 4 * e) =
@@ -680,7 +680,7 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
           }
         }
         if (w.whole && valid && bad) *redo = 1;
-        if (!w.whole && hf == 0) {
+        if (!w.whole && valid && hf == 0) {
           part[2 * kTile * D + row] = m;
           part[2 * kTile * D + 2 * kTile + row] = l;
         }
