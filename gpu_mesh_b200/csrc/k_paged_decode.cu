@@ -134,6 +134,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
+  // This grid may be resident while the append before it writes pages, scales
+  // and tables: everything is read behind this wait by ordinary loads, as the
+  // non-coherent ones are for data that nothing writes in a kernel's lifetime.
   pdl_wait();
   for (int b = tid; b < bt.B; b += kWarps * 32) {
     const SeqSpan s = seq_span(bt, b, pool.ps);
@@ -230,7 +233,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
     fresh = false;
 #pragma unroll
     for (int i = 0; i < SUB; ++i)
-      x.page[i] = x.k0 + 16 * i < x.len ? __ldg(ctab + ((x.k0 + 16 * i) >> page_shift)) : -1;
+      x.page[i] = x.k0 + 16 * i < x.len ? ctab[(x.k0 + 16 * i) >> page_shift] : -1;
     ++cu;
     if (++cblk == cnb && cu < u1) {
       cblk = 0;
@@ -295,8 +298,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
             kx[i][r][p] = page >= 0 && k0 + g + 8 * r < x.len ? load_once(kp + r * k8 + 64 * p) : make_uint4(0u, 0u, 0u, 0u);
       }
       if constexpr (E4) {
-        ks[i] = page >= 0 ? __ldg(pool.ks + page * pool.kse + x.h) : 0.f;
-        vs[i] = page >= 0 ? __ldg(pool.vs + page * pool.vse + x.h) : 1.f;
+        ks[i] = page >= 0 ? pool.ks[page * pool.kse + x.h] : 0.f;
+        vs[i] = page >= 0 ? pool.vs[page * pool.vse + x.h] : 1.f;
       }
     }
     if (!kQShared && x.valid && x.first) load_q(x, 0, qx);
