@@ -61,17 +61,27 @@ namespace mg {
 
 std::atomic<int> g_reserved_sms[64];
 
-int usable_sms() {
+static int sms_of(int dev) {
   static int full[64] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return 148;
   if (!full[dev]) {
     int v = 0;
     cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev);
     full[dev] = v > 0 ? v : 148;
   }
-  const int n = full[dev] - g_reserved_sms[dev].load();
+  return full[dev];
+}
+
+int device_sms() {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  return sms_of(dev);
+}
+
+int usable_sms() {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const int n = sms_of(dev) - (dev >= 0 && dev < 64 ? g_reserved_sms[dev].load() : 0);
   return n > 1 ? n : 1;
 }
 
@@ -1444,6 +1454,7 @@ uint64_t mg_paged_attention_workspace(const mg_paged_pool* pool, const mg_paged_
   if (paged_args(pool, batch, dtype, num_q_heads, &a.pool, &a.batch) || a.batch.B == 0 || a.batch.T == 0) return 0;
   a.dtype = dtype;
   a.nq = num_q_heads;
+  a.sms = device_sms();
   return paged_attention_workspace(a);
 }
 
@@ -1467,7 +1478,12 @@ int mg_paged_attention(const mg_paged_pool* pool, const mg_paged_batch* batch, c
   if (!aligned16(q) || !aligned16(out)) return fail(MG_EINVAL, "q and out must start on 16-byte boundaries");
   a.dtype = dtype;
   a.nq = num_q_heads;
+  // Sized for the whole device, so that no change of the reservation between
+  // the caller's query, this check and the launches outgrows it; the launches
+  // and their offsets share one reading.
+  a.sms = device_sms();
   const uint64_t need = paged_attention_workspace(a);
+  a.sms = std::min(usable_sms(), a.sms);
   if (workspace_bytes < need || (need && (!workspace || (uintptr_t)workspace % 256)))
     return fail(MG_EINVAL, "the workspace must be 256-byte aligned and hold %llu bytes", (unsigned long long)need);
   rc = paged_err_word(stream, &a.err);

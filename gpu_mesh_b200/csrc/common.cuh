@@ -133,7 +133,10 @@ __device__ __forceinline__ float hist_value(uint32_t b) {
 
 // Streaming multiprocessors a persistent kernel spreads over on the current
 // device: the device's count minus the SMs left free for concurrent work
-// (NCCL's kernels in a multi-process pipeline; mg_reserve_sms).  Host code.
+// (NCCL's kernels in a multi-process pipeline; mg_reserve_sms), and that count
+// itself.  Host code.  Another thread may change the reservation between two
+// calls of usable_sms: what must agree is derived from one.
 int usable_sms();
+int device_sms();
 
 }  // namespace mg

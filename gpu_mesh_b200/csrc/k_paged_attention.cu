@@ -298,7 +298,7 @@ int64_t simt_tiles(const PagedAttnArgs& a) { return (most_rows(a) + kRows - 1) /
 int simt_splits(const PagedAttnArgs& a) {
   const int64_t ctas = a.batch.B * simt_tiles(a) * a.pool.nkv;
   const int64_t keys = (int64_t)a.batch.max_pages * a.pool.ps;
-  int64_t n = ctas > 0 ? (9LL * usable_sms() + ctas - 1) / ctas : 1;
+  int64_t n = ctas > 0 ? (9LL * a.sms + ctas - 1) / ctas : 1;
   n = std::min<int64_t>(n, (keys + kKeys - 1) / kKeys);
   return (int)std::max<int64_t>(1, std::min<int64_t>(n, kMaxSplits));
 }

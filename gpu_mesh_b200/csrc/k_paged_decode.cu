@@ -741,7 +741,7 @@ cudaError_t launch_decode(const PagedAttnArgs& a, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
-  const int rows = row_cap(a), grid = usable_sms();
+  const int rows = row_cap(a), grid = a.sms;
   PagedAttnArgs args = a;
   if (!may_cut(a)) args.ws = nullptr;
   cudaError_t e = launch_pdl(kernel, dim3(grid), dim3(kWarps * 32), bytes(rows, a.batch.B), s, args, rows);
@@ -758,7 +758,7 @@ bool paged_decode_applicable(const PagedAttnArgs& a) {
 
 size_t paged_decode_workspace(const PagedAttnArgs& a) {
   if (!may_cut(a)) return 0;
-  return (size_t)usable_sms() * (2 * piece_floats(row_cap(a), a.pool.D) * sizeof(float) + sizeof(Cut));
+  return (size_t)a.sms * (2 * piece_floats(row_cap(a), a.pool.D) * sizeof(float) + sizeof(Cut));
 }
 
 cudaError_t launch_paged_decode(const PagedAttnArgs& a, cudaStream_t s) {

@@ -1037,8 +1037,6 @@ __global__ void __launch_bounds__(256) paged_extend_join_kernel(const __grid_con
   }
 }
 
-int extend_grid() { return usable_sms(); }
-
 template <int D, bool E4>
 cudaError_t launch_extend(const PagedAttnArgs& a, cudaStream_t s) {
   PoolMaps maps{};
@@ -1065,7 +1063,7 @@ cudaError_t launch_extend(const PagedAttnArgs& a, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
-  const int grid = extend_grid();
+  const int grid = a.sms;
   cudaError_t e = launch_pdl(kernel, dim3(grid), dim3(Roles<E4>::kThreads), ExtendLayout<D, E4>::bytes(a.batch.B), s, maps,
                              tq_map, a);
   if (e != cudaSuccess) return e;
@@ -1075,7 +1073,7 @@ cudaError_t launch_extend(const PagedAttnArgs& a, cudaStream_t s) {
 }  // namespace
 
 size_t paged_extend_workspace(const PagedAttnArgs& a) {
-  return (size_t)extend_grid() * (2 * (a.pool.D == 128 ? partial_floats<128>() : partial_floats<64>()) * sizeof(float) + sizeof(CutItem));
+  return (size_t)a.sms * (2 * (a.pool.D == 128 ? partial_floats<128>() : partial_floats<64>()) * sizeof(float) + sizeof(CutItem));
 }
 
 cudaError_t launch_paged_extend(const PagedAttnArgs& a, cudaStream_t s) {

@@ -74,6 +74,7 @@ struct PagedAttnArgs {
   void* ws;
   size_t ws_bytes;
   int* err;
+  int sms;  // CTAs of the persistent kernels, read once per call: workspace, offsets and grids follow it
 };
 size_t paged_attention_workspace(const PagedAttnArgs& a);
 

@@ -420,7 +420,8 @@ int mg_paged_attention(const mg_paged_pool* pool, const mg_paged_batch* batch, c
 
 /* Workspace of mg_paged_attention for this pool and batch (0 where the
  * arguments are invalid; the call itself says why).  It depends on the sizes
- * and on mg_reserve_sms alone, not on the lengths on the device. */
+ * and the current device alone, not on the lengths on the device nor on
+ * mg_reserve_sms, which may change between this query and the call. */
 uint64_t mg_paged_attention_workspace(const mg_paged_pool* pool, const mg_paged_batch* batch, int32_t dtype,
                                       int32_t num_q_heads);
 

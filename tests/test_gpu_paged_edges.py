@@ -2,12 +2,14 @@
 not reach.  Reference, tolerances and pools as in ``test_gpu_paged``."""
 from __future__ import annotations
 
+import threading
+
 import pytest
 import torch
 
-from gpu_mesh_b200 import kernels
+from gpu_mesh_b200 import _lib, kernels
 from tests import paged_ref as R
-from tests.test_gpu_paged import BF16, DEV, E4M3, P_STEP, Cache, check_append, dev32, starts, tables
+from tests.test_gpu_paged import BF16, DEV, E4M3, F32, P_STEP, Cache, check_append, dev32, starts, tables
 
 pytestmark = pytest.mark.gpu
 
@@ -70,3 +72,80 @@ def test_attention_directly_behind_an_append(nkv, n):
             tol += half_floor(q[t0:t0 + n].cpu().double(), k, v, key_scales(c, pools["v"][1], b, lens[b]), gone, D**-0.5,
                               14 if n * nq // nkv <= 16 else 7)
             assert ((out[t0:t0 + n].cpu().double() - ref).abs() <= tol).all(), (i, b)
+
+
+def workspace_and_call(c, q, out, q_start, kv_len, max_new, between):
+    """``kernels.paged_attention`` by the C ABI, with ``between()`` between the workspace's query and the call."""
+    lib, table = _lib.lib(), c.table.to(DEV)
+    ks, vs, e4m3 = c.k.stride(), c.v.stride(), c.cache == E4M3
+    dt = {BF16: _lib.MG_DTYPE_BF16, F32: _lib.MG_DTYPE_F32}[c.dtype]
+    pool = _lib.PagedPool(c.k.data_ptr(), c.v.data_ptr(), c.ks.data_ptr() if e4m3 else None, c.vs.data_ptr() if e4m3 else None,
+                          *ks[:3], *vs[:3], c.ks.stride(0) if e4m3 else 0, c.vs.stride(0) if e4m3 else 0, c.pages, c.ps, c.nkv,
+                          c.D, _lib.MG_DTYPE_E4M3 if e4m3 else dt)
+    batch = _lib.PagedBatch(table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), table.stride(0), len(c.table), len(q),
+                            table.shape[1], max_new)
+    need = lib.mg_paged_attention_workspace(pool, batch, dt, q.shape[1])
+    ws = torch.empty(need, dtype=torch.uint8, device=DEV)
+    between()
+    args = _lib.PagedAttentionArgs(q.data_ptr(), out.data_ptr(), ws.data_ptr(), need, *q.stride()[:2], *out.stride()[:2], dt,
+                                   q.shape[1], c.D**-0.5)
+    _lib.check(lib.mg_paged_attention(pool, batch, args, torch.cuda.current_stream().cuda_stream))
+    return need
+
+
+@pytest.mark.parametrize("dtype,cache", [(BF16, BF16), (BF16, E4M3), (F32, F32)])
+def test_workspace_does_not_follow_reserved_sms(dtype, cache):
+    """SMs that are reserved, or given back, between the query of the workspace and the call."""
+    lens, new = [3000, 1, 777, 200], [1, 1, 1, 90]
+    c = Cache(lens, 2, 16, 64, dtype, cache)
+    c.fill(lens)
+    q = torch.randn(sum(new), 8, 64, generator=torch.Generator().manual_seed(1)).to(dtype).to(DEV)
+    reserve = lambda n: _lib.check(_lib.lib().mg_reserve_sms(0, n))  # noqa: E731
+    rows = {n: (q[:sum(n)], dev32(starts(n)), dev32(lens), max(n)) for n in ((1, 1, 1, 1), tuple(new))}
+    pools, good, sizes = c.host(), {}, {}
+    for n in rows:
+        good[n] = []
+        for b, (t0, m, past) in enumerate(R.spans(starts(n), lens)):
+            x = q[t0:t0 + m].cpu().double()
+            k, v = (R.dense(*pools[key], c.table[b], lens[b]) for key in ("k", "v"))
+            ref, weight, top = R.attend(x, k, v, past, 64**-0.5)
+            tol = R.attention_tolerance(ref, weight, top, 64, lens[b], dtype, P_STEP[dtype], cache == E4M3)
+            if cache == E4M3:
+                tol += half_floor(x, k, v, key_scales(c, pools["v"][1], b, lens[b]), past, 64**-0.5, 14 if 4 * m <= 16 else 7)
+            good[n].append((ref, tol))
+
+    def check(out, n):
+        ref, tol = (torch.cat(x) for x in zip(*good[n]))
+        assert ((out.cpu().double() - ref).abs() <= tol).all()
+
+    try:
+        for n, (x, s, m, most) in rows.items():
+            sizes[n] = set()
+            for before, after in ((0, 0), (70, 0), (0, 70), (70, 16)):
+                reserve(before)
+                out = torch.empty_like(x)
+                sizes[n].add(workspace_and_call(c, x, out, s, m, most, lambda: reserve(after)))
+                check(out, n)
+        assert all(len(s) == 1 for s in sizes.values())
+        # The wrapper, with another thread that changes the reservation all the time.
+        stop = threading.Event()
+
+        def toggle():
+            i = 0
+            while not stop.is_set():
+                reserve((0, 70, 5)[i % 3])
+                i += 1
+
+        t = threading.Thread(target=toggle)
+        t.start()
+        try:
+            got = [(n, kernels.paged_attention(x, c.k, c.v, c.table.to(DEV), s, m, max_new=most, **c.scales()))
+                   for _ in range(100) for n, (x, s, m, most) in rows.items()]
+        finally:
+            stop.set()
+            t.join()
+        for n, out in got:
+            check(out, n)
+    finally:
+        reserve(0)
+    kernels.paged_check_device()
