@@ -29,8 +29,9 @@
 //       scaled by a power of two per row (exact), K's scale multiplies the
 //       fp32 scores.  V's scale 2^e goes into the exponent: with the running
 //       maximum m of s + e, P' = 2^(s + e - m + 14) (rounded to half: 2^-11
-//       relative, down to 2^-28 of the largest) weighs the raw codes, while
-//       the sum adds P'·2^(-e - 14) = 2^(s - m) in fp32; out = O / l · 2^-14.
+//       relative, down to 2^-28 of the largest, and within 2^-39 of it below)
+//       weighs the raw codes, while the sum adds P'·2^(-e - 14) = 2^(s - m) in
+//       fp32 (scales far apart: odd_exp); out = O / l · 2^-14.
 //
 // Measured (32 query, 8 KV heads of 128): 64 tokens on 7.9 to 8.2 K positions,
 // e4m3, 204 us = 5.2 TB/s; 32 tokens, bf16, 182 us = 5.8 TB/s (a copy runs at
@@ -81,14 +82,16 @@ constexpr int kLeast = 4;
 
 // What a CTA leaves for the join: the (sequence, head) that its run ends and
 // earlier ones began, as its first token row, KV head, query rows (0: there
-// is none) and number of pieces, this run's the last.
+// is none) and number of pieces, this run's the last; and whether its piece in
+// slot 0 or 1 has met an odd_exp.
 struct Cut {
   int q0, h, rows, pieces;
+  int odd[2], pad[2];
 };
 
 // What a warp's piece of a cut (sequence, head) is: rows 0 where there is none.
 struct PieceMeta {
-  int b, h, rows, ends;
+  int b, h, rows, ends, odd;
 };
 
 // Floats of a run's piece of one (sequence, head): per row O [D], max, sum.
@@ -126,7 +129,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
   constexpr bool kQShared = NT == 2;
   __shared__ uint2 qs[kQShared ? kWarps : 1][kQShared ? NT * KS : 1][32];
   extern __shared__ __align__(16) float held[];  // [warp][2][row][O(D), max, sum]: pieces for the CTA's join
-  __shared__ int lost;                           // a row came out with NaN
+  __shared__ int lost;                           // a row came out with NaN, or its pages may span too much
   __shared__ PieceMeta meta[kWarps][2];          // 0: began in an earlier warp's part, 1: goes on in the next one's
   int* pre = (int*)(held + 2 * kWarps * piece_floats(row_cap, D));  // [B + 1] blocks before a sequence
   int* slen = pre + bt.B + 1;                                       // [B] cached tokens
@@ -189,7 +192,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
   };
   // No workspace where no (sequence, head) can be cut.
   Cut* cuts = (Cut*)((float*)a.ws + (size_t)2 * gridDim.x * piece_floats(row_cap, D));
-  if (a.ws && tid == 0) cuts[c] = Cut{0, 0, 0, 0};
+  if (a.ws && tid == 0) cuts[c] = Cut{};
   if (tid < 2 * kWarps) meta[tid >> 1][tid & 1].rows = 0;
   if (tid == 0) lost = 0;
   if (c >= grid) return;
@@ -345,6 +348,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
   // rows 2t, 2t + 1 of each 8-row tile; vis: keys those rows see.
   int rows = 0, least = 0, from = 0, vis[NT][2];
   float mrow[NT][2], lrow[NT][2], rowf[NT][2];
+  uint32_t odd = 0;  // largest odd_key of the piece
   float o[NT][DM][4];
   uint32_t qb[KS][2] = {};  // of the only tile
   auto query = [&](int nt, int ks) {  // the B fragment of k-step ks
@@ -355,6 +359,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
     if (now.first) {
       const int n = sqn[now.b] & 31, past = now.len - n;
       rows = n * G;
+      odd = 0;
       least = past + 1;  // keys that every row sees
       from = now.k0;
 #pragma unroll
@@ -438,12 +443,15 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
         }
       }
     }
-    float ksc[SUB];
+    float ksc[SUB], vw[SUB];  // vw: 2^(-e - 14)
     int ve[SUB];
 #pragma unroll
     for (int i = 0; i < SUB; ++i) {
       ksc[i] = E4 ? ks[i] : 1.f;
-      ve[i] = E4 ? scale_exp(vs[i]) : 0;
+      const uint32_t field = __float_as_uint(vs[i]) & 0x7f800000u;
+      ve[i] = E4 ? (int)(field >> 23) - 127 : 0;
+      vw[i] = __int_as_float(max((int)((254u - 14u) << 23) - (int)field, 0));
+      if (E4) odd = max(odd, odd_key(vs[i]));
     }
     check(next);
     load_k(next);
@@ -500,9 +508,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
         s[2] = ex2(s[2] - base0);
         s[3] = ex2(s[3] - base1);
         if constexpr (E4) {
-          const float w = pow2i(-ve[i] - 14);
-          lrow[nt][0] = fmaf(s[0] + s[2], w, lrow[nt][0]);
-          lrow[nt][1] = fmaf(s[1] + s[3], w, lrow[nt][1]);
+          lrow[nt][0] = fmaf(s[0] + s[2], vw[i], lrow[nt][0]);
+          lrow[nt][1] = fmaf(s[1] + s[3], vw[i], lrow[nt][1]);
           // Pᵀ as the B operand of Oᵀ += Vᵀ·Pᵀ: an 8x8 (keys x rows) matrix each, transposed in registers.
           ph[nt][i][0] = movm_trans(pack_f16(s[0], s[1]));
           ph[nt][i][1] = movm_trans(pack_f16(s[2], s[3]));
@@ -545,7 +552,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
     if (now.last) {  // end of the piece: out, or kept for the CTA's join
       const bool ends = now.k0 + BK >= now.len, whole = from == 0 && ends;
       const int slot = from > 0 ? 0 : 1;
-      if (!whole && lane == 0) meta[warp][slot] = PieceMeta{now.b, now.h, rows, ends};
+      if (!whole && lane == 0) meta[warp][slot] = PieceMeta{now.b, now.h, rows, ends, odd_exp(odd)};
+      if (E4 && whole && odd_exp(odd)) lost = 1;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -593,8 +601,12 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
     const PieceMeta head = begun ? meta[0][0] : meta[i][1];
     if (head.rows == 0) continue;
     int last = max(i, 0);
-    bool ends = begun && head.ends;
-    while (!ends && last + 1 < kWarps && meta[last + 1][0].rows > 0) ends = meta[++last][0].ends;
+    bool ends = begun && head.ends, odd = head.odd;
+    while (!ends && last + 1 < kWarps && meta[last + 1][0].rows > 0) ends = meta[++last][0].ends, odd |= meta[last][0].odd;
+    if (E4 && odd && tid == 0) {
+      if (!begun && ends) lost = 1;
+      else cuts[c].odd[begun ? 0 : 1] = 1;
+    }
     const int q0 = sqn[head.b] >> 5, np = last - i + (begun ? 0 : 1);  // pieces of the chain
     const int lowest = begun ? 0 : i;
     float* part = (float*)a.ws + (size_t)(2 * c + (begun ? 0 : 1)) * piece_floats(row_cap, D);
@@ -624,15 +636,15 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
       int k = min(c, (int)(((long long)p0 + 1) * grid / total));
       while (k > 0 && begin(k) > p0) --k;
       while (k + 1 < c && begin(k + 1) <= p0) ++k;
-      cuts[c] = Cut{q0, head.h, head.rows, c - k + 1};
+      *reinterpret_cast<int4*>(&cuts[c]) = make_int4(q0, head.h, head.rows, c - k + 1);
     }
   }
   __syncthreads();
-  if (lost) {  // the rows with NaN of the (sequence, head)s that lie in this run, again
+  if (lost) {  // the lost rows of the (sequence, head)s that lie in this run, again
     for (int u = c0; u < c1;) {
       const int b = seq_of(u), nb = max(1, (slen[b] + BK - 1) / BK), h = (u - pre[b]) / nb, from = pre[b] + h * nb;
       if (from >= c0 && from + nb <= c1)
-        for (int r = warp; r < (sqn[b] & 31) * G; r += kWarps) redo_if_nan<D, E4>(a, (sqn[b] >> 5) + r / G, h * G + r % G);
+        for (int r = warp; r < (sqn[b] & 31) * G; r += kWarps) redo_if_lost<D, E4>(a, (sqn[b] >> 5) + r / G, h * G + r % G);
       u = from + nb;
     }
   }
@@ -654,9 +666,15 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(cons
   const int grid = gridDim.x, last = blockIdx.x;
   pdl_trigger();
   pdl_wait();
-  const int4 x = __ldcg(reinterpret_cast<const int4*>(ws + (size_t)2 * grid * piece_floats(row_cap, D)) + last);
+  const Cut* cuts = (const Cut*)(ws + (size_t)2 * grid * piece_floats(row_cap, D));
+  const int4 x = __ldcg(reinterpret_cast<const int4*>(cuts + last));
   const Cut cut{x.x, x.y, x.z, x.w};
   if (cut.rows == 0) return;
+  bool odd = false;
+  if constexpr (E4) {
+    for (int k = lane; k < cut.pieces; k += 32) odd |= __ldcg(&cuts[last - cut.pieces + 1 + k].odd[k == 0 ? 1 : 0]) != 0;
+    odd = __any_sync(0xffffffffu, odd);
+  }
   const int per = cut.rows >= kJoinWarps ? 1 : kJoinWarps / cut.rows;  // warps of a row
   for (int r0 = 0; r0 < cut.rows; r0 += kJoinWarps / per) {
     const int r = r0 + warp / per, sub = warp % per;
@@ -713,7 +731,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(cons
         *reinterpret_cast<uint32_t*>(out + 2 * i) = pack2(acc[2 * i] * f, acc[2 * i + 1] * f);
         bad = fmaf(acc[2 * i] * f, 0.f, fmaf(acc[2 * i + 1] * f, 0.f, bad));
       }
-      if (__any_sync(0xffffffffu, bad != 0.f)) redo_row<D, E4>(a, cut.q0 + r / G, cut.h * G + r % G);
+      if (__any_sync(0xffffffffu, bad != 0.f) || (odd && wide_row(a, cut.q0 + r / G, cut.h))) redo_row<D, E4>(a, cut.q0 + r / G, cut.h * G + r % G);
     }
   }
 }

@@ -33,9 +33,9 @@
 //   * K's scale multiplies the fp32 scores; V's scale 2^e joins the exponent:
 //     P' = 2^(s + e - m + 7) in half (2^-11 relative, down to 2^-21 of the
 //     largest, and within 2^-31 of it below), while the sum adds 2^(s - m) in
-//     fp32.  P in e4m3 would be 2^-4, so the values are not multiplied as
-//     codes: two converter warps turn them into halves (exact), MN-major;
-//     rows behind the sequence become zeros.
+//     fp32 (scales far apart: odd_exp).  P in e4m3 would be 2^-4, so the
+//     values are not multiplied as codes: two converter warps turn them into
+//     halves (exact), MN-major; rows behind the sequence become zeros.
 // P is bf16 over bf16 pages (half a step: 2^-8 relative): the precision in
 // which the stage's own prefill multiplies the values.
 //
@@ -257,10 +257,11 @@ __host__ __device__ constexpr size_t partial_floats() {
 
 // What a CTA leaves for the join: the item that its run ends and earlier ones
 // began, as its sequence's first token row and new tokens, its KV head and
-// tile pair, and its pieces (0: there is none), this run's the last; and
-// whether a row of a whole item in its run came out with NaN.
+// tile pair, and its pieces (0: there is none), this run's the last; whether a
+// row of a whole item in its run came out with NaN or its pages may span too
+// much; and whether its piece in slot 0 or 1 has met an odd_exp.
 struct CutItem {
-  int q0, n, h, j, pieces, redo, pad[2];
+  int q0, n, h, j, pieces, redo, odd[2];
 };
 
 __device__ __forceinline__ uint64_t desc_mn(const void* p, uint32_t lbo) {
@@ -401,7 +402,7 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
   uint64_t* drain = bars + 28;    // every MMA finished
   uint32_t* tmem_holder = (uint32_t*)(bars + 29);
   volatile int* abort_flag = (volatile int*)(tmem_holder + 1);
-  volatile int* redo = abort_flag + 1;  // a row came out with NaN
+  volatile int* redo = abort_flag + 1;  // a row came out with NaN, or its pages may span too much
   // The scales of chunk n in slot n & 3: the keys' stage is free again before
   // the softmax of the chunk has ended, but chunk n + 4 is not converted before.
   float* sks = (float*)(smem + L::kOffScale);  // [4][8]
@@ -439,7 +440,7 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
   const RunsE runs(pre[bt.B], (int)gridDim.x);
   const int c = blockIdx.x;
   CutItem* cut = (CutItem*)((float*)a.ws + (size_t)2 * gridDim.x * partial_floats<D>()) + c;
-  if (threadIdx.x == 0) *redo = cut->pieces = cut->redo = 0;
+  if (threadIdx.x == 0) *redo = cut->pieces = cut->redo = cut->odd[0] = cut->odd[1] = 0;
   if (c >= runs.grid) return;
   if (warp == R::kProducer) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
@@ -766,6 +767,7 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
       }
       {
         const int len = w.p.s.past + w.p.s.n;
+        bool odd = false;
         for (int c0 = 0; c0 < w.nch && ok; c0 += 4) {
           // Lane (j, i): page i of chunk c0 + j.
           const int i = lane & 7, cj = c0 + (lane >> 3);
@@ -783,6 +785,7 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
           if (E4 && page >= 0) {
             ks = pool.ks[page * pool.kse + w.at.h];
             vs = pool.vs[page * pool.vse + w.at.h];
+            odd |= odd_exp(odd_key(vs));
           }
           const int nsl = (keys + kSlice - 1) / kSlice;
           for (int j = 0; j < 4 && c0 + j < w.nch; ++j, ++n) {
@@ -830,6 +833,12 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
               __syncwarp();
               if (lane == 0) mbar_arrive(&sready[n & 3]);
             }
+          }
+        }
+        if constexpr (E4) {
+          if (__any_sync(0xffffffffu, odd) && lane == 0) {
+            if (w.whole) *redo = 1;
+            else cut->odd[w.lo > 0 ? 0 : 1] = 1;
           }
         }
       }
@@ -953,8 +962,8 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
 }
 
 // Joins the pieces of cut items, in order: block (c, y) 32 of the 256 rows of
-// the item that CTA c's run ends, eight lanes per row; and computes rows with
-// NaN of its run's whole items again (here, since the first kernel's roles
+// the item that CTA c's run ends, eight lanes per row; and computes lost rows
+// of its run's whole items again (here, since the first kernel's roles
 // wait for one another with a limit).
 template <int D, bool E4>
 __global__ void __launch_bounds__(256) paged_extend_join_kernel(const __grid_constant__ PagedAttnArgs a) {
@@ -972,7 +981,7 @@ __global__ void __launch_bounds__(256) paged_extend_join_kernel(const __grid_con
       if (!w.whole) continue;
       for (int i = threadIdx.x >> 5; i < 32; i += 8) {
         const int row = blockIdx.y * 32 + i, r = row % kTile, s_tok = (2 * w.at.j + row / kTile) * tq + r / G;
-        if (r / G < tq && s_tok < w.p.s.n) redo_if_nan<D, E4>(a, w.p.s.q0 + s_tok, w.at.h * G + r % G);
+        if (r / G < tq && s_tok < w.p.s.n) redo_if_lost<D, E4>(a, w.p.s.q0 + s_tok, w.at.h * G + r % G);
       }
     }
   }
@@ -986,6 +995,7 @@ __global__ void __launch_bounds__(256) paged_extend_join_kernel(const __grid_con
   auto piece = [&](int k) {
     return (const float*)a.ws + (size_t)(2 * (c - pieces + 1 + k) + (k == 0 ? 1 : 0)) * partial_floats<D>();
   };
+  bool odd = false;
   float M = -INFINITY, L = 0.f, o[D / 8];
 #pragma unroll
   for (int e = 0; e < D / 8; ++e) o[e] = 0.f;
@@ -997,6 +1007,10 @@ __global__ void __launch_bounds__(256) paged_extend_join_kernel(const __grid_con
       const float* q = piece(min(k0 + k, pieces - 1));
       m[k] = __ldcg(q + 2 * kTile * D + row);
       l[k] = __ldcg(q + 2 * kTile * D + 2 * kTile + row);
+      if constexpr (E4) {
+        const int i = min(k0 + k, pieces - 1);
+        odd |= __ldcg(&(cut - pieces + 1 + i)->odd[i == 0 ? 1 : 0]) != 0;
+      }
 #pragma unroll
       for (int e = 0; e < D / 32; ++e) v[k][e] = __ldcg(reinterpret_cast<const float4*>(q + (size_t)row * D + d0 + 4 * e));
     }
@@ -1029,10 +1043,12 @@ __global__ void __launch_bounds__(256) paged_extend_join_kernel(const __grid_con
       *reinterpret_cast<uint4*>(out + 8 * e) = make_uint4(bf16_pair(o[8 * e], o[8 * e + 1]), bf16_pair(o[8 * e + 2], o[8 * e + 3]),
                                                           bf16_pair(o[8 * e + 4], o[8 * e + 5]), bf16_pair(o[8 * e + 6], o[8 * e + 7]));
   }
-  unsigned again = __ballot_sync(0xffffffffu, valid && bad != 0.f);
+  unsigned again = __ballot_sync(0xffffffffu, valid && (bad != 0.f || odd)), nan = __ballot_sync(0xffffffffu, bad != 0.f);
   while (again) {  // eight lanes are a row
     const int lane = __ffs(again) - 1;
-    again &= ~(0xffu << (lane & ~7));
+    const unsigned row_lanes = 0xffu << (lane & ~7);
+    again &= ~row_lanes;
+    if ((nan & row_lanes) == 0 && !wide_row(a, __shfl_sync(0xffffffffu, it.x + s_tok, lane), it.z)) continue;
     redo_row<D, E4>(a, __shfl_sync(0xffffffffu, it.x + s_tok, lane), __shfl_sync(0xffffffffu, it.z * G + r % G, lane));
   }
 }

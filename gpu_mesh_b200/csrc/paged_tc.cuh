@@ -63,6 +63,24 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Over e4m3 pages the running maximum m of a row is one of s + e (2^e the scale
+// of the values' page), while its sum l holds Σ 2^(s - m), the keys' own
+// weights.  What lies 2^126 below m vanishes: a key taken as 2^(s + e - m)·2^-e,
+// a sum multiplied by 2^(m_old - m_new).  Either is then below 2^(span - 126) of
+// l, `span` the difference of the row's largest and least e: nothing up to a
+// span of 98 (2^-28).  Beyond (a page of zeros, whose scale is 2^-100, beside
+// values above 112) it can be all of l, and the rows are computed again by
+// redo_row, whose maximum is one of s.  The kernels note whether a piece has met
+// an odd_exp, without which no span exceeds 98; wide_row then looks at the pages.
+constexpr int kSpan = 98;
+// A scale's distance above 2^-49, as a float's exponent field; one below 2^-49
+// wraps around.  A warp keeps the largest of a piece's (in the loop over the
+// keys a flag took 2.3 % more, the longest step at 8 K 209 us against 204).
+__device__ __forceinline__ uint32_t odd_key(float scale) {
+  return (__float_as_uint(scale) & 0x7f800000u) - ((uint32_t)(127 - kSpan / 2) << 23);
+}
+__device__ __forceinline__ bool odd_exp(uint32_t key) { return key > (uint32_t)kSpan << 23; }
+
 // Two e4m3 codes (the low half of `codes`) to two halves: exact.
 __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t codes) {
   uint32_t r;
@@ -99,6 +117,37 @@ __device__ __forceinline__ int row_shift(float amax) {
   return amax > 0.f ? min(7 - ((int)(__float_as_uint(amax) >> 23) - 127), 126) : 0;
 }
 
+// The sequence of token row t (-1: none), by a whole warp, and the keys that t sees.
+__device__ __forceinline__ int seq_of_row(const PagedAttnArgs& a, int t, int* vis) {
+  const int lane = threadIdx.x & 31;
+  for (int b0 = 0; b0 < a.batch.B; b0 += 32) {
+    SeqSpan s{0, 0, 0, false};
+    if (b0 + lane < a.batch.B) s = seq_span(a.batch, b0 + lane, a.pool.ps);
+    const unsigned found = __ballot_sync(0xffffffffu, s.ok && s.q0 <= t && t < s.q0 + s.n);
+    if (found) {
+      *vis = __shfl_sync(0xffffffffu, s.past + t - s.q0 + 1, __ffs(found) - 1);
+      return b0 + __ffs(found) - 1;
+    }
+  }
+  return -1;
+}
+
+// Whether the exponents of the value pages that token row t sees, of KV head h,
+// span more than kSpan; by a whole warp.
+static __device__ __noinline__ bool wide_row(const PagedAttnArgs& a, int t, int h) {
+  const PagedPool& pool = a.pool;
+  int vis = 0, lo = 127, hi = -127;
+  const int b = seq_of_row(a, t, &vis);
+  if (b < 0) return false;
+  for (int i = threadIdx.x & 31; (int64_t)i * pool.ps < vis; i += 32) {
+    const int page = a.batch.table[(int64_t)b * a.batch.ld + i];
+    const int e = page >= 0 && page < pool.pages ? scale_exp(pool.vs[page * pool.vse + h]) : 0;
+    lo = min(lo, e);
+    hi = max(hi, e);
+  }
+  return __reduce_max_sync(0xffffffffu, hi) - __reduce_min_sync(0xffffffffu, lo) > kSpan;
+}
+
 // One (token row, query head) again, by a whole warp, key
 // by key in fp32.  The tensor-core kernels multiply all values of a block, a
 // row's invisible ones by the weight 0, and 0 times an infinity or a NaN of a
@@ -110,16 +159,8 @@ __device__ __noinline__ void redo_row(const PagedAttnArgs& a, int t, int head) {
   constexpr int N = D / 32;  // dims of a lane
   const PagedPool& pool = a.pool;
   const int lane = threadIdx.x & 31, h = head / (a.nq / pool.nkv);
-  int b = -1, vis = 0;
-  for (int b0 = 0; b0 < a.batch.B && b < 0; b0 += 32) {
-    SeqSpan s{0, 0, 0, false};
-    if (b0 + lane < a.batch.B) s = seq_span(a.batch, b0 + lane, pool.ps);
-    const unsigned found = __ballot_sync(0xffffffffu, s.ok && s.q0 <= t && t < s.q0 + s.n);
-    if (found) {
-      b = b0 + __ffs(found) - 1;
-      vis = __shfl_sync(0xffffffffu, s.past + t - s.q0 + 1, __ffs(found) - 1);
-    }
-  }
+  int vis = 0;
+  const int b = seq_of_row(a, t, &vis);
   if (b < 0) return;
   float q[N], acc[N], m = -INFINITY, l = 0.f;
 #pragma unroll
@@ -165,13 +206,13 @@ __device__ __noinline__ void redo_row(const PagedAttnArgs& a, int t, int head) {
   for (int i = 0; i < N; ++i) out[lane * N + i] = __float2bfloat16_rn(l == 0.f ? 0.f : acc[i] / l);
 }
 
-// The same for a row that this block has written, if it holds a NaN.
+// The same for a row that this block has written, if it holds a NaN or sees too wide a span of scales.
 template <int D, bool E4>
-__device__ __forceinline__ void redo_if_nan(const PagedAttnArgs& a, int t, int head) {
+__device__ __forceinline__ void redo_if_lost(const PagedAttnArgs& a, int t, int head) {
   const __nv_bfloat16* out = (const __nv_bfloat16*)a.out + (int64_t)t * a.ldo + (int64_t)head * a.hdo;
   bool bad = false;
   for (int d = threadIdx.x & 31; d < D; d += 32) bad |= __hisnan(out[d]);
-  if (__any_sync(0xffffffffu, bad)) redo_row<D, E4>(a, t, head);
+  if (__any_sync(0xffffffffu, bad) || (E4 && wide_row(a, t, head / (a.nq / a.pool.nkv)))) redo_row<D, E4>(a, t, head);
 }
 
 }  // namespace paged

@@ -149,3 +149,49 @@ def test_workspace_does_not_follow_reserved_sms(dtype, cache):
     finally:
         reserve(0)
     kernels.paged_check_device()
+
+
+def fill_exponents(c, b, exps, g, zero=-100):
+    """Sequence b's pages: random keys of one size, values whose pages have the scale 2^e (`zero`: a page of zeros)."""
+    for i, e in enumerate(exps):
+        p = int(c.table[b, i])
+        k = torch.randn(c.nkv, c.ps, c.D, generator=g)
+        ek = torch.tensor([float(R.least_exp(float(k[h].abs().max()))) for h in range(c.nkv)])
+        c.ks[p] = torch.exp2(ek).to(DEV)
+        c.k.view(torch.uint8)[p] = (k * torch.exp2(-ek)[:, None, None]).to(E4M3).view(torch.uint8).to(DEV)
+        x = torch.zeros(c.nkv, c.ps, c.D) if e == zero else torch.randn(c.nkv, c.ps, c.D, generator=g)
+        x *= 448.0 / x.abs().amax((1, 2), keepdim=True).clamp(min=1.0)
+        c.vs[p] = 2.0**e
+        c.v.view(torch.uint8)[p] = x.to(E4M3).view(torch.uint8).to(DEV)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("n", [1, 4, 40])
+@pytest.mark.parametrize("big", [0, 30, 34, 41, 60, 100])
+def test_softmax_sum_over_pages_of_all_scales(dtype, n, big):
+    """Pages of zeros (scale 2^-100), of tiny and of huge values in one sequence, in every order, next to one another
+    and so far apart that the run's parts are joined: a key weighs the same in the softmax whatever its values."""
+    D, nkv, nq, ps = (64, 2, 8, 16) if n == 4 else (128, 1, 4, 32)
+    g = torch.Generator().manual_seed(big + n)
+    low = -100
+    orders = [[low, big], [big, low], [low, big, -30, 0], [big] + [low] * 40, [low] * 40 + [big], [low] * 60 + [big] * 60,
+              ([low] * 7 + [big] + [-8] * 5) * 9, [-30, low, big, low] * 3, [low] * 3]
+    lens = [max(ps * len(o) - 5 * (i % 2), 1) for i, o in enumerate(orders)]
+    c = Cache(lens, nkv, ps, D, dtype, E4M3, seed=big)
+    for b, o in enumerate(orders):
+        fill_exponents(c, b, o, g)
+    for amp in (1e-3, 1.0):  # equal scores, ordinary ones
+        new = [min(n, L) for L in lens]
+        q = (torch.randn(sum(new), nq, D, generator=g) * amp).to(dtype)
+        out = kernels.paged_attention(q.to(DEV), c.k, c.v, c.table.to(DEV), dev32(starts(new)), dev32(lens), max_new=n, **c.scales())
+        kernels.paged_check_device()
+        pools = c.host()
+        for b, (t0, m, past) in enumerate(R.spans(starts(new), lens)):
+            x = q[t0:t0 + m].double()
+            k, v = (R.dense(*pools[key], c.table[b], lens[b]) for key in ("k", "v"))
+            ref, weight, top = R.attend(x, k, v, past, D**-0.5)
+            tol = R.attention_tolerance(ref, weight, top, D, lens[b], dtype, P_STEP[dtype], dtype == BF16)
+            if dtype == BF16:
+                tol += half_floor(x, k, v, key_scales(c, pools["v"][1], b, lens[b]), past, D**-0.5, 14 if 4 * m <= 16 else 7)
+            err = (out[t0:t0 + m].cpu().double() - ref).abs()
+            assert (err <= tol).all(), (b, amp, float((err / tol).max()))
