@@ -195,7 +195,8 @@ __device__ __noinline__ void redo_row(const PagedAttnArgs& a, int t, int head) {
     for (int i = 0; i < N; ++i) s = fmaf(q[i], k[i], s);
 #pragma unroll
     for (int i = 16; i > 0; i >>= 1) s += __shfl_xor_sync(0xffffffffu, s, i);
-    const float top = fmaxf(m, s), keep = m == -INFINITY ? 0.f : ex2(m - top), w = ex2(s - top);
+    const float top = fmaxf(m, s), keep = m == -INFINITY ? 0.f : ex2(m - top);
+    const float w = s == -INFINITY ? 0.f : ex2(s - top);  // also where nothing lies above -inf yet
     m = top;
     l = l * keep + w;
 #pragma unroll

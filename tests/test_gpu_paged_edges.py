@@ -195,3 +195,38 @@ def test_softmax_sum_over_pages_of_all_scales(dtype, n, big):
                 tol += half_floor(x, k, v, key_scales(c, pools["v"][1], b, lens[b]), past, D**-0.5, 14 if 4 * m <= 16 else 7)
             err = (out[t0:t0 + m].cpu().double() - ref).abs()
             assert (err <= tol).all(), (b, amp, float((err / tol).max()))
+
+
+@pytest.mark.parametrize("dtype,cache", [(BF16, BF16), (F32, F32)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_keys_of_no_weight_before_broken_tokens(dtype, cache, D):
+    """Infinite first keys whose scores are -inf (weight 0), while values of later tokens are NaN or infinite: the rows
+    before those come out as if the first keys were not there."""
+    new, lens = [4, 60, 3, 200, 1], [700, 90, 5000, 3000, 40]
+    c = Cache(lens, 2, 16, D, dtype, cache, seed=D)
+    c.fill(lens)
+    g = torch.Generator().manual_seed(D)
+    q = torch.randn(sum(new), 8, D, generator=g)
+    q[..., 5] = q[..., 5].abs() + 0.1
+    q = q.to(dtype)
+    none = 3  # first keys without weight, fewer than any row sees
+    for b, (n, L) in enumerate(zip(new, lens)):
+        for j in range(none):
+            c.k[int(c.table[b, 0]), :, j, 5] = -torch.inf
+        if n > 1:
+            p, o = int(c.table[b, (L - 1) // 16]), (L - 1) % 16
+            c.v[p, 0, o, 3] = torch.nan
+            c.v[p, 1, o, ::7] = torch.inf
+    out = kernels.paged_attention(q.to(DEV), c.k, c.v, c.table.to(DEV), dev32(starts(new)), dev32(lens), **c.scales())
+    kernels.paged_check_device()
+    pools = c.host()
+    for b, (t0, n, past) in enumerate(R.spans(starts(new), lens)):
+        k, v = (R.dense(*pools[key], c.table[b], lens[b])[:, none:] for key in ("k", "v"))
+        for s in range(n):
+            seen = past + s + 1 - none
+            ref, weight, top = R.attend(q[t0 + s:t0 + s + 1].double(), k[:, :seen], v[:, :seen], seen - 1, D**-0.5)
+            tol = R.attention_tolerance(ref, weight, top, D, lens[b], dtype, P_STEP[dtype])
+            x = out[t0 + s].cpu().double()
+            fine = ref[0].isfinite()
+            assert torch.equal(x.isnan(), ref[0].isnan()) and torch.equal(x.isinf(), ref[0].isinf()), (b, s)
+            assert ((x - ref[0]).abs()[fine] <= tol[0][fine]).all(), (b, s)
