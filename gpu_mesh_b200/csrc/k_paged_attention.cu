@@ -33,6 +33,7 @@ constexpr int kRows = 16;     // most query rows of a CTA
 constexpr int kKeys = 32;     // keys of a round
 constexpr int kSimt = 128;    // threads
 constexpr int kMaxSplits = 64;
+constexpr float kUnseen = -1.f;  // in place of a weight: the row does not see the key
 
 // One 16-byte (e4m3: 8-code) piece of a cached row, widened.
 template <typename C>
@@ -192,7 +193,7 @@ __global__ void __launch_bounds__(kSimt) paged_attn_simt_kernel(const __grid_con
 #pragma unroll
     for (int i = 0; i < KPT; ++i) {
       const float p = s[i] == -INFINITY ? 0.f : exp2f(s[i] - mx);
-      sp[qr][kq + TPR * i] = p;
+      sp[qr][kq + TPR * i] = k0 + kq + TPR * i < vis ? p : kUnseen;
       part += p;
     }
 #pragma unroll
@@ -204,7 +205,8 @@ __global__ void __launch_bounds__(kSimt) paged_attn_simt_kernel(const __grid_con
 #pragma unroll
     for (int i = 0; i < RPT; ++i) acc[i] *= keep[og * RPT + i];
     // Keys that no row of the tile sees were loaded as zeros; a row's own
-    // invisible keys weigh 0, but 0 · NaN is not 0, so they are left out.
+    // invisible keys weigh 0, but 0 · NaN is not 0, so they are left out (and
+    // only they: a visible key's NaN counts, however little it weighs).
     for (int k = 0; k < kKeys; k += 4) {
       const float v[4] = {sv[k][od], sv[k + 1][od], sv[k + 2][od], sv[k + 3][od]};
 #pragma unroll
@@ -212,7 +214,7 @@ __global__ void __launch_bounds__(kSimt) paged_attn_simt_kernel(const __grid_con
         const float4 p4 = *reinterpret_cast<const float4*>(&sp[og * RPT + i][k]);
         const float p[4] = {p4.x, p4.y, p4.z, p4.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i] = p[e] != 0.f ? fmaf(p[e], v[e], acc[i]) : acc[i];
+        for (int e = 0; e < 4; ++e) acc[i] = p[e] != kUnseen ? fmaf(p[e], v[e], acc[i]) : acc[i];
       }
     }
   }
@@ -257,7 +259,10 @@ __global__ void __launch_bounds__(kJoinParts * D) paged_attn_join_kernel(const _
   const float* w = (const float*)a.ws + ((part_row(a, b) + s) * a.nq + head) * splits * (D + 2);
   float M = -INFINITY, l = 0.f, o = 0.f;
   auto add = [&](float m, float sum, float v) {
-    if (sum == 0.f) return;  // it saw no key
+    if (sum == 0.f) {  // it saw no key (v is 0), or its keys weigh nothing (v is 0 or NaN)
+      o = fmaf(0.f, v, o);
+      return;
+    }
     const float top = fmaxf(M, m), keep = M == -INFINITY ? 0.f : exp2f(M - top), f = exp2f(m - top);
     M = top;
     l = l * keep + f * sum;

@@ -1016,8 +1016,11 @@ __global__ void __launch_bounds__(256) paged_extend_join_kernel(const __grid_con
     }
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      if (k0 + k >= pieces || l[k] == 0.f) continue;  // none, or it saw no key
-      const float top = fmaxf(M, m[k]), keep = M == -INFINITY ? 0.f : ex2(M - top), f = ex2(m[k] - top);
+      if (k0 + k >= pieces) continue;
+      // One that saw no key has O = 0, or NaN from values that the row does not
+      // see: such a row is computed again below.
+      const float top = fmaxf(M, m[k]), keep = M == -INFINITY ? 0.f : ex2(M - top);
+      const float f = m[k] == -INFINITY ? 0.f : ex2(m[k] - top);
       M = top;
       L = L * keep + f * l[k];
 #pragma unroll

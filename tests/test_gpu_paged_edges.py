@@ -230,3 +230,40 @@ def test_keys_of_no_weight_before_broken_tokens(dtype, cache, D):
             fine = ref[0].isfinite()
             assert torch.equal(x.isnan(), ref[0].isnan()) and torch.equal(x.isinf(), ref[0].isinf()), (b, s)
             assert ((x - ref[0]).abs()[fine] <= tol[0][fine]).all(), (b, s)
+
+
+@pytest.mark.parametrize("dtype,cache,D", [(F32, F32, 64), (F32, E4M3, 128), (BF16, BF16, 32), (BF16, E4M3, 16),
+                                           (BF16, BF16, 64), (BF16, E4M3, 64), (BF16, BF16, 128), (BF16, E4M3, 128)])
+@pytest.mark.parametrize("n", [1, 3, 40])
+def test_broken_values_of_keys_without_weight(dtype, cache, D, n):
+    """A NaN or an infinity in a value that a row sees reaches it however little its key weighs (0 times either is
+    NaN), also where the key's part of the context holds no other weight."""
+    lens, ps = [2500, 70], 16
+    new = [n, n]
+    c = Cache(lens, 2, ps, D, dtype, cache, seed=n)
+    c.fill(lens, spread=0)
+    q = torch.zeros(sum(new), 4, D, dtype=dtype)
+    q[..., 0] = 64.0 * D**0.5
+    for b, L in enumerate(lens):  # scores 64 times the first dim: 16 for the keys that count, -16 for the first tokens
+        for j in range(L):
+            at = (int(c.table[b, j // ps]), slice(None), j % ps)
+            low = j < min(40, L - n)
+            if cache == E4M3:
+                c.k.view(torch.uint8)[at] = 0
+                c.k.view(torch.uint8)[at[0], :, at[2], 0] = 0x48 | (0x80 if low else 0)  # 4.0
+            else:
+                c.k[at] = 0.0
+                c.k[at[0], :, at[2], 0] = -4.0 if low else 4.0
+        if cache == E4M3:
+            c.ks[c.table[b][: -(-L // ps)].long().to(DEV)] = 1.0
+        for h, d, x in ((0, 1, torch.nan), (1, 2, torch.inf)):
+            if cache == E4M3:
+                c.v.view(torch.uint8)[int(c.table[b, 0]), h, 7, d] = 0x7F
+            else:
+                c.v[int(c.table[b, 0]), h, 7, d] = x
+    out = kernels.paged_attention(q.to(DEV), c.k, c.v, c.table.to(DEV), dev32(starts(new)), dev32(lens), **c.scales())
+    kernels.paged_check_device()
+    broken = torch.zeros(out.shape, dtype=torch.bool)
+    broken[:, :2, 1] = True
+    broken[:, 2:, 2] = True
+    assert torch.equal(out.cpu().isfinite(), ~broken)
