@@ -31,8 +31,10 @@ Page sizes 16, 32, 64 and 128, head sizes 8, 16, 32, 64 and 128, up to 16 query 
 and 2^26 - 1 token rows per call.  bf16 with head sizes 64 and 128 runs attention on the tensor cores.
 
 The current stream runs the work, and nothing waits for it (a call can be captured once one has run on its device
-outside a capture): what only the device can see (a page id outside the
-pool, a length outside the table) leaves that sequence out and is raised by ``paged_check_device``.
+outside a capture).  What only the device can see is raised by ``paged_check_device``: a length or rows outside the
+table, the bound or the batch, which leave that sequence out, and a page id outside the pool, which leaves out that
+page: nothing is stored for its tokens, and attention takes its keys and values as zeros, so that the rows of that
+sequence are written but mean nothing.  Other sequences are not disturbed.
 """
 from __future__ import annotations
 

@@ -350,8 +350,11 @@ typedef struct mg_paged_pool {
  * its columns hold at most 2^30 tokens.  Rows of the token tensors behind
  * q_start[batch] are left as they are.  A sequence whose ranges do not fit (a
  * length above max_pages page_size, more than max_new new tokens, rows outside
- * [0, tokens)) is left out, and, like a page id outside the pool, reported by
- * mg_paged_check_device. */
+ * [0, tokens)) is left out and reported by mg_paged_check_device.  So is a page
+ * id outside the pool, but it leaves out that page alone: nothing is stored for
+ * its tokens, and attention takes its keys and values as zeros, so that the
+ * sequence's rows are written but mean nothing.  Other sequences are not
+ * disturbed. */
 typedef struct mg_paged_batch {
   const int32_t* page_table; /* [batch, max_pages] */
   const int32_t* q_start;    /* [batch + 1] */

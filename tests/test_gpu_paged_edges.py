@@ -267,3 +267,75 @@ def test_broken_values_of_keys_without_weight(dtype, cache, D, n):
     broken[:, :2, 1] = True
     broken[:, 2:, 2] = True
     assert torch.equal(out.cpu().isfinite(), ~broken)
+
+
+@pytest.mark.parametrize("dtype,cache", [(BF16, BF16), (BF16, E4M3), (F32, F32)])
+@pytest.mark.parametrize("limit", [None, 4])
+def test_bad_metadata_disturbs_no_other_sequence(dtype, cache, limit):
+    """Lengths, row ranges and page ids that do not fit: the other sequences' rows, pages and scales come out as ever,
+    and nothing is stored for what was left out.  A page id outside the pool leaves out its page alone."""
+    few = limit is not None
+    lens, new = [40, 20, 33, 10, 300], [2, 1, 4 if few else 33, 2, 3 if few else 50]
+    nq, nkv, D, ps = 8, 2, 64, 16
+    g = torch.Generator().manual_seed(3)
+    q = torch.randn(sum(new), nq, D, generator=g).to(dtype)
+    qkv = torch.randn(sum(new), (nq + 2 * nkv) * D, generator=g).to(dtype).to(DEV)
+
+    def cache_of():
+        c = Cache(lens, nkv, ps, D, dtype, cache)
+        c.fill(lens)  # the attention's own tokens; the append writes over them
+        return c
+
+    def run_append(q_start, n, table, wrong):
+        c = cache_of()
+        out = torch.full((sum(new), nq, D), 7.0, dtype=dtype, device=DEV)
+        kernels.paged_append(qkv, c.k, c.v, table.to(DEV), dev32(q_start), dev32(n), num_q_heads=nq, max_new=limit, out=out,
+                             **c.scales())
+        if wrong:
+            with pytest.raises(_lib.DeviceRangeError, match="page id, length"):
+                kernels.paged_check_device()
+        kernels.paged_check_device()
+        return c, out
+
+    bits = lambda t: t.cpu().contiguous().view(torch.int8)  # noqa: E731
+    c = cache_of()
+    cap = c.cols * ps
+    good, good_q = run_append(starts(new), lens, c.table, False)
+    at = starts(new)
+    cases = [(at, [40, cap + 1, 33, 10, 300], 1, None), (at, [40, -1, 33, 10, 300], 1, None),
+             (at[:4] + [2000] + at[5:], lens, 3, None)]  # (sequence 4 then begins at 2000 too: left out as well)
+    cases += [(at, lens, b, wrong) for b in (0, 4) for wrong in (-1, c.pages, 2**31 - 1, -(2**31))]
+    pools = c.host()
+    for q_start, n, b, wrong in cases:
+        table, last = c.table.clone(), (lens[b] - 1) // ps
+        if wrong is not None:
+            table[b, last] = wrong
+        bad = [i for i in range(len(lens)) if i == b or (q_start[i] != at[i])]
+        out = torch.full_like(q, 7.0).to(DEV)
+        kernels.paged_attention(q.to(DEV), c.k, c.v, table.to(DEV), dev32(q_start), dev32(n), max_new=limit, out=out, **c.scales())
+        with pytest.raises(_lib.DeviceRangeError, match="page id, length"):
+            kernels.paged_check_device()
+        after, after_q = run_append(q_start, n, table, True)
+        skipped = torch.zeros(c.pages, dtype=torch.bool)
+        for i, (t0, m, past) in enumerate(R.spans(at, lens)):
+            rows = slice(t0, t0 + m)
+            if i in bad:
+                if wrong is None:
+                    assert (out[rows] == 7.0).all() and (after_q[rows] == 7.0).all()
+                    skipped[c.table[i][past // ps: (lens[i] - 1) // ps + 1].long()] = True
+                else:
+                    assert torch.equal(after_q[rows], good_q[rows])
+                    skipped[int(c.table[i, last])] = True
+                continue
+            assert torch.equal(after_q[rows], good_q[rows])
+            k, v = (R.dense(*pools[key], c.table[i], lens[i]) for key in ("k", "v"))
+            ref, weight, top = R.attend(q[rows].double(), k, v, past, D**-0.5)
+            tol = R.attention_tolerance(ref, weight, top, D, lens[i], dtype, P_STEP[dtype], cache == E4M3 and dtype == BF16)
+            if cache == E4M3:
+                tol += half_floor(q[rows].double(), k, v, key_scales(c, pools["v"][1], i, lens[i]), past, D**-0.5,
+                                  14 if 4 * m <= 16 else 7)
+            assert ((out[rows].cpu().double() - ref).abs() <= tol).all(), (b, wrong, i)
+        for x, y, start in ((after.k, good.k, c.k), (after.v, good.v, c.v), (after.ks, good.ks, c.ks), (after.vs, good.vs, c.vs)):
+            if x is not None:
+                assert torch.equal(bits(x[(~skipped).to(DEV)]), bits(y[(~skipped).to(DEV)]))
+                assert torch.equal(bits(x[skipped.to(DEV)]), bits(start[skipped.to(DEV)]))
