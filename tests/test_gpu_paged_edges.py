@@ -339,3 +339,48 @@ def test_bad_metadata_disturbs_no_other_sequence(dtype, cache, limit):
             if x is not None:
                 assert torch.equal(bits(x[(~skipped).to(DEV)]), bits(y[(~skipped).to(DEV)]))
                 assert torch.equal(bits(x[skipped.to(DEV)]), bits(start[skipped.to(DEV)]))
+
+
+@pytest.mark.parametrize("cache", [BF16, E4M3])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n", [1, 2, 4])
+def test_precision_with_few_query_rows(cache, D, n):
+    """Up to 16 query rows per KV head the queries stay exact and the weights are a bf16 and its remainder (each off by
+    half a step: 2^-16 together) or a half (2^-11).  Neighbouring keys are nearly alike and their values of opposite
+    sign, so that outputs are small beside sum(p|v|) and the output's own rounding hides nothing: weights rounded to
+    bf16 alone would not pass."""
+    nq, nkv, ps = 8, 2, 16
+    lens, g = [24, 40, 12, 300, 64, 1000], torch.Generator().manual_seed(D + n)
+    c = Cache(lens, nkv, ps, D, BF16, cache, seed=n)
+    for b, L in enumerate(lens):
+        k, v = (torch.randn(nkv, L, D, generator=g).clamp(-6, 6) for _ in range(2))
+        k[:, 1::2] = k[:, ::2] + 0.02 * torch.randn(nkv, L // 2, D, generator=g)
+        v[:, 1::2] = -v[:, ::2]
+        for x, pages, scale in ((k, c.k, c.ks), (v, c.v, c.vs)):
+            for i in range(-(-L // ps)):
+                p, y = int(c.table[b, i]), x[:, i * ps:(i + 1) * ps]
+                if cache == E4M3:
+                    scale[p] = 2.0**-6
+                    pages.view(torch.uint8)[p, :, :y.shape[1]] = (y * 64.0).to(E4M3).view(torch.uint8).to(DEV)
+                else:
+                    pages[p, :, :y.shape[1]] = y.to(BF16).to(DEV)
+    new = [n] * len(lens)
+    q = (torch.randn(sum(new), nq, D, generator=g) * torch.tensor([0.3, 1.0, 3.0, 0.3] * 2)[:nq, None]).to(BF16)
+    out = kernels.paged_attention(q.to(DEV), c.k, c.v, c.table.to(DEV), dev32(starts(new)), dev32(lens), max_new=n, **c.scales())
+    kernels.paged_check_device()
+    pools, coarse = c.host(), 0
+    for b, (t0, _, past) in enumerate(R.spans(starts(new), lens)):
+        x = q[t0:t0 + n].double()
+        k, v = (R.dense(*pools[key], c.table[b], lens[b]) for key in ("k", "v"))
+        ref, weight, top = R.attend(x, k, v, past, D**-0.5)
+        tol = R.attention_tolerance(ref, weight, top, D, lens[b], BF16, 2.0**-16 if cache == BF16 else 2.0**-11)
+        if cache == E4M3:
+            # The exponent carries V's -6 and 14 beside the score: two roundings of it more, in every weight and the sum.
+            tol += half_floor(x, k, v, key_scales(c, pools["v"][1], b, lens[b]), past, D**-0.5, 14) + 4 * R.F32 * 20 * weight
+        assert ((out[t0:t0 + n].cpu().double() - ref).abs() <= tol).all(), (b, lens[b])
+        s = torch.einsum("nhd,hld->hnl", x, k.repeat_interleave(nq // nkv, 0)) * D**-0.5
+        s = s.masked_fill(torch.arange(lens[b])[None] > past + torch.arange(n)[:, None], -torch.inf)
+        p = torch.exp(s - s.amax(-1, keepdim=True))
+        rough = torch.einsum("hnl,hld->nhd", p.to(BF16).double() / p.sum(-1, keepdim=True), v.repeat_interleave(nq // nkv, 0))
+        coarse += int(((rough - ref).abs() > tol).sum())
+    assert coarse > 0  # the tolerance tells a coarser P apart
