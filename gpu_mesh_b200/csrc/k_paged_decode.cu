@@ -31,7 +31,7 @@
 //       maximum m of s + e, P' = 2^(s + e - m + 14) (rounded to half: 2^-11
 //       relative, down to 2^-28 of the largest, and within 2^-39 of it below)
 //       weighs the raw codes, while the sum adds P'·2^(-e - 14) = 2^(s - m) in
-//       fp32 (scales far apart: odd_exp); out = O / l · 2^-14.
+//       fp32 (scales far apart: kSpan); out = O / l · 2^-14.
 //
 // Measured (32 query, 8 KV heads of 128): 64 tokens on 7.9 to 8.2 K positions,
 // e4m3, 204 us = 5.2 TB/s; 32 tokens, bf16, 182 us = 5.8 TB/s (a copy runs at
@@ -83,15 +83,15 @@ constexpr int kLeast = 4;
 // What a CTA leaves for the join: the (sequence, head) that its run ends and
 // earlier ones began, as its first token row, KV head, query rows (0: there
 // is none) and number of pieces, this run's the last; and whether its piece in
-// slot 0 or 1 has met an odd_exp.
+// slot 0 or 1 has met a high_scale.
 struct Cut {
   int q0, h, rows, pieces;
-  int odd[2], pad[2];
+  int high[2], pad[2];
 };
 
 // What a warp's piece of a cut (sequence, head) is: rows 0 where there is none.
 struct PieceMeta {
-  int b, h, rows, ends, odd;
+  int b, h, rows, ends, high;
 };
 
 // Floats of a run's piece of one (sequence, head): per row O [D], max, sum.
@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
   // rows 2t, 2t + 1 of each 8-row tile; vis: keys those rows see.
   int rows = 0, least = 0, from = 0, vis[NT][2];
   float mrow[NT][2], lrow[NT][2], rowf[NT][2];
-  uint32_t odd = 0;  // largest odd_key of the piece
+  float top_vs = 0.f;  // largest scale of the piece's values (a flag took 2.3 % more: 209 us on 8 K)
   float o[NT][DM][4];
   uint32_t qb[KS][2] = {};  // of the only tile
   auto query = [&](int nt, int ks) {  // the B fragment of k-step ks
@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
     if (now.first) {
       const int n = sqn[now.b] & 31, past = now.len - n;
       rows = n * G;
-      odd = 0;
+      top_vs = 0.f;
       least = past + 1;  // keys that every row sees
       from = now.k0;
 #pragma unroll
@@ -448,10 +448,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
 #pragma unroll
     for (int i = 0; i < SUB; ++i) {
       ksc[i] = E4 ? ks[i] : 1.f;
-      const uint32_t field = __float_as_uint(vs[i]) & 0x7f800000u;
-      ve[i] = E4 ? (int)(field >> 23) - 127 : 0;
-      vw[i] = __int_as_float(max((int)((254u - 14u) << 23) - (int)field, 0));
-      if (E4) odd = max(odd, odd_key(vs[i]));
+      ve[i] = E4 ? scale_exp(vs[i]) : 0;
+      vw[i] = E4 ? pow2i(-ve[i] - 14) : 1.f;
+      if (E4) top_vs = fmaxf(top_vs, vs[i]);
     }
     check(next);
     load_k(next);
@@ -485,9 +484,16 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
         float keep[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          keep[e] = mrow[nt][e] == -INFINITY ? 0.f : ex2(mrow[nt][e] - mx[e]);
+          const float d = mrow[nt][e] == -INFINITY ? -INFINITY : mrow[nt][e] - mx[e];
           mrow[nt][e] = mx[e];
-          lrow[nt][e] *= keep[e];
+          if constexpr (E4) {
+            const float half = ex2(0.5f * d);
+            keep[e] = half * half;
+            lrow[nt][e] = lrow[nt][e] * half * half;
+          } else {
+            keep[e] = ex2(d);
+            lrow[nt][e] *= keep[e];
+          }
         }
 #pragma unroll
         for (int i = 0; i < DM; ++i) {
@@ -552,8 +558,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
     if (now.last) {  // end of the piece: out, or kept for the CTA's join
       const bool ends = now.k0 + BK >= now.len, whole = from == 0 && ends;
       const int slot = from > 0 ? 0 : 1;
-      if (!whole && lane == 0) meta[warp][slot] = PieceMeta{now.b, now.h, rows, ends, odd_exp(odd)};
-      if (E4 && whole && odd_exp(odd)) lost = 1;
+      if (!whole && lane == 0) meta[warp][slot] = PieceMeta{now.b, now.h, rows, ends, high_scale(top_vs)};
+      if (E4 && whole && high_scale(top_vs)) lost = 1;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -601,11 +607,11 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
     const PieceMeta head = begun ? meta[0][0] : meta[i][1];
     if (head.rows == 0) continue;
     int last = max(i, 0);
-    bool ends = begun && head.ends, odd = head.odd;
-    while (!ends && last + 1 < kWarps && meta[last + 1][0].rows > 0) ends = meta[++last][0].ends, odd |= meta[last][0].odd;
-    if (E4 && odd && tid == 0) {
+    bool ends = begun && head.ends, high = head.high;
+    while (!ends && last + 1 < kWarps && meta[last + 1][0].rows > 0) ends = meta[++last][0].ends, high |= meta[last][0].high;
+    if (E4 && high && tid == 0) {
       if (!begun && ends) lost = 1;
-      else cuts[c].odd[begun ? 0 : 1] = 1;
+      else cuts[c].high[begun ? 0 : 1] = 1;
     }
     const int q0 = sqn[head.b] >> 5, np = last - i + (begun ? 0 : 1);  // pieces of the chain
     const int lowest = begun ? 0 : i;
@@ -619,7 +625,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
       for (int j = 0; j < np; ++j) M = fmaxf(M, at(j)[D]);
       for (int j = 0; j < np; ++j) {
         const float m = at(j)[D], f = m == -INFINITY ? 0.f : ex2(m - M);
-        S += f * at(j)[D + 1];
+        S = add_sum<E4>(S, at(j)[D + 1], m - M, f);
         acc += f * at(j)[d];
       }
       if (!begun && ends) {
@@ -643,8 +649,11 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_decode_kernel(const __gr
   if (lost) {  // the lost rows of the (sequence, head)s that lie in this run, again
     for (int u = c0; u < c1;) {
       const int b = seq_of(u), nb = max(1, (slen[b] + BK - 1) / BK), h = (u - pre[b]) / nb, from = pre[b] + h * nb;
-      if (from >= c0 && from + nb <= c1)
-        for (int r = warp; r < (sqn[b] & 31) * G; r += kWarps) redo_if_lost<D, E4>(a, (sqn[b] >> 5) + r / G, h * G + r % G);
+      if (from >= c0 && from + nb <= c1) {
+        const int q0 = sqn[b] >> 5, n = sqn[b] & 31;
+        const bool wide = E4 && wide_row(a, q0 + n - 1, h);
+        for (int r = warp; r < n * G; r += kWarps) redo_if_lost<D, E4>(a, q0 + r / G, h * G + r % G, wide);
+      }
       u = from + nb;
     }
   }
@@ -670,10 +679,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(cons
   const int4 x = __ldcg(reinterpret_cast<const int4*>(cuts + last));
   const Cut cut{x.x, x.y, x.z, x.w};
   if (cut.rows == 0) return;
-  bool odd = false;
+  bool high = false;
   if constexpr (E4) {
-    for (int k = lane; k < cut.pieces; k += 32) odd |= __ldcg(&cuts[last - cut.pieces + 1 + k].odd[k == 0 ? 1 : 0]) != 0;
-    odd = __any_sync(0xffffffffu, odd);
+    for (int k = lane; k < cut.pieces; k += 32) high |= __ldcg(&cuts[last - cut.pieces + 1 + k].high[k == 0 ? 1 : 0]) != 0;
+    high = __any_sync(0xffffffffu, high);
   }
   const int per = cut.rows >= kJoinWarps ? 1 : kJoinWarps / cut.rows;  // warps of a row
   for (int r0 = 0; r0 < cut.rows; r0 += kJoinWarps / per) {
@@ -685,8 +694,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(cons
     auto add = [&](float m, float l, const float* v) {
       const float top = fmaxf(M, m);
       const float keep = M == -INFINITY ? 0.f : ex2(M - top), f = m == -INFINITY ? 0.f : ex2(m - top);
+      L = add_sum<E4>(add_sum<E4>(0.f, L, M - top, keep), l, m - top, f);
       M = top;
-      L = L * keep + f * l;
 #pragma unroll
       for (int i = 0; i < N; ++i) acc[i] = acc[i] * keep + f * v[i];
     };
@@ -731,7 +740,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(cons
         *reinterpret_cast<uint32_t*>(out + 2 * i) = pack2(acc[2 * i] * f, acc[2 * i + 1] * f);
         bad = fmaf(acc[2 * i] * f, 0.f, fmaf(acc[2 * i + 1] * f, 0.f, bad));
       }
-      if (__any_sync(0xffffffffu, bad != 0.f) || (odd && wide_row(a, cut.q0 + r / G, cut.h))) redo_row<D, E4>(a, cut.q0 + r / G, cut.h * G + r % G);
+      if (__any_sync(0xffffffffu, bad != 0.f) || (high && wide_row(a, cut.q0 + r / G, cut.h))) redo_row<D, E4>(a, cut.q0 + r / G, cut.h * G + r % G);
     }
   }
 }

@@ -33,7 +33,7 @@
 //   * K's scale multiplies the fp32 scores; V's scale 2^e joins the exponent:
 //     P' = 2^(s + e - m + 7) in half (2^-11 relative, down to 2^-21 of the
 //     largest, and within 2^-31 of it below), while the sum adds 2^(s - m) in
-//     fp32 (scales far apart: odd_exp).  P in e4m3 would be 2^-4, so the
+//     fp32 (scales far apart: kSpan).  P in e4m3 would be 2^-4, so the
 //     values are not multiplied as codes: two converter warps turn them into
 //     halves (exact), MN-major; rows behind the sequence become zeros.
 // P is bf16 over bf16 pages (half a step: 2^-8 relative): the precision in
@@ -259,9 +259,9 @@ __host__ __device__ constexpr size_t partial_floats() {
 // began, as its sequence's first token row and new tokens, its KV head and
 // tile pair, and its pieces (0: there is none), this run's the last; whether a
 // row of a whole item in its run came out with NaN or its pages may span too
-// much; and whether its piece in slot 0 or 1 has met an odd_exp.
+// much; and whether its piece in slot 0 or 1 has met a high_scale.
 struct CutItem {
-  int q0, n, h, j, pieces, redo, odd[2];
+  int q0, n, h, j, pieces, redo, high[2];
 };
 
 __device__ __forceinline__ uint64_t desc_mn(const void* p, uint32_t lbo) {
@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
   const RunsE runs(pre[bt.B], (int)gridDim.x);
   const int c = blockIdx.x;
   CutItem* cut = (CutItem*)((float*)a.ws + (size_t)2 * gridDim.x * partial_floats<D>()) + c;
-  if (threadIdx.x == 0) *redo = cut->pieces = cut->redo = cut->odd[0] = cut->odd[1] = 0;
+  if (threadIdx.x == 0) *redo = cut->pieces = cut->redo = cut->high[0] = cut->high[1] = 0;
   if (c >= runs.grid) return;
   if (warp == R::kProducer) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
@@ -576,7 +576,7 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
           m_new = mt;
           moved = true;
         }
-        const float alpha = moved ? ex2(m - m_new) : 1.f;
+        const float half = moved ? ex2((E4 ? 0.5f : 1.f) * (m - m_new)) : 1.f, alpha = E4 ? half * half : half;
         const float mb = m_new == -INFINITY ? 0.f : m_new - (E4 ? 7.f : 0.f);
         m = m_new;
         float add = 0.f;
@@ -601,7 +601,7 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
         // P over the scores, two keys per column: both threads of the row have
         // read theirs (the exchange).
         tmem_st32(tS + 32 * hf, sc);
-        l = l * alpha + add;
+        l = E4 ? l * half * half + add : l * alpha + add;
         // The previous value product of this tile has finished (the score
         // product just read was issued after it).
         if (__any_sync(0xffffffffu, moved)) {
@@ -767,7 +767,7 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
       }
       {
         const int len = w.p.s.past + w.p.s.n;
-        bool odd = false;
+        bool high = false;
         for (int c0 = 0; c0 < w.nch && ok; c0 += 4) {
           // Lane (j, i): page i of chunk c0 + j.
           const int i = lane & 7, cj = c0 + (lane >> 3);
@@ -785,7 +785,7 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
           if (E4 && page >= 0) {
             ks = pool.ks[page * pool.kse + w.at.h];
             vs = pool.vs[page * pool.vse + w.at.h];
-            odd |= odd_exp(odd_key(vs));
+            high |= high_scale(vs);
           }
           const int nsl = (keys + kSlice - 1) / kSlice;
           for (int j = 0; j < 4 && c0 + j < w.nch; ++j, ++n) {
@@ -828,7 +828,7 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
               if (mine)
                 for (int q = 0; q < pool.ps / 16; ++q) {
                   sks[(n & 3) * 8 + i * (pool.ps / 16) + q] = ks;
-                  sve[(n & 3) * 8 + i * (pool.ps / 16) + q] = scale_exp(vs);
+                  sve[(n & 3) * 8 + i * (pool.ps / 16) + q] = max(scale_exp(vs), kPagedMinExp);
                 }
               __syncwarp();
               if (lane == 0) mbar_arrive(&sready[n & 3]);
@@ -836,9 +836,9 @@ __global__ void __launch_bounds__(Roles<E4>::kThreads, 1)
           }
         }
         if constexpr (E4) {
-          if (__any_sync(0xffffffffu, odd) && lane == 0) {
+          if (__any_sync(0xffffffffu, high) && lane == 0) {
             if (w.whole) *redo = 1;
-            else cut->odd[w.lo > 0 ? 0 : 1] = 1;
+            else cut->high[w.lo > 0 ? 0 : 1] = 1;
           }
         }
       }
@@ -979,9 +979,10 @@ __global__ void __launch_bounds__(256) paged_extend_join_kernel(const __grid_con
     const RunsE runs(pre[a.batch.B], (int)gridDim.x);
     for (Walk w(a, pre, runs.begin(c), runs.begin(c + 1)); !w.done(); w.next()) {
       if (!w.whole) continue;
+      const bool wide = E4 && wide_row(a, w.p.s.q0 + w.p.s.n - 1, w.at.h);
       for (int i = threadIdx.x >> 5; i < 32; i += 8) {
         const int row = blockIdx.y * 32 + i, r = row % kTile, s_tok = (2 * w.at.j + row / kTile) * tq + r / G;
-        if (r / G < tq && s_tok < w.p.s.n) redo_if_lost<D, E4>(a, w.p.s.q0 + s_tok, w.at.h * G + r % G);
+        if (r / G < tq && s_tok < w.p.s.n) redo_if_lost<D, E4>(a, w.p.s.q0 + s_tok, w.at.h * G + r % G, wide);
       }
     }
   }
@@ -995,7 +996,7 @@ __global__ void __launch_bounds__(256) paged_extend_join_kernel(const __grid_con
   auto piece = [&](int k) {
     return (const float*)a.ws + (size_t)(2 * (c - pieces + 1 + k) + (k == 0 ? 1 : 0)) * partial_floats<D>();
   };
-  bool odd = false;
+  bool high = false;
   float M = -INFINITY, L = 0.f, o[D / 8];
 #pragma unroll
   for (int e = 0; e < D / 8; ++e) o[e] = 0.f;
@@ -1009,7 +1010,7 @@ __global__ void __launch_bounds__(256) paged_extend_join_kernel(const __grid_con
       l[k] = __ldcg(q + 2 * kTile * D + 2 * kTile + row);
       if constexpr (E4) {
         const int i = min(k0 + k, pieces - 1);
-        odd |= __ldcg(&(cut - pieces + 1 + i)->odd[i == 0 ? 1 : 0]) != 0;
+        high |= __ldcg(&(cut - pieces + 1 + i)->high[i == 0 ? 1 : 0]) != 0;
       }
 #pragma unroll
       for (int e = 0; e < D / 32; ++e) v[k][e] = __ldcg(reinterpret_cast<const float4*>(q + (size_t)row * D + d0 + 4 * e));
@@ -1021,8 +1022,8 @@ __global__ void __launch_bounds__(256) paged_extend_join_kernel(const __grid_con
       // see: such a row is computed again below.
       const float top = fmaxf(M, m[k]), keep = M == -INFINITY ? 0.f : ex2(M - top);
       const float f = m[k] == -INFINITY ? 0.f : ex2(m[k] - top);
+      L = add_sum<E4>(add_sum<E4>(0.f, L, M - top, keep), l[k], m[k] - top, f);
       M = top;
-      L = L * keep + f * l[k];
 #pragma unroll
       for (int e = 0; e < D / 32; ++e) {
         o[4 * e] = o[4 * e] * keep + f * v[k][e].x;
@@ -1046,7 +1047,7 @@ __global__ void __launch_bounds__(256) paged_extend_join_kernel(const __grid_con
       *reinterpret_cast<uint4*>(out + 8 * e) = make_uint4(bf16_pair(o[8 * e], o[8 * e + 1]), bf16_pair(o[8 * e + 2], o[8 * e + 3]),
                                                           bf16_pair(o[8 * e + 4], o[8 * e + 5]), bf16_pair(o[8 * e + 6], o[8 * e + 7]));
   }
-  unsigned again = __ballot_sync(0xffffffffu, valid && (bad != 0.f || odd)), nan = __ballot_sync(0xffffffffu, bad != 0.f);
+  unsigned again = __ballot_sync(0xffffffffu, valid && (bad != 0.f || high)), nan = __ballot_sync(0xffffffffu, bad != 0.f);
   while (again) {  // eight lanes are a row
     const int lane = __ffs(again) - 1;
     const unsigned row_lanes = 0xffu << (lane & ~7);

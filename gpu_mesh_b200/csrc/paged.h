@@ -14,7 +14,7 @@ constexpr int kE4M3 = 2;             // cache type, next to kF32 / kBF16
 constexpr int kErrPaged = 4;         // a page id, length or token range outside the pool or the batch
 constexpr int kPagedMaxBatch = 2048; // sequences of one call (the kernels keep a prefix over them in shared memory)
 constexpr int kPagedMinExp = -100;   // least exponent of a page's scale
-constexpr int kPagedMaxExp = 100;    // largest: sums weighed by 2^-e do not overflow (pages far apart: odd_exp in paged_tc.cuh)
+constexpr int kPagedMaxExp = 100;    // largest: sums weighed by 2^-e do not overflow
 constexpr int kPagedMaxTokens = 1 << 26;  // token rows of one call
 constexpr int64_t kPagedMaxLen = 1 << 30; // tokens that a table row may hold: positions stay clear of 32 bits
 

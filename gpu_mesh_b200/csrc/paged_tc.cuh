@@ -65,21 +65,30 @@ __device__ __forceinline__ float ex2(float x) {
 
 // Over e4m3 pages the running maximum m of a row is one of s + e (2^e the scale
 // of the values' page), while its sum l holds Σ 2^(s - m), the keys' own
-// weights.  What lies 2^126 below m vanishes: a key taken as 2^(s + e - m)·2^-e,
-// a sum multiplied by 2^(m_old - m_new).  Either is then below 2^(span - 126) of
-// l, `span` the difference of the row's largest and least e: nothing up to a
-// span of 98 (2^-28).  Beyond (a page of zeros, whose scale is 2^-100, beside
-// values above 112) it can be all of l, and the rows are computed again by
-// redo_row, whose maximum is one of s.  The kernels note whether a piece has met
-// an odd_exp, without which no span exceeds 98; wide_row then looks at the pages.
-constexpr int kSpan = 98;
-// A scale's distance above 2^-49, as a float's exponent field; one below 2^-49
-// wraps around.  A warp keeps the largest of a piece's (in the loop over the
-// keys a flag took 2.3 % more, the longest step at 8 K 209 us against 204).
-__device__ __forceinline__ uint32_t odd_key(float scale) {
-  return (__float_as_uint(scale) & 0x7f800000u) - ((uint32_t)(127 - kSpan / 2) << 23);
+// weights.
+//   * A key is added as 2^(s + e - m + offset)·2^(-e - offset), offset at least
+//     7, of which the first factor vanishes below 2^-126.  The key is then below
+//     2^(span - 133) of l, `span` the difference of the row's largest and least
+//     e: nothing up to a span of 108 (2^-25), but it can be all of l beyond, with
+//     e > 8 on one page and a page of zeros, e = -100, on the other.  Rows that
+//     see so wide a span are computed again by redo_row, whose maximum is one of
+//     s: the kernels note whether a piece has met a scale above 2^8 (values
+//     above 114,688), and wide_row then looks at the sequence's pages.
+//   * l·2^d is taken in two steps, as 2^d alone may vanish where l does not.
+constexpr int kSpan = 108;
+__device__ __forceinline__ bool high_scale(float scale) { return scale > 256.f; }
+static_assert(kSpan + kPagedMinExp == 8, "no wider span without a high scale");
+// L + l·2^d with f = 2^d: a piece's sum joined to those of others.
+template <bool E4>
+__device__ __forceinline__ float add_sum(float L, float l, float d, float f) {
+  if constexpr (E4) {
+    if (d < -64.f) {
+      const float h = ex2(0.5f * d);
+      return L + l * h * h;
+    }
+  }
+  return fmaf(f, l, L);
 }
-__device__ __forceinline__ bool odd_exp(uint32_t key) { return key > (uint32_t)kSpan << 23; }
 
 // Two e4m3 codes (the low half of `codes`) to two halves: exact.
 __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t codes) {
@@ -141,7 +150,7 @@ static __device__ __noinline__ bool wide_row(const PagedAttnArgs& a, int t, int 
   if (b < 0) return false;
   for (int i = threadIdx.x & 31; (int64_t)i * pool.ps < vis; i += 32) {
     const int page = a.batch.table[(int64_t)b * a.batch.ld + i];
-    const int e = page >= 0 && page < pool.pages ? scale_exp(pool.vs[page * pool.vse + h]) : 0;
+    const int e = page >= 0 && page < pool.pages ? max(scale_exp(pool.vs[page * pool.vse + h]), kPagedMinExp) : 0;
     lo = min(lo, e);
     hi = max(hi, e);
   }
@@ -207,13 +216,13 @@ __device__ __noinline__ void redo_row(const PagedAttnArgs& a, int t, int head) {
   for (int i = 0; i < N; ++i) out[lane * N + i] = __float2bfloat16_rn(l == 0.f ? 0.f : acc[i] / l);
 }
 
-// The same for a row that this block has written, if it holds a NaN or sees too wide a span of scales.
+// The same for a row that this block has written, if it holds a NaN or its sequence's scales span too much (`wide`).
 template <int D, bool E4>
-__device__ __forceinline__ void redo_if_lost(const PagedAttnArgs& a, int t, int head) {
+__device__ __forceinline__ void redo_if_lost(const PagedAttnArgs& a, int t, int head, bool wide) {
   const __nv_bfloat16* out = (const __nv_bfloat16*)a.out + (int64_t)t * a.ldo + (int64_t)head * a.hdo;
   bool bad = false;
   for (int d = threadIdx.x & 31; d < D; d += 32) bad |= __hisnan(out[d]);
-  if (__any_sync(0xffffffffu, bad) || (E4 && wide_row(a, t, head / (a.nq / a.pool.nkv)))) redo_row<D, E4>(a, t, head);
+  if (wide || __any_sync(0xffffffffu, bad)) redo_row<D, E4>(a, t, head);
 }
 
 }  // namespace paged
