@@ -21,10 +21,12 @@
 // one token, whose table entries stay in its registers over all heads (eight
 // warps share a token where there are few); its rows are requested before the
 // sequence is looked up.
-// Measured: 24 ragged fp32 chunks (83 MB) 13.7 us = 6.0 TB/s; 8 x 1024 bf16
-// tokens into e4m3 pages (189 MB) 52.7 us = 3.6 TB/s, where issue slots are the
-// bound (60 % active: norm and rotation run twice, once for the page's scale);
-// 32 tokens 5.1 us, one token 3.1 us.
+// Measured: 24 ragged fp32 chunks (83 MB) 13.3 us = 6.2 TB/s; 8 x 1024 bf16
+// tokens into e4m3 pages (189 MB) 52.4 us = 3.6 TB/s, where norm and rotation run
+// twice, once for the page's scale, and registers spill (issue slots 60 % active,
+// DRAM 42 %: neither is full); the same rows into bf16 pages 41.5 us = 5.0 TB/s,
+// fp32 rows into e4m3 pages (357 MB) 81.9 us = 4.4 TB/s; 32 tokens 4.9 us, one
+// token 3.1 us.
 #include <math.h>
 
 #include <algorithm>
@@ -196,9 +198,11 @@ __device__ __forceinline__ float finite_abs(float x) {
 
 // One run of rows, the new tokens of a sequence in one page, for one (head, K
 // or V) of an e4m3 pool, or several where the pages are small, by a whole
-// CTA: the largest magnitude of all rows gives the scale, so the rows stay in
-// registers as they were read and the norm and rotation run twice, which
-// costs less than registers for fp32 rows (they bound the loads in flight).
+// CTA: the largest magnitude of all rows gives the scale, so the rows are held
+// as they were read and the norm and rotation run twice, which takes fewer
+// registers than their results as fp32.  At four CTAs per SM (64 registers) part
+// of the rows is spilled all the same: 216 bytes written and 468 read per thread
+// with bf16 and head_dim 128, 1380 and 3012 with fp32.
 template <typename T, int D>
 struct RunShape {
   static constexpr int RPI = kThreads / Shape<T, D>::LPH;  // rows per round

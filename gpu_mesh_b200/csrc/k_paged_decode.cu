@@ -35,7 +35,7 @@
 //
 // Measured (32 query, 8 KV heads of 128): 64 tokens on 7.9 to 8.2 K positions,
 // e4m3, 204 us = 5.2 TB/s; 32 tokens, bf16, 182 us = 5.8 TB/s (a copy runs at
-// 6.5); 32 tokens on 1 K, e4m3 29 us, bf16 37 us; one token on 130, 8.5 us.
+// 6.5); 32 tokens on 1 K, e4m3 27 us, bf16 37 us; one token on 130, 8.5 us.
 // The long ones are bound by a warp's way through a block between its
 // requests (issue slots 37 % active, 8 warps per SM), the short ones by their
 // round trips: lengths, page, block, the CTA's join, the second kernel.
@@ -778,7 +778,8 @@ cudaError_t launch_decode(const PagedAttnArgs& a, cudaStream_t s) {
 
 }  // namespace
 
-// Whether this kernel takes the sequences with at most 16 query rows per KV head.
+// Whether the tensor-core kernels take the batch: this one the sequences with at
+// most 16 query rows per KV head, its partner, which needs tensor maps, the others.
 bool paged_decode_applicable(const PagedAttnArgs& a) {
   return a.dtype == kBF16 && (a.pool.D == 64 || a.pool.D == 128) && tc_host::encoder() != nullptr;
 }

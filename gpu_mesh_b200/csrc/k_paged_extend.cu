@@ -44,8 +44,9 @@
 // 4,300 cycles per chunk with two tiles in flight (2,050 of them the
 // exponentials of both; the MMA pipe is 34 to 40 % busy).  Measured: chunks of
 // 700 to 1024 tokens on 5 to 8 K positions (4 sequences, 32 query, 8 KV heads
-// of 128) 411 us over bf16 pages, 830 TFLOP/s, 505 us over e4m3 ones; 8
-// prompts of 801 to 1024 (32 query, 4 KV heads of 64) 120 us.
+// of 128) 410 us over bf16 pages, 830 TFLOP/s, 508 us over e4m3 ones; 8
+// prompts of 801 to 1024 (32 query, 4 KV heads of 64) 117 us.  The softmax warps
+// use all 96 registers of a thread and spill 120 to 210 bytes.
 // Slower were steps of 64 keys with the next scores under the softmax (655 us
 // for the bf16 chunks: twice the issue and barrier work per key), an issuing
 // warp per tile (503 us), one softmax thread per row (553 us).

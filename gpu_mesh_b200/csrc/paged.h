@@ -81,8 +81,9 @@ size_t paged_attention_workspace(const PagedAttnArgs& a);
 // Tensor-core kernel for the sequences with at most kPagedFewRows query rows
 // ((token, head) pairs) per KV head (k_paged_decode.cu): it reads the cache
 // once for two tiles of 8 rows, the kernel for more rows computes 128-row
-// tiles however few they hold (16 sequences of up to 5 K, 4 heads per KV head,
-// e4m3: 4 tokens each 50 us here, 5 tokens each 106 us there).
+// tiles however few they hold (16 sequences on 17 to 5,000 positions, 4 heads
+// per KV head, e4m3, pages of 16: exactly 4 tokens each 50 us here, 5 tokens
+// each 91 us there).
 constexpr int kPagedFewRows = 16;
 bool paged_decode_applicable(const PagedAttnArgs& a);
 size_t paged_decode_workspace(const PagedAttnArgs& a);

@@ -414,7 +414,10 @@ typedef struct mg_paged_attention_args {
  * num_q_heads / num_kv_heads (at most 16) query heads per KV head (at most
  * 65535 in all).  The s-th
  * of n new tokens sees the keys j <= kv_len - n + s; a row without any gives
- * 0; an infinity or a NaN reaches the rows that see it alone.  q and out do
+ * 0; an infinity or a NaN reaches the rows that see it, and those alone, however
+ * little its key weighs.  bf16 queries over e4m3 pages: a key whose weight times
+ * its values' scale lies below 2^-31 of the row's largest may count for nothing in
+ * the output (its weight counts in the softmax's sum all the same).  q and out do
  * not overlap.  `workspace` (device
  * memory, 256-byte aligned, mg_paged_attention_workspace bytes) belongs to
  * the call until it has run on `stream`; it needs no initialisation. */
